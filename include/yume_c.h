@@ -296,6 +296,76 @@ yl_status yl_adam_multi(yl_ctx* ctx, const yl_adam_tensor* table, int count, flo
                         float b2, float eps, int t, float grad_scale, float clip_max_norm,
                         int sanitize, float* norm_out_dev);
 
+/* LayerNorm over the last axis of `rows` rows of `cols` floats (ldx, ldy, ...
+ * are row strides in floats, at least cols): the rows of a Linear's input, or
+ * the channels of every pixel of an NHWC activation.  The reference's Swift
+ * path has none; its PyTorch prototype normalises transformer rows this way
+ * (src/diffusion.py:12-35).
+ *   mean = sum x / cols, var = sum (x - mean)^2 / cols, r = 1 / sqrt(var + eps),
+ *   y = (x - mean) r gamma + beta     (gamma NULL: 1, beta NULL: 0).
+ * mean_out / rstd_out (rows, optional) receive the statistics for the backward
+ * call.  y may be x itself (same stride); any other overlap is YL_ERR_INVALID.
+ * A row with a NaN or an infinity becomes NaN; other rows do not see it.
+ * Columns past cols in a padded row are neither read nor written. */
+yl_status yl_layernorm_fwd(yl_ctx* ctx, const float* x, long long ldx, long long rows, int cols,
+                           float eps, const float* gamma, const float* beta, float* y,
+                           long long ldy, float* mean_out, float* rstd_out);
+/* Backward, with h = (x - mean) r and t = dy gamma:
+ *   dx = r (t - mean(t) - h mean(t h))  (+ addend when not NULL),
+ *   dgamma = sum over rows of dy h, dbeta = sum over rows of dy (overwritten;
+ *   zero for rows = 0; fixed summation order).
+ * mean and rstd come from the forward call or are both NULL (recomputed with
+ * eps).  dx, dgamma, dbeta may be NULL.  dx may be addend (same stride); it
+ * must not overlap x or dy (YL_ERR_INVALID). */
+yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const float* dy,
+                           long long lddy, long long rows, int cols, float eps, const float* gamma,
+                           const float* mean, const float* rstd, const float* addend,
+                           long long ldadd, float* dx, long long lddx, float* dgamma,
+                           float* dbeta);
+
+/* Newton-Schulz orthogonalisation of `count` matrices (device pointers in a
+ * host table; row strides in floats): X0 = x / (|x|_F + eps), then `steps`
+ * times X <- (a I + b A + c A^2) X with A = X X^T (X^T X A-products on the right
+ * for matrices with more rows than columns), y = X.  coeffs is a host array of
+ * (a, b, c) per step, or NULL for (3.4445, -4.7750, 2.0315) in every step.  All
+ * products carry fp32 accuracy.  Coefficients that let a singular value grow
+ * past 4 are YL_ERR_UNSUPPORTED; sides go to 65536.  y may be x itself (same
+ * stride); any other overlap between a result and another matrix of the table
+ * is YL_ERR_INVALID.  An empty matrix is skipped, a zero matrix gives zeros, and
+ * one with a NaN or an infinity gives NaN and leaves the others alone.
+ * No counterpart in the reference. */
+typedef struct yl_ns_matrix {
+  const float* x;
+  float* y;
+  int rows, cols;
+  long long ldx, ldy;
+} yl_ns_matrix;
+yl_status yl_newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int steps,
+                           const float* coeffs, float eps);
+
+/* One Muon step over a table of weight matrices (contiguous, device), the
+ * matrix counterpart of yl_adam_multi: g' = grad * grad_scale (non-finite
+ * values zeroed when sanitize != 0; scaled by clip_max_norm / norm when
+ * clip_max_norm > 0 and the global L2 norm exceeds it);
+ *   momentum <- mu momentum + g',  u = g' + mu momentum (nesterov) or momentum,
+ *   param <- param (1 - lr weight_decay) - lr scale NS(u)
+ * with NS, steps, coeffs and eps as in yl_newton_schulz.  scale is each matrix's
+ * own factor on lr, e.g. sqrt(max(1, rows / cols)).  norm_out_dev (optional)
+ * receives the pre-clip norm.  Parameters and momenta must not overlap anything
+ * else in the table (YL_ERR_INVALID).  Summation orders are fixed: equal inputs
+ * give equal bits.  No counterpart in the reference. */
+typedef struct yl_muon_tensor {
+  float* param;
+  const float* grad;
+  float* momentum;
+  int rows, cols;
+  float scale;
+} yl_muon_tensor;
+yl_status yl_muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, float lr,
+                        float momentum, int nesterov, float weight_decay, int steps,
+                        const float* coeffs, float eps, float grad_scale, float clip_max_norm,
+                        int sanitize, float* norm_out_dev);
+
 /* VAE latent head (ConvVAEGPU encode tail, split2 + expHalf + randn + fma,
  * GpuSessionOps.swift:472-535): e is (n, 2c, h, w) = [mu | logvar];
  * z = mu + exp(0.5*clamp(logvar,-10,10)) * eps, eps[img][ch][p] =

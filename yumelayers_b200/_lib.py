@@ -40,6 +40,18 @@ class AdamTensor(C.Structure):
                 ("v", C.c_void_p), ("n", C.c_longlong)]
 
 
+class NsMatrix(C.Structure):
+    """``yl_ns_matrix``."""
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("rows", C.c_int), ("cols", C.c_int),
+                ("ldx", C.c_longlong), ("ldy", C.c_longlong)]
+
+
+class MuonTensor(C.Structure):
+    """``yl_muon_tensor``."""
+    _fields_ = [("param", C.c_void_p), ("grad", C.c_void_p), ("momentum", C.c_void_p),
+                ("rows", C.c_int), ("cols", C.c_int), ("scale", C.c_float)]
+
+
 class TrainerConfig(C.Structure):
     """``yl_trainer_config``."""
     _fields_ = [("batch", C.c_int), ("height", C.c_int), ("width", C.c_int),
@@ -132,6 +144,10 @@ SIGNATURES: dict[str, list] = {
     "yl_linear_bwd": [P, P, P, P, P, P, P, I, I, I],
     "yl_timestep_embedding": [P, P, I, I, I, P],
     "yl_adam_multi": [P, C.POINTER(AdamTensor), I, F, F, F, F, I, F, F, I, P],
+    "yl_layernorm_fwd": [P, P, LL, LL, I, F, P, P, P, LL, P, P],
+    "yl_layernorm_bwd": [P, P, LL, P, LL, LL, I, F, P, P, P, P, LL, P, LL, P, P],
+    "yl_newton_schulz": [P, C.POINTER(NsMatrix), I, I, C.POINTER(F), F],
+    "yl_muon_multi": [P, C.POINTER(MuonTensor), I, F, F, I, F, I, C.POINTER(F), F, F, F, I, P],
     "yl_vae_latent_head_fwd": [P, P, I, I, I, I, I, I64, P],
     "yl_vae_latent_head_bwd": [P, P, P, I, I, I, I, I, I64, F, P],
     "yl_loss_l1_kl": [P, P, P, SZ, P, I, I, I, I, I, F, P, P],

@@ -77,6 +77,13 @@ struct yl_ctx {
   // C-ABI entry points; 2: GroupNorm statistics partials written by a conv
   void* scratch[3] = {nullptr, nullptr, nullptr};
   size_t scratch_bytes[3] = {0, 0, 0};
+  // workspace of the operators that take theirs through yl::Workspace, with an
+  // event behind its last use and the stream of that use
+  void* work = nullptr;
+  size_t work_bytes = 0;
+  cudaEvent_t work_ev = nullptr;
+  cudaStream_t work_stream = nullptr;
+  bool work_used = false;
 };
 
 namespace yl {
@@ -87,6 +94,44 @@ constexpr int kSchedSlots = 64;
 // Grows with cudaMallocAsync/cudaFreeAsync (stream-ordered, so a buffer
 // still in use by queued work is never reused early).
 yl_status scratch_get(yl_ctx* ctx, size_t bytes, void** out, int slot = 0);
+
+// Makes the context's device current for one call and restores the caller's.
+class DeviceGuard {
+ public:
+  explicit DeviceGuard(int device) {
+    if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+    if (prev_ != device) {
+      status_ = cudaSetDevice(device);
+      restore_ = prev_ >= 0;
+    }
+  }
+  ~DeviceGuard() {
+    if (restore_) cudaSetDevice(prev_);
+  }
+  cudaError_t status() const { return status_; }
+
+ private:
+  int prev_ = -1;
+  bool restore_ = false;
+  cudaError_t status_ = cudaSuccess;
+};
+
+// Temporaries of one operator call.  Outside a stream capture they live in the
+// context's workspace, and a call on another stream than the last one's waits
+// for that call's work first.  Inside a capture they are allocated and freed by
+// nodes of the graph itself, so a graph neither keeps a pointer into the
+// context's workspace (which may grow) nor shares it with another graph.
+class Workspace {
+ public:
+  ~Workspace() { done(); }  // an early return must not leak a graph's allocation
+  yl_status get(yl_ctx* ctx, size_t bytes, char** out);
+  yl_status done();
+
+ private:
+  yl_ctx* ctx_ = nullptr;
+  void* p_ = nullptr;
+  bool captured_ = false;
+};
 
 // Bump allocator over one scratch buffer (256-byte aligned pieces).
 struct ScratchCarver {

@@ -53,6 +53,58 @@ yl_status scratch_get(yl_ctx* ctx, size_t bytes, void** out, int slot) {
   return YL_OK;
 }
 
+yl_status Workspace::get(yl_ctx* ctx, size_t bytes, char** out) {
+  if (bytes == 0) bytes = 256;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  YL_CUDA(cudaStreamIsCapturing(ctx->stream, &cap));
+  if (cap != cudaStreamCaptureStatusNone) {
+    cudaError_t e = cudaMallocAsync(&p_, bytes, ctx->stream);
+    if (e != cudaSuccess) {
+      p_ = nullptr;
+      return set_error(YL_ERR_OOM, "workspace of %zu bytes in a captured graph: %s", bytes,
+                       cudaGetErrorString(e));
+    }
+    ctx_ = ctx;
+    captured_ = true;
+    *out = (char*)p_;
+    return YL_OK;
+  }
+  if (!ctx->work_ev) YL_CUDA(cudaEventCreateWithFlags(&ctx->work_ev, cudaEventDisableTiming));
+  if (ctx->work_used && ctx->work_stream != ctx->stream)
+    YL_CUDA(cudaStreamWaitEvent(ctx->stream, ctx->work_ev, 0));
+  if (bytes > ctx->work_bytes) {
+    if (ctx->work) YL_CUDA(cudaFreeAsync(ctx->work, ctx->stream));
+    ctx->work = nullptr;
+    ctx->work_bytes = 0;
+    const size_t want = bytes + bytes / 8;
+    cudaError_t e = cudaMallocAsync(&ctx->work, want, ctx->stream);
+    if (e != cudaSuccess) {
+      ctx->work = nullptr;
+      cudaGetLastError();
+      return set_error(YL_ERR_OOM, "workspace allocation of %zu bytes failed: %s", want,
+                       cudaGetErrorString(e));
+    }
+    ctx->work_bytes = want;
+  }
+  ctx_ = ctx;
+  *out = (char*)ctx->work;
+  return YL_OK;
+}
+
+yl_status Workspace::done() {
+  if (!ctx_) return YL_OK;
+  yl_ctx* ctx = ctx_;
+  ctx_ = nullptr;
+  if (captured_) {
+    YL_CUDA(cudaFreeAsync(p_, ctx->stream));
+    return YL_OK;
+  }
+  YL_CUDA(cudaEventRecord(ctx->work_ev, ctx->stream));
+  ctx->work_stream = ctx->stream;
+  ctx->work_used = true;
+  return YL_OK;
+}
+
 }  // namespace yl
 
 using namespace yl;
@@ -98,6 +150,12 @@ yl_status yl_ctx_destroy(yl_ctx* ctx) {
   cudaStreamSynchronize(ctx->stream);
   for (int s = 0; s < 3; ++s)
     if (ctx->scratch[s]) cudaFreeAsync(ctx->scratch[s], ctx->stream);
+  if (ctx->work) {
+    cudaEventSynchronize(ctx->work_ev);  // its last use may be on another stream
+    cudaFreeAsync(ctx->work, ctx->own_stream);
+    cudaStreamSynchronize(ctx->own_stream);
+  }
+  if (ctx->work_ev) cudaEventDestroy(ctx->work_ev);
   cudaStreamSynchronize(ctx->stream);
   cudaFree(ctx->dev_err);
   cudaFree(ctx->sched);

@@ -11,7 +11,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import LAYOUT_NCHW, AdamTensor, ConvDesc, call
+from ._lib import LAYOUT_NCHW, AdamTensor, ConvDesc, MuonTensor, NsMatrix, call
 from .session import Context, GPUTensor
 
 
@@ -151,6 +151,95 @@ def adam_multi(params, grads, ms, vs, lr, t, b1=0.9, b2=0.999, eps=1e-8, grad_sc
     sizes = [int(np.asarray(p).size) for p in params]
     out = [[d.toArray()[:s] for d, s in zip(dev[k], sizes)] for k in (0, 2, 3)]
     return out[0], out[1], out[2], float(nd.toArray()[0])
+
+
+def layernorm_fwd(x, gamma=None, beta=None, eps=1e-5, ctx: Context | None = None):
+    """LayerNorm over the last axis of x [..., cols] -> (y, mean, rstd); the
+    statistics have x's shape without its last axis."""
+    ctx = ctx or Context.shared()
+    x = np.asarray(x, np.float32)
+    cols = x.shape[-1]
+    rows = x.size // cols
+    xd = _dev(ctx, x)
+    gd = _dev(ctx, gamma) if gamma is not None else None
+    bd = _dev(ctx, beta) if beta is not None else None
+    yd, md, rd = _out(ctx, x.size), _out(ctx, rows), _out(ctx, rows)
+    call("yl_layernorm_fwd", ctx.handle, _ptr(xd), cols, rows, cols, float(eps), _ptr(gd),
+         _ptr(bd), _ptr(yd), cols, _ptr(md), _ptr(rd))
+    return (yd.toArray()[: x.size].reshape(x.shape), md.toArray()[:rows].reshape(x.shape[:-1]),
+            rd.toArray()[:rows].reshape(x.shape[:-1]))
+
+
+def layernorm_bwd(x, dy, gamma=None, eps=1e-5, mean=None, rstd=None, addend=None,
+                  ctx: Context | None = None):
+    """Gradients (dx, dgamma, dbeta) of layernorm_fwd; mean and rstd from the
+    forward call, or both None."""
+    ctx = ctx or Context.shared()
+    x = np.asarray(x, np.float32)
+    cols = x.shape[-1]
+    rows = x.size // cols
+    if np.shape(dy) != x.shape or (addend is not None and np.shape(addend) != x.shape):
+        raise ValueError(f"layernorm_bwd: dy and addend must have x's shape {x.shape}")
+    xd, dyd = _dev(ctx, x), _dev(ctx, dy)
+    gd, md, rd, ad = (_dev(ctx, a) if a is not None else None
+                      for a in (gamma, mean, rstd, addend))
+    dxd, dgd, dbd = _out(ctx, x.size), _out(ctx, cols), _out(ctx, cols)
+    call("yl_layernorm_bwd", ctx.handle, _ptr(xd), cols, _ptr(dyd), cols, rows, cols, float(eps),
+         _ptr(gd), _ptr(md), _ptr(rd), _ptr(ad), cols if addend is not None else 0, _ptr(dxd),
+         cols, _ptr(dgd), _ptr(dbd))
+    return dxd.toArray()[: x.size].reshape(x.shape), dgd.toArray()[:cols], dbd.toArray()[:cols]
+
+
+def _coeffs(coeffs, steps):
+    if coeffs is None:
+        return None
+    a = np.asarray(coeffs, np.float32).reshape(-1)
+    if a.size != 3 * steps:
+        raise ValueError(f"{a.size} coefficients for {steps} steps (three per step)")
+    return (C.c_float * a.size)(*a.tolist())
+
+
+def newton_schulz(matrices, steps=5, coeffs=None, eps=1e-7, ctx: Context | None = None):
+    """Newton-Schulz orthogonalisation of each 2-D array -> list of arrays."""
+    ctx = ctx or Context.shared()
+    shapes = [np.shape(m) for m in matrices]
+    xd = [_dev(ctx, m) for m in matrices]
+    yd = [_out(ctx, r * c) for r, c in shapes]
+    table = (NsMatrix * len(shapes))(*[NsMatrix(x.ptr, y.ptr, r, c, c, c)
+                                       for x, y, (r, c) in zip(xd, yd, shapes)])
+    call("yl_newton_schulz", ctx.handle, table, len(shapes), int(steps), _coeffs(coeffs, steps),
+         float(eps))
+    return [y.toArray()[: r * c].reshape(r, c) for y, (r, c) in zip(yd, shapes)]
+
+
+def muon_scale(rows: int, cols: int) -> float:
+    """sqrt(max(1, rows / cols)): a factor on lr that gives the update of a tall
+    matrix the root-mean-square gain of a square one's."""
+    return float(max(1.0, rows / cols) ** 0.5)
+
+
+def muon_multi(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0,
+               steps=5, coeffs=None, eps=1e-7, grad_scale=1.0, clip_max_norm=0.0, sanitize=False,
+               scales=None, ctx: Context | None = None):
+    """Runs one Muon step on 2-D arrays; returns (params, momenta, norm) as numpy.
+    scales: each matrix's factor on lr (None: muon_scale of its shape)."""
+    ctx = ctx or Context.shared()
+    shapes = [np.shape(p) for p in params]
+    for group in (grads, momenta):
+        if [np.shape(a) for a in group] != shapes:
+            raise ValueError("muon_multi: gradients and momenta must have the parameters' shapes")
+    pd, gd, md = ([_dev(ctx, a) for a in group] for group in (params, grads, momenta))
+    scales = [muon_scale(*s) for s in shapes] if scales is None else scales
+    table = (MuonTensor * len(shapes))(*[
+        MuonTensor(p.ptr, g.ptr, m.ptr, r, c, float(k))
+        for p, g, m, (r, c), k in zip(pd, gd, md, shapes, scales)])
+    nd = _out(ctx, 1)
+    call("yl_muon_multi", ctx.handle, table, len(shapes), float(lr), float(momentum),
+         int(bool(nesterov)), float(weight_decay), int(steps), _coeffs(coeffs, steps), float(eps),
+         float(grad_scale), float(clip_max_norm), int(bool(sanitize)), _ptr(nd))
+    return ([d.toArray()[: r * c].reshape(r, c) for d, (r, c) in zip(pd, shapes)],
+            [d.toArray()[: r * c].reshape(r, c) for d, (r, c) in zip(md, shapes)],
+            float(nd.toArray()[0]))
 
 
 def vae_latent_head_fwd(e, step, ctx: Context | None = None) -> np.ndarray:

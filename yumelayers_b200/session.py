@@ -14,7 +14,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import BINARY, UNARY, YumeError, call, lib
+from ._lib import BINARY, UNARY, MuonTensor, NsMatrix, YumeError, call, lib
 
 _CTX: dict[int, "Context"] = {}
 
@@ -225,6 +225,30 @@ class GpuSession:
              groups)
         return out
 
+    def layerNorm(self, A, gamma=None, beta=None, eps=1e-5) -> GPUTensor:  # noqa: N802
+        """LayerNorm of every row of A (no counterpart in the reference's GpuSession)."""
+        out = self._new(A.rows, A.cols)
+        self._row_vectors("layerNorm", A, gamma, beta)
+        call("yl_layernorm_fwd", self.ctx.handle, A.ptr, A.cols, A.rows, A.cols, float(eps),
+             gamma.ptr if gamma else None, beta.ptr if beta else None, out.ptr, A.cols, None, None)
+        return out
+
+    def encodeLayerNormGrad(self, x, dy, gamma=None, eps=1e-5):  # noqa: N802
+        """(dx, dgamma, dbeta) of layerNorm."""
+        self._same(x, dy, "encodeLayerNormGrad")
+        self._row_vectors("encodeLayerNormGrad", x, gamma)
+        dx, dg, db = self._new(x.rows, x.cols), self._new(1, x.cols), self._new(1, x.cols)
+        call("yl_layernorm_bwd", self.ctx.handle, x.ptr, x.cols, dy.ptr, x.cols, x.rows, x.cols,
+             float(eps), gamma.ptr if gamma else None, None, None, None, 0, dx.ptr, x.cols, dg.ptr,
+             db.ptr)
+        return dx, dg, db
+
+    @staticmethod
+    def _row_vectors(what: str, A: GPUTensor, *vectors) -> None:
+        for v in vectors:
+            if v is not None and v.n != A.cols:
+                raise YumeError(1, f"{what}: a vector of {v.n} for rows of {A.cols}")
+
     # -- elementwise --
     def _unary(self, op, A) -> GPUTensor:
         out = self._new(A.rows, A.cols)
@@ -328,6 +352,23 @@ class GpuSession:
         return dmu, dlv
 
     # -- optimiser --
+    def orthogonalize(self, A, steps=5, eps=1e-7) -> GPUTensor:
+        """Newton-Schulz orthogonalisation of A (yl_newton_schulz)."""
+        out = self._new(A.rows, A.cols)
+        table = (NsMatrix * 1)(NsMatrix(A.ptr, out.ptr, A.rows, A.cols, A.cols, A.cols))
+        call("yl_newton_schulz", self.ctx.handle, table, 1, int(steps), None, float(eps))
+        return out
+
+    def muonUpdate(self, param, grad, momentum, lr, mu=0.95, nesterov=True,  # noqa: N802
+                   weight_decay=0.0, scale=1.0) -> None:
+        """One Muon step of one weight matrix, in place (yl_muon_multi)."""
+        self._same(param, grad, "muonUpdate")
+        self._same(param, momentum, "muonUpdate")
+        table = (MuonTensor * 1)(MuonTensor(param.ptr, grad.ptr, momentum.ptr, param.rows,
+                                            param.cols, float(scale)))
+        call("yl_muon_multi", self.ctx.handle, table, 1, float(lr), float(mu), int(bool(nesterov)),
+             float(weight_decay), 5, None, 1e-7, 1.0, 0.0, 0, None)
+
     def adamUpdate(self, param, grad, m, v, t, lr) -> None:  # noqa: N802
         call("yl_adam_update", self.ctx.handle, param.ptr, grad.ptr, m.ptr, v.ptr, param.n,
              int(t), float(lr))
