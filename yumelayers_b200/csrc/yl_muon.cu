@@ -8,37 +8,65 @@
 //   orthonormal rows (or columns).
 //   Muon: m <- mu m + g', u = g' + mu m (Nesterov) or m,
 //   p <- p (1 - lr decay) - lr scale NS(u).
+#include <cuda_fp16.h>
+
 #include <algorithm>
 #include <cmath>
+#include <memory>
 #include <new>
 #include <vector>
 
 #include "yl_internal.h"
 #include "yl_muon.h"
+#include "yl_ptx.cuh"
 #include "yume_c.h"
 
 namespace yl {
 namespace {
 
-constexpr int kMaxItems = 64;    // matrices of one launch (their table is a kernel argument)
+constexpr int kMaxSteps = 32;
+// Largest singular value the iteration may reach on the way.
+constexpr double kMaxSigma = 4.0;
+constexpr int kMaxItems = 64;      // matrices of one launch's table
 constexpr int kNormChunk = 16384;  // elements of one partial of a Frobenius norm
-constexpr int kTile = 64;
+
+// ---------------------------------------------------------------- data layout
+// X, A and P live in the workspace as fp16 pairs: value * scale = hi + lo with
+// hi the value rounded to fp16 and lo the rest rounded to fp16, 22 bits in all.
+// A product of two pairs is hi hi + hi lo + lo hi, accumulated in fp32 on the
+// tensor cores: as exact as an fp32 product (the dropped lo lo term is 2^-22 of
+// a product), at a third of the fp16 rate, where the tf32 rate is half of it
+// with 11 bits.  The scales are powers of two, per step, that keep the largest
+// value the iteration can reach under fp16's range.
+//
+// Each plane (hi, lo) is a grid of 64 x 64 blocks of 8 KB whose bytes are
+// already in the 128-byte-swizzled order the tensor core reads: 64 rows of 128
+// bytes, 16-byte chunk j of row r at position j ^ (r & 7).  A block loads with
+// one untiled bulk copy, needs no tensor map, and serves as a K-major or an
+// MN-major operand alike, so tall matrices (X^T X on the left, X P) run from the
+// same row-major blocks as wide ones (X X^T, P X) and nothing is transposed.
+// Rows and columns past a matrix's edge are zeros inside its blocks.
+constexpr int kBlk = 64;
+constexpr int kBlkBytes = kBlk * kBlk * 2;
 
 struct Item {
-  const float* src;   // NS: x; Muon: the gradient
-  float* mom;         // Muon: momentum, contiguous
-  float* dst;         // NS: y; Muon: the parameter
+  const float* src;  // NS: x; Muon: the gradient
+  float* mom;        // Muon: momentum, contiguous
+  float* dst;        // NS: y; Muon: the parameter
   long long lds, ldd;
   int rows, cols;
   float scale;
-  int m, n;           // shorter and longer side
-  float *x0, *x1, *a, *p;  // workspace: [m][n], [m][n], [m][m], [m][m]
-  double* part;       // partial sums of squares
+  int rb, cb, mb;       // blocks of the rows, the columns and the shorter side
+  uint8_t *x[2], *a, *p;  // workspace: pairs of planes (X before and after a step, A, P)
+  double* part;         // partial sums of squares
   int chunks;
 };
-struct Pack {
+enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
+struct Table {
   Item it[kMaxItems];
-  int start[kMaxItems + 1];  // blocks of the launch before each item
+  int tiles[3][kMaxItems + 1];  // GRAM, SQUARE, UPDATE tiles before each item
+  int blocks[kMaxItems + 1];    // 64 x 64 blocks of X before each item
+  int chunks[kMaxItems + 1];    // norm chunks before each item
   int count;
 };
 struct Update {
@@ -47,10 +75,14 @@ struct Update {
   const float* norm;
 };
 
-__device__ __forceinline__ int find_item(const Pack& p, int block) {
-  int k = 0;
-  while (k + 1 < p.count && p.start[k + 1] <= block) ++k;
-  return k;
+__device__ __forceinline__ int find_item(const int* start, int count, int t) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (start[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
 }
 
 __device__ __forceinline__ float clean(float g, const Update& u, float clipf) {
@@ -62,8 +94,16 @@ __device__ __forceinline__ float clip_factor(const Update& u) {
   if (u.clip > 0.f && u.norm && *u.norm > u.clip) return u.clip / *u.norm;
   return 1.f;
 }
+// What is orthogonalised: x itself, or the momentum (with Nesterov's look ahead).
+__device__ __forceinline__ float update_value(const Item& it, const Update& u, float clipf,
+                                              long long r, long long c) {
+  if (!u.muon) return it.src[r * it.lds + c];
+  const long long i = r * it.cols + c;
+  const float m = it.mom[i];
+  return u.nesterov ? clean(it.src[i], u, clipf) + u.mu * m : m;
+}
 
-// Sum over a block of 256 threads in a fixed order (valid in thread 0).
+// Sum over a block of 256 threads in a fixed order, the same in every thread.
 __device__ __forceinline__ double block_sum256(double s) {
   __shared__ double red[8];
 #pragma unroll
@@ -71,22 +111,30 @@ __device__ __forceinline__ double block_sum256(double s) {
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
   double t = 0;
-  if (threadIdx.x == 0)
-    for (int w = 0; w < 8; ++w) t += red[w];
+#pragma unroll
+  for (int w = 0; w < 8; ++w) t += red[w];
   return t;
 }
 
-// The momentum step and the partial sums of squares of u.
-__global__ void ns_norm_kernel(const __grid_constant__ Pack p, const __grid_constant__ Update u) {
-  const int k = find_item(p, blockIdx.x);
-  const Item& it = p.it[k];
-  const int chunk = blockIdx.x - p.start[k];
+// The momentum step and the partial sums of squares of u; block 0 also leaves
+// the table in device memory for the kernels that follow.
+__global__ void __launch_bounds__(256)
+    ns_norm_kernel(const __grid_constant__ Table t, const __grid_constant__ Update u,
+                   Table* table_out) {
+  if (blockIdx.x == 0) {
+    const int* s = reinterpret_cast<const int*>(&t);
+    int* d = reinterpret_cast<int*>(table_out);
+    for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += 256) d[i] = s[i];
+  }
+  const int k = find_item(t.chunks, t.count, blockIdx.x);
+  const Item& it = t.it[k];
+  const int chunk = blockIdx.x - t.chunks[k];
   const long long total = (long long)it.rows * it.cols;
   const long long lo = (long long)chunk * kNormChunk;
   const long long hi = min(total, lo + (long long)kNormChunk);
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   double s = 0.0;
-  for (long long i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+  for (long long i = lo + threadIdx.x; i < hi; i += 256) {
     float v;
     if (u.muon) {
       const float g = clean(it.src[i], u, clipf);
@@ -104,12 +152,13 @@ __global__ void ns_norm_kernel(const __grid_constant__ Pack p, const __grid_cons
 }
 
 // part[block] = sum of squares of one chunk of scaled (and sanitized) gradients
-__global__ void grad_square_kernel(const float* __restrict__ g, long long n, float scale,
-                                   int sanitize, double* __restrict__ part) {
+__global__ void __launch_bounds__(256)
+    grad_square_kernel(const float* __restrict__ g, long long n, float scale, int sanitize,
+                       double* __restrict__ part) {
   const long long lo = blockIdx.x * (long long)kNormChunk;
   const long long hi = min(n, lo + (long long)kNormChunk);
   double s = 0.0;
-  for (long long i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+  for (long long i = lo + threadIdx.x; i < hi; i += 256) {
     float v = g[i] * scale;
     if (sanitize && !isfinite(v)) v = 0.f;
     s += (double)v * v;
@@ -117,184 +166,514 @@ __global__ void grad_square_kernel(const float* __restrict__ g, long long n, flo
   s = block_sum256(s);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
-__global__ void grad_norm_final_kernel(const double* __restrict__ part, long long n, float* norm) {
+__global__ void __launch_bounds__(256)
+    grad_norm_final_kernel(const double* __restrict__ part, long long n, float* norm) {
   double s = 0.0;
-  for (long long i = threadIdx.x; i < n; i += blockDim.x) s += part[i];
+  for (long long i = threadIdx.x; i < n; i += 256) s += part[i];
   s = block_sum256(s);
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// X0 = u / (|u| + eps), transposed when the rows are the longer side.
-__global__ void ns_scale_kernel(const __grid_constant__ Pack p, const __grid_constant__ Update u) {
-  const int k = find_item(p, blockIdx.x);
-  const Item& it = p.it[k];
-  const int chunk = blockIdx.x - p.start[k];
+// 1 / (|u|_F + eps) from the item's partials.
+__device__ __forceinline__ float inverse_norm(const Item& it, float eps) {
   double s = 0.0;
-  for (int c = 0; c < it.chunks; ++c) s += it.part[c];
-  const float inv = (float)(1.0 / (sqrt(s) + (double)u.eps));
-  const long long total = (long long)it.rows * it.cols;
-  const long long lo = (long long)chunk * kNormChunk;
-  const long long hi = min(total, lo + (long long)kNormChunk);
-  const float clipf = u.muon ? clip_factor(u) : 1.f;
-  for (long long i = lo + threadIdx.x; i < hi; i += blockDim.x) {
-    const long long r = i / it.cols, c = i - r * it.cols;
-    float v;
-    if (u.muon) {
-      v = it.mom[i];
-      if (u.nesterov) v = clean(it.src[i], u, clipf) + u.mu * v;
-    } else {
-      v = it.src[r * it.lds + c];
-    }
-    it.x0[it.rows > it.cols ? c * it.n + r : i] = v * inv;
-  }
+  for (int c = threadIdx.x; c < it.chunks; c += 256) s += it.part[c];
+  return (float)(1.0 / (sqrt(block_sum256(s)) + (double)eps));
 }
 
-enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
+__device__ __forceinline__ void split_pair(float v, __half* hi, __half* lo) {
+  *hi = __float2half_rn(v);
+  *lo = __float2half_rn(v - __half2float(*hi));
+}
 
-// One 64 x 64 tile of A = X X^T, P = a I + b A + c A A or X' = P X.
-template <int MODE>
+// X0 = u / (|u| + eps) as fp16 pairs, one 64 x 64 block per thread block; each
+// thread fills two 16-byte chunks of either plane.
 __global__ void __launch_bounds__(256)
-    ns_product_kernel(const __grid_constant__ Pack p, float a, float b, float c, int flip) {
-  const int k = find_item(p, blockIdx.x);
-  const Item& it = p.it[k];
-  const int m = it.m, N = MODE == UPDATE ? it.n : m, K = MODE == GRAM ? it.n : m;
-  const int tn = (N + kTile - 1) / kTile;
-  const int t = blockIdx.x - p.start[k];
-  const int r0 = (t / tn) * kTile, c0 = (t % tn) * kTile;
-  const float* x = flip ? it.x1 : it.x0;
-  const float* L = MODE == GRAM ? x : MODE == SQUARE ? it.a : it.p;
-  const float* R = MODE == SQUARE ? it.a : x;
-  float* out = MODE == GRAM ? it.a : MODE == SQUARE ? it.p : (flip ? it.x0 : it.x1);
-  const int ldl = MODE == GRAM ? it.n : m, ldr = MODE == SQUARE ? m : it.n;
-  __shared__ float sl[16][kTile + 1], sr[16][kTile + 1];
-  const int ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += 16) {
-    for (int e = threadIdx.x; e < 16 * kTile; e += 256) {
-      const int kk = e % 16, r = e / 16;
-      sl[kk][r] = (r0 + r < m && k0 + kk < K) ? L[(long long)(r0 + r) * ldl + k0 + kk] : 0.f;
-      if (MODE == GRAM) {
-        sr[kk][r] = (c0 + r < N && k0 + kk < K) ? R[(long long)(c0 + r) * ldr + k0 + kk] : 0.f;
-      } else {
-        const int cc = e % kTile, kr = e / kTile;
-        sr[kr][cc] = (c0 + cc < N && k0 + kr < K) ? R[(long long)(k0 + kr) * ldr + c0 + cc] : 0.f;
-      }
+    ns_split_kernel(const Table* __restrict__ t, const __grid_constant__ Update u, float sx) {
+  const int k = find_item(t->blocks, t->count, blockIdx.x);
+  const Item& it = t->it[k];
+  const int b = blockIdx.x - t->blocks[k];
+  const int rb = b / it.cb, cb = b - rb * it.cb;
+  const float inv = inverse_norm(it, u.eps);
+  const float clipf = u.muon ? clip_factor(u) : 1.f;
+  uint8_t* hi = it.x[0] + (size_t)b * kBlkBytes;
+  uint8_t* lo = hi + (size_t)it.rb * it.cb * kBlkBytes;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int idx = threadIdx.x + 256 * e, row = idx >> 3, ch = idx & 7;
+    const long long r = (long long)rb * kBlk + row, c0 = (long long)cb * kBlk + ch * 8;
+    __align__(16) __half h[8], l[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float v =
+          r < it.rows && c0 + j < it.cols ? update_value(it, u, clipf, r, c0 + j) * inv : 0.f;
+      split_pair(v * sx, &h[j], &l[j]);
     }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sl[kk][ty * 4 + i], sr[kk][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+    const int at = row * 128 + ((ch ^ (row & 7)) << 4);
+    *reinterpret_cast<uint4*>(hi + at) = *reinterpret_cast<const uint4*>(h);
+    *reinterpret_cast<uint4*>(lo + at) = *reinterpret_cast<const uint4*>(l);
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + ty * 4 + i, cc = c0 + tx * 4 + j;
-      if (r >= m || cc >= N) continue;
-      const long long o = (long long)r * N + cc;
-      out[o] = MODE == SQUARE ? (r == cc ? a : 0.f) + b * it.a[o] + c * acc[i][j] : acc[i][j];
-    }
 }
 
-// y = X, or p <- p (1 - lr decay) - lr scale X.
-__global__ void ns_finish_kernel(const __grid_constant__ Pack p, const __grid_constant__ Update u,
-                                 int flip) {
-  const int k = find_item(p, blockIdx.x);
-  const Item& it = p.it[k];
-  const int chunk = blockIdx.x - p.start[k];
-  const float* x = flip ? it.x1 : it.x0;
+// No step at all: y = X0 (or the update with it).
+__global__ void __launch_bounds__(256)
+    ns_direct_kernel(const Table* __restrict__ t, const __grid_constant__ Update u) {
+  const int k = find_item(t->chunks, t->count, blockIdx.x);
+  const Item& it = t->it[k];
+  const int chunk = blockIdx.x - t->chunks[k];
+  const float inv = inverse_norm(it, u.eps);
+  const float clipf = u.muon ? clip_factor(u) : 1.f;
   const long long total = (long long)it.rows * it.cols;
   const long long lo = (long long)chunk * kNormChunk;
   const long long hi = min(total, lo + (long long)kNormChunk);
-  for (long long i = lo + threadIdx.x; i < hi; i += blockDim.x) {
+  for (long long i = lo + threadIdx.x; i < hi; i += 256) {
     const long long r = i / it.cols, c = i - r * it.cols;
-    const float v = x[it.rows > it.cols ? c * it.n + r : i];
+    const float v = update_value(it, u, clipf, r, c) * inv;
     if (u.muon) it.dst[i] = it.dst[i] * (1.f - u.lr * u.decay) - u.lr * it.scale * v;
     else it.dst[r * it.ldd + c] = v;
   }
 }
 
-// Sizes the items' workspaces, or (with a base address) places them; returns
-// the bytes they take.
-size_t place(Item* items, int count, char* ws) {
-  ScratchCarver carve;
-  for (int k = 0; k < count; ++k) {
-    Item& it = items[k];
-    it.m = std::min(it.rows, it.cols);
-    it.n = std::max(it.rows, it.cols);
-    it.chunks = (int)(((long long)it.rows * it.cols + kNormChunk - 1) / kNormChunk);
-    const size_t mn = (size_t)it.m * it.n * 4, mm = (size_t)it.m * it.m * 4;
-    it.x0 = (float*)(ws + carve.take(mn));
-    it.x1 = (float*)(ws + carve.take(mn));
-    it.a = (float*)(ws + carve.take(mm));
-    it.p = (float*)(ws + carve.take(mm));
-    it.part = (double*)(ws + carve.take(it.chunks * sizeof(double)));
+// ---------------------------------------------------------------- products
+// D = L R^T-like products over 128 x 128 tiles, persistent over a tile list:
+//   GRAM    A = X X^T (X^T X for tall matrices), lower tiles, mirrored;
+//   SQUARE  P = a I + b A + c A A, lower tiles, mirrored;
+//   UPDATE  X' = P X (X P), or in the last step the result itself.
+// Warp 4 streams operand blocks (128 x 64 of either side, both planes: 64 KB a
+// stage) through a ring of three stages, warp 5 issues the tcgen05.mma of the
+// three partial products of a k-block into one of four TMEM accumulators, and
+// warps 0-3 add each finished accumulator into registers.
+// The tensor core truncates when it adds to its accumulator: kept there over a
+// whole row, the 384 x 1153 test's result was 2.4e-5 off, where an fp32 product
+// gives 2e-6.  So an accumulator holds one k-block only, its small terms
+// (hi lo, lo hi) first and four additions of hi hi last, and the sum over
+// k-blocks is in registers with fp32's rounding.
+constexpr int kTile = 128;
+constexpr int kStages = 3;
+constexpr int kOpBytes = 2 * kBlkBytes;       // one plane of one operand's 128 x 64
+constexpr int kStageBytes = 4 * kOpBytes;     // L hi, L lo, R hi, R lo
+constexpr int kOutOff = kStages * kStageBytes;
+constexpr int kOutWarp = 8192;                // staging of one epilogue warp
+constexpr int kBarOff = kOutOff + 4 * kOutWarp;
+constexpr int kSmemBytes = kBarOff + 1024 + 1024;  // barriers, alignment
+constexpr int kProductThreads = 192;
+constexpr int kAccs = 4;  // TMEM accumulators of 128 columns
+
+struct Phase {
+  int mode, from, last;  // from: which X buffer is read
+  float c0, c1, c2;      // GRAM, UPDATE: c2 * acc; SQUARE: c0 I + c1 A + c2 * acc
+};
+
+struct TileRef {
+  int item, i, j, nk;
+};
+
+__device__ __forceinline__ TileRef tile_ref(const Table* t, const int* start, int count, int mode,
+                                            int tile) {
+  TileRef q;
+  q.item = find_item(start, count, tile);
+  const Item& it = t->it[q.item];
+  const int k = tile - start[q.item];
+  if (mode == UPDATE) {
+    const int tn = (it.cb + 1) / 2;
+    q.i = k / tn;
+    q.j = k - q.i * tn;
+    q.nk = it.mb;
+  } else {  // lower triangle, row by row: k = i (i + 1) / 2 + j
+    int i = (int)((sqrtf(8.f * k + 1.f) - 1.f) * 0.5f);
+    while (i * (i + 1) / 2 > k) --i;
+    while ((i + 1) * (i + 2) / 2 <= k) ++i;
+    q.i = i;
+    q.j = k - i * (i + 1) / 2;
+    q.nk = mode == SQUARE ? it.mb : (it.rows > it.cols ? it.rb : it.cb);
   }
-  return carve.offset;
+  return q;
 }
 
-yl_status run_pack(yl_ctx* ctx, Pack& p, const Update& u, int steps, const float* coeffs,
-                   char* ws) {
-  place(p.it, p.count, ws);
-  auto starts = [&](auto blocks) {
-    p.start[0] = 0;
-    for (int k = 0; k < p.count; ++k) p.start[k + 1] = p.start[k] + blocks(p.it[k]);
-    return (unsigned)p.start[p.count];
+// One operand: block (mn, k) of a plane is at base + (mn * smn + k * sk) blocks.
+struct Operand {
+  const uint8_t* base;
+  size_t plane;  // bytes from the hi to the lo plane
+  int smn, sk, nmn;
+  int mn_major;
+};
+__device__ __forceinline__ Operand operand(const Item& it, const Phase& ph, int right) {
+  Operand o;
+  const bool tall = it.rows > it.cols;
+  const uint8_t* x = it.x[ph.from];
+  const size_t xp = (size_t)it.rb * it.cb * kBlkBytes, mp = (size_t)it.mb * it.mb * kBlkBytes;
+  if (ph.mode == GRAM) {  // rows of X, or columns when tall
+    o = {x, xp, tall ? 1 : it.cb, tall ? it.cb : 1, it.mb, tall};
+  } else if (ph.mode == SQUARE) {
+    o = {it.a, mp, it.mb, 1, it.mb, 0};
+  } else if (tall != (right != 0)) {  // X's rows (tall, left) or columns (wide, right)
+    o = {x, xp, right ? 1 : it.cb, right ? it.cb : 1, right ? it.cb : it.rb, right};
+  } else {
+    o = {it.p, mp, it.mb, 1, it.mb, 0};
+  }
+  return o;
+}
+
+__global__ void __launch_bounds__(kProductThreads, 1)
+    ns_product_kernel(const Table* __restrict__ t, const __grid_constant__ Phase ph,
+                      const __grid_constant__ Update u, int* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);
+  uint64_t* empty = full + kStages;
+  uint64_t* acc_full = empty + kStages;
+  uint64_t* acc_empty = acc_full + kAccs;
+  uint64_t* drain = acc_empty + kAccs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  int* start = reinterpret_cast<int*>(tmem_slot + 1);  // [kMaxItems + 1]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int count = t->count;
+  for (int i = threadIdx.x; i <= count; i += kProductThreads) start[i] = t->tiles[ph.mode][i];
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < kAccs; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 128);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(tmem_slot, kAccs * kTile);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int n_tiles = start[count];
+  const long long lim = wait_limit(err);
+
+  if (warp == 4) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
+        const TileRef q = tile_ref(t, start, count, ph.mode, tile);
+        const Item& im = t->it[q.item];
+        const Operand L = operand(im, ph, 0), R = operand(im, ph, 1);
+        const int nl = min(2, L.nmn - 2 * q.i), nr = min(2, R.nmn - 2 * q.j);
+        for (int kb = 0; kb < q.nk; ++kb, ++it) {
+          const int s = it % kStages;
+          if (it >= kStages && !mbar_wait(&empty[s], ((it / kStages) - 1) & 1, lim)) {
+            report_error(err, YL_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
+          const uint32_t dst = smem_u32(smem + s * kStageBytes);
+          mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * (nl + nr)) * kBlkBytes);
+          for (int side = 0; side < 2; ++side) {
+            const Operand& o = side ? R : L;
+            const int n = side ? nr : nl, mn0 = 2 * (side ? q.j : q.i);
+            for (int b = 0; b < n; ++b) {
+              const uint8_t* src =
+                  o.base + ((size_t)(mn0 + b) * o.smn + (size_t)kb * o.sk) * kBlkBytes;
+              const uint32_t d = dst + (uint32_t)(side * 2 * kOpBytes + b * kBlkBytes);
+              bulk_load(d, src, kBlkBytes, &full[s]);
+              bulk_load(d + kOpBytes, src + o.plane, kBlkBytes, &full[s]);
+            }
+          }
+        }
+      }
+      drain_ring(full, kStages, it);  // no copy may still be landing when the CTA exits
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
+        const TileRef q = tile_ref(t, start, count, ph.mode, tile);
+        const Item& im = t->it[q.item];
+        const int lmn = operand(im, ph, 0).mn_major, rmn = operand(im, ph, 1).mn_major;
+        const uint32_t idesc = idesc_f16(kTile, kTile, lmn, rmn);
+        // K-major: 16 of a row's 64 k are 32 bytes, 8-row groups 1 KB apart.
+        // MN-major: 16 k are two 8-row groups, 64-column blocks 8 KB apart.
+        const uint32_t lstep = lmn ? 2048 : 32, rstep = rmn ? 2048 : 32;
+        const uint32_t llbo = lmn ? kBlkBytes : 16, rlbo = rmn ? kBlkBytes : 16;
+        for (int kb = 0; kb < q.nk; ++kb, ++it) {
+          const int s = it % kStages, buf = it % kAccs;
+          if ((it >= kAccs && !mbar_wait(&acc_empty[buf], (it / kAccs - 1) & 1, lim)) ||
+              !mbar_wait(&full[s], (it / kStages) & 1, lim)) {
+            report_error(err, YL_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t dacc = tmem + (uint32_t)(buf * kTile);
+          const uint32_t l = smem_u32(smem + s * kStageBytes), r = l + 2 * kOpBytes;
+#pragma unroll
+          for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
+            const uint32_t lp = l + (part == 0 ? kOpBytes : 0), rp = r + (part == 1 ? kOpBytes : 0);
+#pragma unroll
+            for (int kk = 0; kk < kBlk / 16; ++kk)
+              umma_f16(dacc, sw128_desc(lp + kk * lstep, llbo, 1024),
+                       sw128_desc(rp + kk * rstep, rlbo, 1024), idesc, (part | kk) != 0);
+          }
+          umma_commit(&empty[s]);
+          umma_commit(&acc_full[buf]);
+        }
+      }
+      // every MMA this thread issued has completed before TMEM is released
+      umma_commit(drain);
+      mbar_wait(drain, 0);
+    }
+  } else {
+    // epilogue: warp w owns TMEM lanes, that is rows, 32w .. 32w+31 of the tile
+    uint32_t it = 0;
+    bool ok = true;
+    uint8_t* stage = smem + kOutOff + warp * kOutWarp;
+    for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
+      const TileRef q = tile_ref(t, start, count, ph.mode, tile);
+      const Item& im = t->it[q.item];
+      float v[kTile];
+#pragma unroll
+      for (int c = 0; c < kTile; ++c) v[c] = 0.f;
+      for (int kb = 0; kb < q.nk; ++kb, ++it) {
+        const int buf = it % kAccs;
+        if (!mbar_wait(&acc_full[buf], (it / kAccs) & 1, lim)) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(buf * kTile);
+#pragma unroll
+        for (int c0 = 0; c0 < kTile; c0 += 32) {
+          uint32_t acc[32];
+          tmem_ld_32x32b_x32(at + c0, acc);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c0 + c] += __uint_as_float(acc[c]);
+        }
+        tc_fence_before();
+        mbar_arrive(&acc_empty[buf]);
+      }
+      if (!ok) break;
+      const bool sq = ph.mode != UPDATE;
+      const int rbt = sq ? im.mb : im.rb, cbt = sq ? im.mb : im.cb;
+      const int rblk = 2 * q.i + (warp >> 1), r64 = (warp & 1) * 32 + lane;  // row inside its block
+      uint8_t* out = sq ? (ph.mode == GRAM ? im.a : im.p) : im.x[ph.from ^ 1];
+      const size_t plane = (size_t)rbt * cbt * kBlkBytes;
+#pragma unroll
+      for (int slab = 0; slab < 2; ++slab) {
+        const int cblk = 2 * q.j + slab;
+        if (rblk >= rbt || cblk >= cbt) continue;  // uniform in the warp
+        float* w = v + slab * 64;
+#pragma unroll
+        for (int c = 0; c < 64; ++c) w[c] *= ph.c2;
+        if (ph.mode == UPDATE && ph.last) {
+          // 32 rows x 32 columns through shared memory (columns rotated by the
+          // row), then whole row pieces to the result
+          float* st = reinterpret_cast<float*>(stage);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) st[lane * 32 + ((c + lane) & 31)] = w[half * 32 + c];
+            __syncwarp();
+            const long long r0 = (long long)rblk * kBlk + (warp & 1) * 32;
+            const long long col = (long long)cblk * kBlk + half * 32 + lane;
+            if (col < im.cols) {
+              const int nr = (int)min(32LL, im.rows - r0);
+#pragma unroll 4
+              for (int r = 0; r < nr; ++r) {
+                const float x = st[r * 32 + ((lane + r) & 31)];
+                if (u.muon) {
+                  float* d = im.dst + (r0 + r) * im.cols + col;
+                  *d = *d * (1.f - u.lr * u.decay) - u.lr * im.scale * x;
+                } else {
+                  im.dst[(r0 + r) * im.ldd + col] = x;
+                }
+              }
+            }
+          }
+          continue;
+        }
+        const size_t blk = ((size_t)rblk * cbt + cblk) * kBlkBytes;
+        if (ph.mode == SQUARE) {
+          const uint8_t* ah = im.a + blk + r64 * 128;
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) {
+            const int at = (ch ^ (r64 & 7)) << 4;
+            const uint4 h4 = *reinterpret_cast<const uint4*>(ah + at);
+            const uint4 l4 = *reinterpret_cast<const uint4*>(ah + plane + at);
+            const __half* h = reinterpret_cast<const __half*>(&h4);
+            const __half* l = reinterpret_cast<const __half*>(&l4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              w[ch * 8 + j] += ph.c1 * (__half2float(h[j]) + __half2float(l[j]));
+          }
+          if (rblk == cblk) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (r64 == c) w[c] += ph.c0;
+          }
+        }
+        if (lane == 0) bulk_wait_group_read<0>();  // the staging rows are free again
+        __syncwarp();
+        const bool mirror = sq && q.i != q.j;
+        uint8_t* mir = out + ((size_t)cblk * cbt + rblk) * kBlkBytes;
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+          __align__(16) __half h[8], l[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            split_pair(w[ch * 8 + j], &h[j], &l[j]);
+            if (mirror) {
+              const int row = ch * 8 + j;  // row of the mirrored block; its column is r64
+              const int at = row * 128 + (((r64 >> 3) ^ (row & 7)) << 4) + (r64 & 7) * 2;
+              *reinterpret_cast<__half*>(mir + at) = h[j];
+              *reinterpret_cast<__half*>(mir + plane + at) = l[j];
+            }
+          }
+          const int at = lane * 128 + ((ch ^ (r64 & 7)) << 4);
+          *reinterpret_cast<uint4*>(stage + at) = *reinterpret_cast<const uint4*>(h);
+          *reinterpret_cast<uint4*>(stage + 4096 + at) = *reinterpret_cast<const uint4*>(l);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          uint8_t* d = out + blk + (warp & 1) * 4096;
+          bulk_store(d, smem_u32(stage), 4096);
+          bulk_store(d + plane, smem_u32(stage) + 4096, 4096);
+          bulk_commit_group();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kAccs * kTile);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+// Sizes the table's workspace, or (with a base address) places it; returns the
+// bytes it takes.
+size_t place(Table* t, char* ws) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* p = ws + off;
+    off += (bytes + 1023) & ~(size_t)1023;
+    return (uint8_t*)p;
   };
-  auto tiles = [](int v) { return (v + kTile - 1) / kTile; };
-  unsigned grid = starts([](const Item& it) { return it.chunks; });
-  ns_norm_kernel<<<grid, 256, 0, ctx->stream>>>(p, u);
-  YL_TRY(check_launch("ns_norm_kernel"));
-  ns_scale_kernel<<<grid, 256, 0, ctx->stream>>>(p, u);
-  YL_TRY(check_launch("ns_scale_kernel"));
-  int flip = 0;
-  for (int s = 0; s < steps; ++s, flip ^= 1) {
-    const float a = coeffs[3 * s], b = coeffs[3 * s + 1], c = coeffs[3 * s + 2];
-    grid = starts([&](const Item& it) { return tiles(it.m) * tiles(it.m); });
-    ns_product_kernel<GRAM><<<grid, 256, 0, ctx->stream>>>(p, a, b, c, flip);
-    YL_TRY(check_launch("ns_product_kernel"));
-    ns_product_kernel<SQUARE><<<grid, 256, 0, ctx->stream>>>(p, a, b, c, flip);
-    YL_TRY(check_launch("ns_product_kernel"));
-    grid = starts([&](const Item& it) { return tiles(it.m) * tiles(it.n); });
-    ns_product_kernel<UPDATE><<<grid, 256, 0, ctx->stream>>>(p, a, b, c, flip);
-    YL_TRY(check_launch("ns_product_kernel"));
+  take(sizeof(Table));
+  for (int k = 0; k < t->count; ++k) {
+    Item& it = t->it[k];
+    auto blocks = [](int v) { return (v + kBlk - 1) / kBlk; };
+    it.rb = blocks(it.rows);
+    it.cb = blocks(it.cols);
+    it.mb = std::min(it.rb, it.cb);
+    it.chunks = (int)(((long long)it.rows * it.cols + kNormChunk - 1) / kNormChunk);
+    const size_t xb = (size_t)2 * it.rb * it.cb * kBlkBytes;
+    const size_t mb = (size_t)2 * it.mb * it.mb * kBlkBytes;
+    it.x[0] = take(xb);
+    it.x[1] = take(xb);
+    it.a = take(mb);
+    it.p = take(mb);
+    it.part = (double*)take(it.chunks * sizeof(double));
   }
-  grid = starts([](const Item& it) { return it.chunks; });
-  ns_finish_kernel<<<grid, 256, 0, ctx->stream>>>(p, u, flip);
-  return check_launch("ns_finish_kernel");
+  return off;
 }
 
-// All packs of a call, one after the other in the same workspace.
-yl_status run_items(yl_ctx* ctx, std::vector<Item>& items, const Update& u, int steps,
-                    const float* coeffs, char* ws) {
+struct Schedule {
+  int steps;
+  float q[3 * kMaxSteps];    // coefficients
+  float sx[kMaxSteps + 1];   // scales of X before each step and at the end
+  float sa[kMaxSteps], sp[kMaxSteps];
+};
+
+yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, char* ws) {
+  place(&t, ws);
+  auto half_up = [](int v) { return (v + 1) / 2; };
+  for (int m = 0; m < 3; ++m) t.tiles[m][0] = 0;
+  t.blocks[0] = t.chunks[0] = 0;
+  for (int k = 0; k < t.count; ++k) {
+    const Item& it = t.it[k];
+    const int mt = half_up(it.mb);
+    t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + mt * (mt + 1) / 2;
+    t.tiles[SQUARE][k + 1] = t.tiles[SQUARE][k] + mt * (mt + 1) / 2;
+    t.tiles[UPDATE][k + 1] = t.tiles[UPDATE][k] + half_up(it.rb) * half_up(it.cb);
+    t.blocks[k + 1] = t.blocks[k] + it.rb * it.cb;
+    t.chunks[k + 1] = t.chunks[k] + it.chunks;
+  }
+  Table* dt = (Table*)ws;
+  ns_norm_kernel<<<t.chunks[t.count], 256, 0, ctx->stream>>>(t, u, dt);
+  YL_TRY(check_launch("ns_norm_kernel"));
+  if (s.steps == 0) {
+    ns_direct_kernel<<<t.chunks[t.count], 256, 0, ctx->stream>>>(dt, u);
+    return check_launch("ns_direct_kernel");
+  }
+  ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0]);
+  YL_TRY(check_launch("ns_split_kernel"));
+  YL_CUDA(cudaFuncSetAttribute(ns_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kSmemBytes));
+  for (int k = 0; k < s.steps; ++k) {
+    const float a = s.q[3 * k], b = s.q[3 * k + 1], c = s.q[3 * k + 2];
+    const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
+    const bool last = k + 1 == s.steps;
+    Phase ph[3] = {{GRAM, k & 1, 0, 0.f, 0.f, sa / (sx * sx)},
+                   {SQUARE, k & 1, 0, a * sp, b * sp / sa, c * sp / (sa * sa)},
+                   {UPDATE, k & 1, last, 0.f, 0.f, (last ? 1.f : s.sx[k + 1]) / (sp * sx)}};
+    for (const Phase& f : ph) {
+      const int grid = std::min(t.tiles[f.mode][t.count], ctx->num_sms);
+      ns_product_kernel<<<grid, kProductThreads, kSmemBytes, ctx->stream>>>(dt, f, u, ctx->dev_err);
+      YL_TRY(check_launch("ns_product_kernel"));
+    }
+  }
+  return YL_OK;
+}
+
+// All tables of a call, one after the other in the same workspace.
+yl_status run_items(yl_ctx* ctx, std::vector<Item>& items, const Update& u, const Schedule& s,
+                    char* ws) {
+  auto t = std::make_unique<Table>();
   for (size_t base = 0; base < items.size(); base += kMaxItems) {
-    Pack p;
-    p.count = (int)std::min<size_t>(kMaxItems, items.size() - base);
-    std::copy_n(items.begin() + base, p.count, p.it);
-    YL_TRY(run_pack(ctx, p, u, steps, coeffs, ws));
+    t->count = (int)std::min<size_t>(kMaxItems, items.size() - base);
+    std::copy_n(items.begin() + base, t->count, t->it);
+    YL_TRY(run_table(ctx, *t, u, s, ws));
   }
   return YL_OK;
 }
 size_t items_bytes(std::vector<Item>& items) {
   size_t most = 0;
-  for (size_t base = 0; base < items.size(); base += kMaxItems)
-    most = std::max(most, place(items.data() + base,
-                                (int)std::min<size_t>(kMaxItems, items.size() - base), nullptr));
+  auto t = std::make_unique<Table>();
+  for (size_t base = 0; base < items.size(); base += kMaxItems) {
+    t->count = (int)std::min<size_t>(kMaxItems, items.size() - base);
+    std::copy_n(items.begin() + base, t->count, t->it);
+    most = std::max(most, place(t.get(), nullptr));
+  }
   return most;
 }
 
 size_t norm_parts(long long n) { return (size_t)((n + kNormChunk - 1) / kNormChunk); }
 
 constexpr float kQuintic[3] = {3.4445f, -4.7750f, 2.0315f};
-constexpr int kMaxSteps = 32;
-// Largest singular value the iteration may reach on the way.
-constexpr double kMaxSigma = 4.0;
 
-// The coefficients of every step, and whether they keep the singular values
-// (at most 1 at the start) below kMaxSigma.
-yl_status coefficients(const char* who, int steps, const float* given, float* out) {
+// Largest power of two that keeps values up to `top` under fp16's 65504 with
+// room for rounding.
+float scale_for(double top) {
+  int e;
+  std::frexp(32768.0 / std::max(top, 1e-3), &e);
+  return (float)std::ldexp(1.0, std::min(e - 1, 20));
+}
+
+// The coefficients and scales of every step, if the coefficients keep the
+// singular values (at most 1 at the start) below kMaxSigma.
+yl_status plan_steps(const char* who, int steps, const float* given, Schedule* s_out) {
+  float* out = s_out->q;
+  s_out->steps = steps;
   YL_CHECK(steps >= 0 && steps <= kMaxSteps, YL_ERR_INVALID, "%s: %d steps (0 to %d)", who, steps,
            kMaxSteps);
   double top = 1.0;
@@ -325,8 +704,14 @@ yl_status coefficients(const char* who, int steps, const float* given, float* ou
     YL_CHECK(next <= kMaxSigma && inner <= 1024.0, YL_ERR_UNSUPPORTED,
              "%s: the coefficients of step %d let singular values grow to %.3g (at most %.3g)", who,
              s, next, kMaxSigma);
+    // entries of X are bounded by its largest singular value, those of A by its
+    // square, those of P by inner
+    s_out->sx[s] = scale_for(top);
+    s_out->sa[s] = scale_for(top * top);
+    s_out->sp[s] = scale_for(inner);
     top = next;
   }
+  s_out->sx[std::max(steps, 0)] = scale_for(top);
   return YL_OK;
 }
 
@@ -355,8 +740,8 @@ bool rows_overlap(const float* a, long long lda, long long rows_a, long long col
 yl_status newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int steps,
                         const float* coeffs, float eps) {
   const char* who = "yl_newton_schulz";
-  float q[3 * kMaxSteps];
-  YL_TRY(coefficients(who, steps, coeffs, q));
+  Schedule q;
+  YL_TRY(plan_steps(who, steps, coeffs, &q));
   YL_CHECK(eps >= 0.f, YL_ERR_INVALID, "%s: eps %g is negative or NaN", who, (double)eps);
   std::vector<Item> items;
   for (int k = 0; k < count; ++k) {
@@ -390,7 +775,7 @@ yl_status newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int s
   Workspace work;
   char* ws = nullptr;
   YL_TRY(work.get(ctx, items_bytes(items), &ws));
-  YL_TRY(run_items(ctx, items, u, steps, q, ws));
+  YL_TRY(run_items(ctx, items, u, q, ws));
   return work.done();
 }
 
@@ -415,8 +800,8 @@ yl_status grad_norm(yl_ctx* ctx, const float* g, long long n, float grad_scale, 
 yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const MuonStep& st,
                      const float* coeffs, const float* norm, float* norm_out) {
   const char* who = "yl_muon_multi";
-  float q[3 * kMaxSteps];
-  YL_TRY(coefficients(who, st.steps, coeffs, q));
+  Schedule q;
+  YL_TRY(plan_steps(who, st.steps, coeffs, &q));
   YL_CHECK(st.eps >= 0.f, YL_ERR_INVALID, "%s: eps %g is negative or NaN", who, (double)st.eps);
   std::vector<Item> items;
   for (int k = 0; k < count; ++k) {
@@ -459,6 +844,7 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
     for (const Item& it : items) parts += norm_parts((long long)it.rows * it.cols);
   ScratchCarver carve;
   const size_t o_norm = carve.take(sizeof(float)), o_parts = carve.take(parts * sizeof(double));
+  carve.offset = (carve.offset + 1023) & ~(size_t)1023;
   const size_t o_items = carve.take(items_bytes(items));
   Workspace work;
   char* ws = nullptr;
@@ -482,7 +868,7 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
   u.muon = 1, u.nesterov = st.nesterov, u.sanitize = st.sanitize;
   u.mu = st.momentum, u.lr = st.lr, u.decay = st.weight_decay, u.grad_scale = st.grad_scale;
   u.clip = st.clip_max_norm, u.eps = st.eps, u.norm = norm;
-  YL_TRY(run_items(ctx, items, u, st.steps, q, ws + o_items));
+  YL_TRY(run_items(ctx, items, u, q, ws + o_items));
   return work.done();
 }
 
