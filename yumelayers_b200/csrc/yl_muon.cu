@@ -28,7 +28,8 @@ constexpr int kMaxSteps = 32;
 // Largest singular value the iteration may reach on the way.
 constexpr double kMaxSigma = 4.0;
 constexpr int kMaxItems = 64;      // matrices of one launch's table
-constexpr int kNormChunk = 16384;  // elements of one partial of a Frobenius norm
+constexpr int kNormChunk = 4096;   // elements of one partial of a Frobenius norm
+constexpr int kNormParts = 1024;   // most partials of one matrix: larger ones take longer chunks
 
 // ---------------------------------------------------------------- data layout
 // X, A and P live in the workspace as fp16 pairs: value * scale = hi + lo with
@@ -60,15 +61,23 @@ struct Item {
   uint8_t *x[2], *a, *p;  // workspace: pairs of planes (X before and after a step, A, P)
   double* part;         // partial sums of squares
   int chunks;
+  int chunk;            // elements of one partial
+  int vec;              // 16-byte loads of src and mom: 1 everywhere
+  int ks;               // GRAM: shares of the long side, each a ticket of its own
+  int split0;           // its first arrival counter
+  float* partial;       // [GRAM tile][share][column][row] sums of the shares
 };
 enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
 struct Table {
   Item it[kMaxItems];
-  int tiles[3][kMaxItems + 1];  // GRAM, SQUARE, UPDATE tiles before each item
+  int tiles[3][kMaxItems + 1];  // GRAM, SQUARE, UPDATE tickets before each item
   int blocks[kMaxItems + 1];    // 64 x 64 blocks of X before each item
   int chunks[kMaxItems + 1];    // norm chunks before each item
   int count;
+  int* ctrl;                    // ticket counter, done[item][3], arrivals of split GRAM tiles
+  int ctrl_ints;
 };
+constexpr int kCtrlDone = 1, kCtrlSplit = kCtrlDone + 3 * kMaxItems;
 struct Update {
   int muon, nesterov, sanitize;
   float mu, lr, decay, grad_scale, clip, eps;
@@ -125,27 +134,69 @@ __global__ void __launch_bounds__(256)
     const int* s = reinterpret_cast<const int*>(&t);
     int* d = reinterpret_cast<int*>(table_out);
     for (int i = threadIdx.x; i < (int)(sizeof(Table) / 4); i += 256) d[i] = s[i];
+    for (int i = threadIdx.x; i < t.ctrl_ints; i += 256) t.ctrl[i] = 0;
   }
   const int k = find_item(t.chunks, t.count, blockIdx.x);
   const Item& it = t.it[k];
   const int chunk = blockIdx.x - t.chunks[k];
   const long long total = (long long)it.rows * it.cols;
-  const long long lo = (long long)chunk * kNormChunk;
-  const long long hi = min(total, lo + (long long)kNormChunk);
+  const long long lo = (long long)chunk * it.chunk;
+  const int n = (int)min((long long)it.chunk, total - lo);
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   double s = 0.0;
-  for (long long i = lo + threadIdx.x; i < hi; i += 256) {
-    float v;
-    if (u.muon) {
-      const float g = clean(it.src[i], u, clipf);
-      const float m = u.mu * it.mom[i] + g;
-      it.mom[i] = m;
-      v = u.nesterov ? g + u.mu * m : m;
-    } else {
-      const long long r = i / it.cols;
-      v = it.src[r * it.lds + (i - r * it.cols)];
+  if (u.muon) {
+    const float* g = it.src + lo;
+    float* mo = it.mom + lo;
+    auto one = [&](float graw, float& m) {
+      const float gv = clean(graw, u, clipf);
+      m = u.mu * m + gv;
+      const float v = u.nesterov ? gv + u.mu * m : m;
+      s += (double)v * v;
+    };
+    int i = 0;
+    if (it.vec) {
+#pragma unroll 2
+      for (i = threadIdx.x; i < n / 4; i += 256) {
+        const float4 gv = __ldg(reinterpret_cast<const float4*>(g) + i);
+        float4 m = reinterpret_cast<const float4*>(mo)[i];
+        one(gv.x, m.x), one(gv.y, m.y), one(gv.z, m.z), one(gv.w, m.w);
+        reinterpret_cast<float4*>(mo)[i] = m;
+      }
+      i = n & ~3;
     }
-    s += (double)v * v;
+#pragma unroll 4
+    for (i += threadIdx.x; i < n; i += 256) {
+      float m = mo[i];
+      one(__ldg(g + i), m);
+      mo[i] = m;
+    }
+  } else if (it.lds == it.cols) {
+    const float* x = it.src + lo;
+    auto one = [&](float v) { s += (double)v * v; };
+    int i = 0;
+    if (it.vec) {
+#pragma unroll 4
+      for (i = threadIdx.x; i < n / 4; i += 256) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(x) + i);
+        one(v.x), one(v.y), one(v.z), one(v.w);
+      }
+      i = n & ~3;
+    }
+#pragma unroll 4
+    for (i += threadIdx.x; i < n; i += 256) one(__ldg(x + i));
+  } else {  // strided rows: walk (row, column) without a division per element
+    const long long i0 = lo + threadIdx.x;
+    long long r = i0 / it.cols;
+    int c = (int)(i0 - r * it.cols);
+    const int dr = 256 / it.cols, dc = 256 - dr * it.cols;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n; i += 256) {
+      const float v = __ldg(it.src + r * it.lds + c);
+      s += (double)v * v;
+      r += dr;
+      c += dc;
+      if (c >= it.cols) c -= it.cols, ++r;
+    }
   }
   s = block_sum256(s);
   if (threadIdx.x == 0) it.part[chunk] = s;
@@ -202,13 +253,29 @@ __global__ void __launch_bounds__(256)
   for (int e = 0; e < 2; ++e) {
     const int idx = threadIdx.x + 256 * e, row = idx >> 3, ch = idx & 7;
     const long long r = (long long)rb * kBlk + row, c0 = (long long)cb * kBlk + ch * 8;
+    float v[8];
+    if (it.vec && r < it.rows && c0 + 8 <= it.cols) {
+      const float* x = it.src + r * it.lds + c0;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        float4 g = make_float4(0.f, 0.f, 0.f, 0.f), m = g;
+        if (!u.muon || u.nesterov) g = __ldg(reinterpret_cast<const float4*>(x) + q);
+        if (u.muon) m = __ldg(reinterpret_cast<const float4*>(it.mom + r * it.cols + c0) + q);
+        const float ge[4] = {g.x, g.y, g.z, g.w}, me[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          v[4 * q + j] = !u.muon ? ge[j]
+                         : u.nesterov ? clean(ge[j], u, clipf) + u.mu * me[j]
+                                      : me[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = r < it.rows && c0 + j < it.cols ? update_value(it, u, clipf, r, c0 + j) : 0.f;
+    }
     __align__(16) __half h[8], l[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v =
-          r < it.rows && c0 + j < it.cols ? update_value(it, u, clipf, r, c0 + j) * inv : 0.f;
-      split_pair(v * sx, &h[j], &l[j]);
-    }
+    for (int j = 0; j < 8; ++j) split_pair(v[j] * inv * sx, &h[j], &l[j]);
     const int at = row * 128 + ((ch ^ (row & 7)) << 4);
     *reinterpret_cast<uint4*>(hi + at) = *reinterpret_cast<const uint4*>(h);
     *reinterpret_cast<uint4*>(lo + at) = *reinterpret_cast<const uint4*>(l);
@@ -224,8 +291,8 @@ __global__ void __launch_bounds__(256)
   const float inv = inverse_norm(it, u.eps);
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   const long long total = (long long)it.rows * it.cols;
-  const long long lo = (long long)chunk * kNormChunk;
-  const long long hi = min(total, lo + (long long)kNormChunk);
+  const long long lo = (long long)chunk * it.chunk;
+  const long long hi = min(total, lo + (long long)it.chunk);
   for (long long i = lo + threadIdx.x; i < hi; i += 256) {
     const long long r = i / it.cols, c = i - r * it.cols;
     const float v = update_value(it, u, clipf, r, c) * inv;
@@ -235,58 +302,97 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------- products
-// D = L R^T-like products over 128 x 128 tiles, persistent over a tile list:
-//   GRAM    A = X X^T (X^T X for tall matrices), lower tiles, mirrored;
+// All steps of all matrices in one persistent kernel.  Its work is a list of
+// tickets, 128 x 128 tiles of
+//   GRAM    A = X X^T (X^T X for tall matrices), lower tiles, mirrored; the long
+//           side may be split into shares whose sums the last one to finish adds
+//           up in share order;
 //   SQUARE  P = a I + b A + c A A, lower tiles, mirrored;
-//   UPDATE  X' = P X (X P), or in the last step the result itself.
-// Warp 4 streams operand blocks (128 x 64 of either side, both planes: 64 KB a
-// stage) through a ring of three stages, warp 5 issues the tcgen05.mma of the
-// three partial products of a k-block into one of four TMEM accumulators, and
-// warps 0-3 add each finished accumulator into registers.
+//   UPDATE  X' = P X (X P), or in the last step the result itself,
+// step by step, phase by phase, matrix by matrix.  A thread block takes the next
+// ticket from a counter; before it loads a tile it waits until that matrix's
+// tiles of the phase before are done.  Tickets are handed out in an order in
+// which every tile comes after the tiles it needs, and a taken ticket belongs to
+// a running block, so the waits end however many blocks are resident.
+//
+// Warp 8 streams operand blocks (128 x 64 of either side, both planes: 64 KB a
+// stage; half of that on the diagonal, where both sides are the same) through a
+// ring of three stages, warp 9 issues the tcgen05.mma, and warps 0-7 add each
+// finished accumulator into registers (64 columns of 32 rows per warp) and write
+// the tile.
 // The tensor core truncates when it adds to its accumulator: kept there over a
-// whole row, the 384 x 1153 test's result was 2.4e-5 off, where an fp32 product
-// gives 2e-6.  So an accumulator holds one k-block only, its small terms
-// (hi lo, lo hi) first and four additions of hi hi last, and the sum over
-// k-blocks is in registers with fp32's rounding.
+// whole row, a 384 x 1153 matrix ended 2.4e-5 off, where an fp32 product gives
+// 2e-6.  So an accumulator holds 32 terms only, its small ones (hi lo, lo hi)
+// first and two additions of hi hi last, and the sum over the row is in
+// registers with fp32's rounding.
 constexpr int kTile = 128;
 constexpr int kStages = 3;
 constexpr int kOpBytes = 2 * kBlkBytes;       // one plane of one operand's 128 x 64
 constexpr int kStageBytes = 4 * kOpBytes;     // L hi, L lo, R hi, R lo
 constexpr int kOutOff = kStages * kStageBytes;
-constexpr int kOutWarp = 8192;                // staging of one epilogue warp
-constexpr int kBarOff = kOutOff + 4 * kOutWarp;
-constexpr int kSmemBytes = kBarOff + 1024 + 1024;  // barriers, alignment
-constexpr int kProductThreads = 192;
-constexpr int kAccs = 4;  // TMEM accumulators of 128 columns
+constexpr int kOutWarp = 4096;                // staging of one epilogue warp
+constexpr int kEpiWarps = 8;
+constexpr int kBarOff = kOutOff + kEpiWarps * kOutWarp;
+constexpr int kSmemBytes = kBarOff + 1536 + 1024;  // barriers and prefixes, alignment
+constexpr int kProductThreads = (kEpiWarps + 2) * 32;
+constexpr int kAccs = 2;  // k-blocks in TMEM, two accumulators of 128 columns each
+constexpr int kRing = 4;  // tickets on their way from the producer to the other warps
 
-struct Phase {
-  int mode, from, last;  // from: which X buffer is read
-  float c0, c1, c2;      // GRAM, UPDATE: c2 * acc; SQUARE: c0 I + c1 A + c2 * acc
+struct Steps {
+  int n;
+  float g2[kMaxSteps];                                // GRAM: A' = g2 acc
+  float s0[kMaxSteps], s1[kMaxSteps], s2[kMaxSteps];  // SQUARE: P' = s0 I + s1 A' + s2 acc
+  float u2[kMaxSteps];                                // UPDATE: X' = u2 acc
 };
 
-struct TileRef {
-  int item, i, j, nk;
+struct Ticket {
+  int step, mode, item, i, j, kb0, nk, share, tile;
 };
 
-__device__ __forceinline__ TileRef tile_ref(const Table* t, const int* start, int count, int mode,
-                                            int tile) {
-  TileRef q;
-  q.item = find_item(start, count, tile);
+// `start` is the table's tiles[3][kMaxItems + 1] in shared memory.
+__device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, int count, int n) {
+  Ticket q;
+  const int gram = start[count], square = start[kMaxItems + 1 + count];
+  const int per = gram + square + start[2 * (kMaxItems + 1) + count];
+  q.step = n / per;
+  n -= q.step * per;
+  q.mode = GRAM;
+  if (n >= gram) {
+    n -= gram;
+    q.mode = SQUARE;
+    if (n >= square) {
+      n -= square;
+      q.mode = UPDATE;
+    }
+  }
+  const int* st = start + q.mode * (kMaxItems + 1);
+  q.item = find_item(st, count, n);
   const Item& it = t->it[q.item];
-  const int k = tile - start[q.item];
-  if (mode == UPDATE) {
+  int k = n - st[q.item];
+  q.kb0 = 0;
+  q.share = 0;
+  q.nk = it.mb;
+  if (q.mode == UPDATE) {
     const int tn = (it.cb + 1) / 2;
     q.i = k / tn;
     q.j = k - q.i * tn;
-    q.nk = it.mb;
-  } else {  // lower triangle, row by row: k = i (i + 1) / 2 + j
-    int i = (int)((sqrtf(8.f * k + 1.f) - 1.f) * 0.5f);
-    while (i * (i + 1) / 2 > k) --i;
-    while ((i + 1) * (i + 2) / 2 <= k) ++i;
-    q.i = i;
-    q.j = k - i * (i + 1) / 2;
-    q.nk = mode == SQUARE ? it.mb : (it.rows > it.cols ? it.rb : it.cb);
+    q.tile = k;
+    return q;
   }
+  if (q.mode == GRAM) {
+    const int nk = it.rows > it.cols ? it.rb : it.cb, ks = it.ks;
+    q.share = k % ks;
+    k /= ks;
+    q.kb0 = (int)((long long)nk * q.share / ks);
+    q.nk = (int)((long long)nk * (q.share + 1) / ks) - q.kb0;
+  }
+  q.tile = k;
+  // lower triangle, row by row: k = i (i + 1) / 2 + j
+  int i = (int)((sqrtf(8.f * k + 1.f) - 1.f) * 0.5f);
+  while (i * (i + 1) / 2 > k) --i;
+  while ((i + 1) * (i + 2) / 2 <= k) ++i;
+  q.i = i;
+  q.j = k - i * (i + 1) / 2;
   return q;
 }
 
@@ -297,38 +403,64 @@ struct Operand {
   int smn, sk, nmn;
   int mn_major;
 };
-__device__ __forceinline__ Operand operand(const Item& it, const Phase& ph, int right) {
-  Operand o;
+__device__ __forceinline__ Operand operand(const Item& it, int mode, int from, int right) {
   const bool tall = it.rows > it.cols;
-  const uint8_t* x = it.x[ph.from];
+  const uint8_t* x = it.x[from];
   const size_t xp = (size_t)it.rb * it.cb * kBlkBytes, mp = (size_t)it.mb * it.mb * kBlkBytes;
-  if (ph.mode == GRAM) {  // rows of X, or columns when tall
-    o = {x, xp, tall ? 1 : it.cb, tall ? it.cb : 1, it.mb, tall};
-  } else if (ph.mode == SQUARE) {
-    o = {it.a, mp, it.mb, 1, it.mb, 0};
-  } else if (tall != (right != 0)) {  // X's rows (tall, left) or columns (wide, right)
-    o = {x, xp, right ? 1 : it.cb, right ? it.cb : 1, right ? it.cb : it.rb, right};
-  } else {
-    o = {it.p, mp, it.mb, 1, it.mb, 0};
-  }
-  return o;
+  if (mode == GRAM)  // rows of X, or columns when tall
+    return {x, xp, tall ? 1 : it.cb, tall ? it.cb : 1, it.mb, tall};
+  if (mode == SQUARE) return {it.a, mp, it.mb, 1, it.mb, 0};
+  if (tall != (right != 0))  // X's rows (tall, left) or columns (wide, right)
+    return {x, xp, right ? 1 : it.cb, right ? it.cb : 1, right ? it.cb : it.rb, right};
+  return {it.p, mp, it.mb, 1, it.mb, 0};
+}
+
+__device__ __forceinline__ int load_acquire(const int* p) {
+  int v;
+  asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void add_release(int* p, int v) {
+  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async_all() {
+  asm volatile("fence.proxy.async;" ::: "memory");
+}
+__device__ __forceinline__ void epilogue_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+}
+
+// The counter a ticket waits for, and the value it must have reached.
+__device__ __forceinline__ const int* needs(const Table* t, const int* start, const Ticket& q,
+                                            int* value) {
+  const int before = (q.mode + 2) % 3;  // GRAM <- UPDATE of the step before
+  const int* st = start + before * (kMaxItems + 1) + q.item;
+  int tiles = st[1] - st[0];
+  if (before == GRAM) tiles /= t->it[q.item].ks;  // counted once per tile
+  *value = tiles * (q.mode == GRAM ? q.step : q.step + 1);
+  return t->ctrl + kCtrlDone + 3 * q.item + before;
 }
 
 __global__ void __launch_bounds__(kProductThreads, 1)
-    ns_product_kernel(const Table* __restrict__ t, const __grid_constant__ Phase ph,
-                      const __grid_constant__ Update u, int* err) {
+    ns_steps_kernel(const Table* __restrict__ t, const __grid_constant__ Steps steps,
+                    const __grid_constant__ Update u, int* err) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);
   uint64_t* empty = full + kStages;
   uint64_t* acc_full = empty + kStages;
   uint64_t* acc_empty = acc_full + kAccs;
-  uint64_t* drain = acc_empty + kAccs;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  int* start = reinterpret_cast<int*>(tmem_slot + 1);  // [kMaxItems + 1]
+  uint64_t* tfull = acc_empty + kAccs;
+  uint64_t* tempty = tfull + kRing;
+  uint64_t* drain = tempty + kRing;
+  int* ring = reinterpret_cast<int*>(drain + 1);
+  int* last_share = ring + kRing;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last_share + 1);
+  int* start = reinterpret_cast<int*>(tmem_slot + 1);  // [3][kMaxItems + 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = t->count;
-  for (int i = threadIdx.x; i <= count; i += kProductThreads) start[i] = t->tiles[ph.mode][i];
+  for (int i = threadIdx.x; i < 3 * (kMaxItems + 1); i += kProductThreads)
+    start[i] = (&t->tiles[0][0])[i];
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -336,31 +468,59 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     }
     for (int b = 0; b < kAccs; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 128);
+      mbar_init(&acc_empty[b], kEpiWarps);
+    }
+    for (int b = 0; b < kRing; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 1 + kEpiWarps);
     }
     mbar_init(drain, 1);
     fence_barrier_init();
   }
-  if (warp == 5) {
-    tmem_alloc(tmem_slot, kAccs * kTile);
+  if (warp == kEpiWarps + 1) {
+    tmem_alloc(tmem_slot, 2 * kAccs * kTile);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n_tiles = start[count];
+  const int total = steps.n * (start[count] + start[kMaxItems + 1 + count] +
+                               start[2 * (kMaxItems + 1) + count]);
   const long long lim = wait_limit(err);
 
-  if (warp == 4) {
+  if (warp == kEpiWarps) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
-        const TileRef q = tile_ref(t, start, count, ph.mode, tile);
+      int next = atomicAdd(t->ctrl, 1);
+      for (uint32_t k = 0; ok; ++k) {
+        const int n = next, slot = k % kRing;
+        if (k >= kRing && !mbar_wait(&tempty[slot], (k / kRing - 1) & 1, lim)) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+          break;
+        }
+        ring[slot] = n;
+        mbar_arrive(&tfull[slot]);
+        if (n >= total) break;
+        next = atomicAdd(t->ctrl, 1);  // on its way while this tile loads
+        const Ticket q = ticket_of(t, start, count, n);
         const Item& im = t->it[q.item];
-        const Operand L = operand(im, ph, 0), R = operand(im, ph, 1);
-        const int nl = min(2, L.nmn - 2 * q.i), nr = min(2, R.nmn - 2 * q.j);
+        const Operand L = operand(im, q.mode, q.step & 1, 0), R = operand(im, q.mode, q.step & 1, 1);
+        const bool same = q.mode != UPDATE && q.i == q.j;
+        const int nl = min(2, L.nmn - 2 * q.i), nr = same ? 0 : min(2, R.nmn - 2 * q.j);
+        int value;
+        const int* counter = needs(t, start, q, &value);
+        const long long t0 = clock64();
+        while (load_acquire(counter) < value) {
+          if (clock64() - t0 > lim) {
+            report_error(err, YL_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
+        }
+        if (!ok) break;
+        fence_proxy_async_all();  // other blocks' plain stores before this thread's bulk loads
         for (int kb = 0; kb < q.nk; ++kb, ++it) {
           const int s = it % kStages;
           if (it >= kStages && !mbar_wait(&empty[s], ((it / kStages) - 1) & 1, lim)) {
@@ -372,10 +532,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * (nl + nr)) * kBlkBytes);
           for (int side = 0; side < 2; ++side) {
             const Operand& o = side ? R : L;
-            const int n = side ? nr : nl, mn0 = 2 * (side ? q.j : q.i);
-            for (int b = 0; b < n; ++b) {
+            const int nb = side ? nr : nl, mn0 = 2 * (side ? q.j : q.i);
+            for (int b = 0; b < nb; ++b) {
               const uint8_t* src =
-                  o.base + ((size_t)(mn0 + b) * o.smn + (size_t)kb * o.sk) * kBlkBytes;
+                  o.base + ((size_t)(mn0 + b) * o.smn + (size_t)(q.kb0 + kb) * o.sk) * kBlkBytes;
               const uint32_t d = dst + (uint32_t)(side * 2 * kOpBytes + b * kBlkBytes);
               bulk_load(d, src, kBlkBytes, &full[s]);
               bulk_load(d + kOpBytes, src + o.plane, kBlkBytes, &full[s]);
@@ -385,14 +545,23 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
       drain_ring(full, kStages, it);  // no copy may still be landing when the CTA exits
     }
-  } else if (warp == 5) {
+  } else if (warp == kEpiWarps + 1) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
-        const TileRef q = tile_ref(t, start, count, ph.mode, tile);
+      for (uint32_t k = 0; ok; ++k) {
+        const int slot = k % kRing;
+        if (!mbar_wait(&tfull[slot], (k / kRing) & 1, lim)) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+          break;
+        }
+        const int n = ring[slot];
+        mbar_arrive(&tempty[slot]);
+        if (n >= total) break;
+        const Ticket q = ticket_of(t, start, count, n);
         const Item& im = t->it[q.item];
-        const int lmn = operand(im, ph, 0).mn_major, rmn = operand(im, ph, 1).mn_major;
+        const int lmn = operand(im, q.mode, 0, 0).mn_major, rmn = operand(im, q.mode, 0, 1).mn_major;
+        const bool same = q.mode != UPDATE && q.i == q.j;
         const uint32_t idesc = idesc_f16(kTile, kTile, lmn, rmn);
         // K-major: 16 of a row's 64 k are 32 bytes, 8-row groups 1 KB apart.
         // MN-major: 16 k are two 8-row groups, 64-column blocks 8 KB apart.
@@ -407,15 +576,20 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t dacc = tmem + (uint32_t)(buf * kTile);
-          const uint32_t l = smem_u32(smem + s * kStageBytes), r = l + 2 * kOpBytes;
+          const uint32_t l = smem_u32(smem + s * kStageBytes), r = same ? l : l + 2 * kOpBytes;
 #pragma unroll
-          for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
-            const uint32_t lp = l + (part == 0 ? kOpBytes : 0), rp = r + (part == 1 ? kOpBytes : 0);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t dacc = tmem + (uint32_t)((2 * buf + h) * kTile);
 #pragma unroll
-            for (int kk = 0; kk < kBlk / 16; ++kk)
-              umma_f16(dacc, sw128_desc(lp + kk * lstep, llbo, 1024),
-                       sw128_desc(rp + kk * rstep, rlbo, 1024), idesc, (part | kk) != 0);
+            for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
+              const uint32_t lp = l + (part == 0 ? kOpBytes : 0);
+              const uint32_t rp = r + (part == 1 ? kOpBytes : 0);
+#pragma unroll
+              for (int kk = 2 * h; kk < 2 * h + 2; ++kk)
+                umma_f16(dacc, sw128_desc(lp + kk * lstep, llbo, 1024),
+                         sw128_desc(rp + kk * rstep, rlbo, 1024), idesc,
+                         (part | (kk & 1)) != 0);
+            }
           }
           umma_commit(&empty[s]);
           umma_commit(&acc_full[buf]);
@@ -426,16 +600,27 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       mbar_wait(drain, 0);
     }
   } else {
-    // epilogue: warp w owns TMEM lanes, that is rows, 32w .. 32w+31 of the tile
+    // epilogue: warp w owns rows 32 (w % 4) .. + 31 (its TMEM lanes) and columns
+    // 64 (w / 4) .. + 63 of the tile
     uint32_t it = 0;
-    bool ok = true;
     uint8_t* stage = smem + kOutOff + warp * kOutWarp;
-    for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
-      const TileRef q = tile_ref(t, start, count, ph.mode, tile);
+    const int wr = warp & 3, wc = warp >> 2;
+    for (uint32_t k = 0;; ++k) {
+      const int slot = k % kRing;
+      if (!mbar_wait(&tfull[slot], (k / kRing) & 1, lim)) {
+        report_error(err, YL_DEVERR_TIMEOUT);
+        break;
+      }
+      const int n = ring[slot];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[slot]);
+      if (n >= total) break;
+      const Ticket q = ticket_of(t, start, count, n);
       const Item& im = t->it[q.item];
-      float v[kTile];
+      float v[64];
 #pragma unroll
-      for (int c = 0; c < kTile; ++c) v[c] = 0.f;
+      for (int c = 0; c < 64; ++c) v[c] = 0.f;
+      bool ok = true;
       for (int kb = 0; kb < q.nk; ++kb, ++it) {
         const int buf = it % kAccs;
         if (!mbar_wait(&acc_full[buf], (it / kAccs) & 1, lim)) {
@@ -444,124 +629,186 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           break;
         }
         tc_fence_after();
-        const uint32_t at = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(buf * kTile);
+        const uint32_t at =
+            tmem + ((uint32_t)(wr * 32) << 16) + (uint32_t)(2 * buf * kTile + wc * 64);
 #pragma unroll
-        for (int c0 = 0; c0 < kTile; c0 += 32) {
+        for (int p = 0; p < 4; ++p) {  // (accumulator, column half)
           uint32_t acc[32];
-          tmem_ld_32x32b_x32(at + c0, acc);
+          tmem_ld_32x32b_x32(at + (p & 1) * kTile + (p >> 1) * 32, acc);
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[c0 + c] += __uint_as_float(acc[c]);
+          for (int c = 0; c < 32; ++c) v[(p >> 1) * 32 + c] += __uint_as_float(acc[c]);
         }
         tc_fence_before();
-        mbar_arrive(&acc_empty[buf]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[buf]);
       }
       if (!ok) break;
-      const bool sq = ph.mode != UPDATE;
+      if (q.mode == GRAM && im.ks > 1) {
+        // leave this share's sum; the block that finishes a tile's last share adds
+        // them all, in share order whoever that is
+        float* part = im.partial + ((size_t)q.tile * im.ks) * kTile * kTile +
+                      (size_t)(wc * 64) * kTile + wr * 32 + lane;
+        float* mine = part + (size_t)q.share * kTile * kTile;
+#pragma unroll
+        for (int c = 0; c < 64; ++c) __stcg(mine + c * kTile, v[c]);
+        __threadfence();
+        epilogue_sync();
+        if (threadIdx.x == 0) {
+          int* arrivals = t->ctrl + kCtrlSplit + im.split0 + q.tile;
+          const int seen = atomicAdd(arrivals, 1);
+          __threadfence();
+          if (seen == im.ks - 1) atomicExch(arrivals, 0);
+          *last_share = seen == im.ks - 1;
+        }
+        epilogue_sync();
+        const bool mine_is_last = *last_share != 0;
+        epilogue_sync();
+        if (!mine_is_last) continue;
+        __threadfence();
+#pragma unroll
+        for (int c = 0; c < 64; ++c) v[c] = 0.f;
+        for (int sh = 0; sh < im.ks; ++sh) {
+          const float* p = part + (size_t)sh * kTile * kTile;
+#pragma unroll
+          for (int c = 0; c < 64; ++c) v[c] += __ldcg(p + c * kTile);
+        }
+      }
+      const bool sq = q.mode != UPDATE, last = !sq && q.step + 1 == steps.n;
       const int rbt = sq ? im.mb : im.rb, cbt = sq ? im.mb : im.cb;
-      const int rblk = 2 * q.i + (warp >> 1), r64 = (warp & 1) * 32 + lane;  // row inside its block
-      uint8_t* out = sq ? (ph.mode == GRAM ? im.a : im.p) : im.x[ph.from ^ 1];
-      const size_t plane = (size_t)rbt * cbt * kBlkBytes;
+      const int rblk = 2 * q.i + (wr >> 1), r64 = (wr & 1) * 32 + lane;  // row inside its block
+      const int cblk = 2 * q.j + wc;
+      const float c2 = q.mode == GRAM     ? steps.g2[q.step]
+                       : q.mode == SQUARE ? steps.s2[q.step]
+                                          : steps.u2[q.step];
+      const bool inside = rblk < rbt && cblk < cbt;  // uniform in the warp
+      if (inside) {
 #pragma unroll
-      for (int slab = 0; slab < 2; ++slab) {
-        const int cblk = 2 * q.j + slab;
-        if (rblk >= rbt || cblk >= cbt) continue;  // uniform in the warp
-        float* w = v + slab * 64;
+        for (int c = 0; c < 64; ++c) v[c] *= c2;
+      }
+      if (inside && last) {
+        // 32 rows x 32 columns through shared memory (columns rotated by the
+        // row), then whole row pieces to the result
+        float* st = reinterpret_cast<float*>(stage);
 #pragma unroll
-        for (int c = 0; c < 64; ++c) w[c] *= ph.c2;
-        if (ph.mode == UPDATE && ph.last) {
-          // 32 rows x 32 columns through shared memory (columns rotated by the
-          // row), then whole row pieces to the result
-          float* st = reinterpret_cast<float*>(stage);
+        for (int half = 0; half < 2; ++half) {
+          __syncwarp();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            __syncwarp();
+          for (int c = 0; c < 32; ++c) st[lane * 32 + ((c + lane) & 31)] = v[half * 32 + c];
+          __syncwarp();
+          const long long r0 = (long long)rblk * kBlk + (wr & 1) * 32;
+          const long long col = (long long)cblk * kBlk + half * 32 + lane;
+          if (col < im.cols) {
+            const int nr = (int)min(32LL, im.rows - r0);
+            float* d = im.dst + r0 * im.ldd + col;
+#pragma unroll 1
+            for (int r1 = 0; r1 < nr; r1 += 16) {
+              float pv[16];  // the parameter's rows are all on their way before the first is used
+              if (u.muon) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) st[lane * 32 + ((c + lane) & 31)] = w[half * 32 + c];
-            __syncwarp();
-            const long long r0 = (long long)rblk * kBlk + (warp & 1) * 32;
-            const long long col = (long long)cblk * kBlk + half * 32 + lane;
-            if (col < im.cols) {
-              const int nr = (int)min(32LL, im.rows - r0);
-#pragma unroll 4
-              for (int r = 0; r < nr; ++r) {
-                const float x = st[r * 32 + ((lane + r) & 31)];
-                if (u.muon) {
-                  float* d = im.dst + (r0 + r) * im.cols + col;
-                  *d = *d * (1.f - u.lr * u.decay) - u.lr * im.scale * x;
-                } else {
-                  im.dst[(r0 + r) * im.ldd + col] = x;
-                }
+                for (int r = 0; r < 16; ++r)
+                  pv[r] = r1 + r < nr ? __ldcs(d + (r1 + r) * im.ldd) : 0.f;
+              }
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                float x = st[(r1 + r) * 32 + ((lane + r1 + r) & 31)];
+                if (u.muon) x = pv[r] * (1.f - u.lr * u.decay) - u.lr * im.scale * x;
+                if (r1 + r < nr) __stcs(d + (r1 + r) * im.ldd, x);
               }
             }
           }
-          continue;
         }
+      }
+      if (last) continue;  // nothing waits for the results
+      if (inside) {
+        uint8_t* out = sq ? (q.mode == GRAM ? im.a : im.p) : im.x[(q.step & 1) ^ 1];
+        const size_t plane = (size_t)rbt * cbt * kBlkBytes;
         const size_t blk = ((size_t)rblk * cbt + cblk) * kBlkBytes;
-        if (ph.mode == SQUARE) {
+        if (q.mode == SQUARE) {
+          int value;
+          load_acquire(needs(t, start, q, &value));  // reached already; orders the reads of A
+          const float s1 = steps.s1[q.step], s0 = steps.s0[q.step];
           const uint8_t* ah = im.a + blk + r64 * 128;
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
             const int at = (ch ^ (r64 & 7)) << 4;
-            const uint4 h4 = *reinterpret_cast<const uint4*>(ah + at);
-            const uint4 l4 = *reinterpret_cast<const uint4*>(ah + plane + at);
-            const __half* h = reinterpret_cast<const __half*>(&h4);
-            const __half* l = reinterpret_cast<const __half*>(&l4);
+            const uint4 h4 = __ldcg(reinterpret_cast<const uint4*>(ah + at));
+            const uint4 l4 = __ldcg(reinterpret_cast<const uint4*>(ah + plane + at));
+            const __half2* h = reinterpret_cast<const __half2*>(&h4);
+            const __half2* l = reinterpret_cast<const __half2*>(&l4);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              w[ch * 8 + j] += ph.c1 * (__half2float(h[j]) + __half2float(l[j]));
+            for (int j = 0; j < 4; ++j) {
+              const float2 hf = __half22float2(h[j]), lf = __half22float2(l[j]);
+              v[ch * 8 + 2 * j] += s1 * (hf.x + lf.x);
+              v[ch * 8 + 2 * j + 1] += s1 * (hf.y + lf.y);
+            }
           }
           if (rblk == cblk) {
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              if (r64 == c) w[c] += ph.c0;
+              if (r64 == c) v[c] += s0;
           }
         }
-        if (lane == 0) bulk_wait_group_read<0>();  // the staging rows are free again
-        __syncwarp();
         const bool mirror = sq && q.i != q.j;
         uint8_t* mir = out + ((size_t)cblk * cbt + rblk) * kBlkBytes;
 #pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-          __align__(16) __half h[8], l[8];
+        for (int pl = 0; pl < 2; ++pl) {  // hi plane, then what is left of v as the lo plane
+          if (lane == 0) bulk_wait_group_read<0>();  // the staging rows are free again
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            split_pair(w[ch * 8 + j], &h[j], &l[j]);
-            if (mirror) {
-              const int row = ch * 8 + j;  // row of the mirrored block; its column is r64
-              const int at = row * 128 + (((r64 >> 3) ^ (row & 7)) << 4) + (r64 & 7) * 2;
-              *reinterpret_cast<__half*>(mir + at) = h[j];
-              *reinterpret_cast<__half*>(mir + plane + at) = l[j];
+          for (int ch = 0; ch < 8; ++ch) {
+            __align__(16) __half2 h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float* w = v + ch * 8 + 2 * j;
+              h[j] = __floats2half2_rn(w[0], w[1]);
+              if (pl == 0) {
+                const float2 f = __half22float2(h[j]);
+                w[0] -= f.x;
+                w[1] -= f.y;
+              }
+              if (mirror) {
+                const int row = ch * 8 + 2 * j;  // rows of the mirrored block; its column is r64
+                const int at = (r64 & 7) * 2;
+                *reinterpret_cast<__half*>(mir + pl * plane + row * 128 +
+                                           (((r64 >> 3) ^ (row & 7)) << 4) + at) = __low2half(h[j]);
+                *reinterpret_cast<__half*>(mir + pl * plane + (row + 1) * 128 +
+                                           (((r64 >> 3) ^ ((row + 1) & 7)) << 4) + at) =
+                    __high2half(h[j]);
+              }
             }
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((ch ^ (r64 & 7)) << 4)) =
+                *reinterpret_cast<const uint4*>(h);
           }
-          const int at = lane * 128 + ((ch ^ (r64 & 7)) << 4);
-          *reinterpret_cast<uint4*>(stage + at) = *reinterpret_cast<const uint4*>(h);
-          *reinterpret_cast<uint4*>(stage + 4096 + at) = *reinterpret_cast<const uint4*>(l);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            bulk_store(out + blk + pl * plane + (wr & 1) * 4096, smem_u32(stage), 4096);
+            bulk_commit_group();
+          }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          uint8_t* d = out + blk + (warp & 1) * 4096;
-          bulk_store(d, smem_u32(stage), 4096);
-          bulk_store(d + plane, smem_u32(stage) + 4096, 4096);
-          bulk_commit_group();
-        }
+        if (lane == 0) bulk_wait_group_all();
       }
+      // everything this block wrote of the tile is in memory before the count says so
+      fence_proxy_async_all();
+      __threadfence();
+      epilogue_sync();
+      if (threadIdx.x == 0) add_release(t->ctrl + kCtrlDone + 3 * q.item + q.mode, 1);
     }
     if (lane == 0) bulk_wait_group_all();
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == kEpiWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, kAccs * kTile);
+    tmem_dealloc(tmem, 2 * kAccs * kTile);
   }
 }
 
 // ---------------------------------------------------------------- host side
 // Sizes the table's workspace, or (with a base address) places it; returns the
 // bytes it takes.
-size_t place(Table* t, char* ws) {
+size_t place(Table* t, int num_sms, char* ws) {
   size_t off = 0;
   auto take = [&](size_t bytes) {
     char* p = ws + off;
@@ -575,7 +822,10 @@ size_t place(Table* t, char* ws) {
     it.rb = blocks(it.rows);
     it.cb = blocks(it.cols);
     it.mb = std::min(it.rb, it.cb);
-    it.chunks = (int)(((long long)it.rows * it.cols + kNormChunk - 1) / kNormChunk);
+    const long long n = (long long)it.rows * it.cols;
+    it.chunk = (int)((n / kNormParts + kNormChunk) / kNormChunk * kNormChunk);
+    it.chunks = (int)((n + it.chunk - 1) / it.chunk);
+    it.vec = !(((uintptr_t)it.src | (uintptr_t)it.mom | (uintptr_t)(it.lds * 4)) & 15);
     const size_t xb = (size_t)2 * it.rb * it.cb * kBlkBytes;
     const size_t mb = (size_t)2 * it.mb * it.mb * kBlkBytes;
     it.x[0] = take(xb);
@@ -584,6 +834,31 @@ size_t place(Table* t, char* ws) {
     it.p = take(mb);
     it.part = (double*)take(it.chunks * sizeof(double));
   }
+  // Shares of GRAM's long side: as many as bring its tickets down to the average
+  // per SM, and at most sqrt(nk / 2), where the sums' way through memory costs as
+  // much as the k-blocks it saves (about 0.6 us a share against 0.4 us a k-block).
+  auto nk = [](const Item& it) { return std::max(it.rb, it.cb); };
+  auto gram_tiles = [](const Item& it) {
+    const int mt = (it.mb + 1) / 2;
+    return mt * (mt + 1) / 2;
+  };
+  double kb = 0;
+  for (int k = 0; k < t->count; ++k) kb += (double)gram_tiles(t->it[k]) * nk(t->it[k]);
+  const double fair = kb / num_sms;
+  int splits = 0;
+  for (int k = 0; k < t->count; ++k) {
+    Item& it = t->it[k];
+    const double most = std::min(std::round(nk(it) / std::max(fair, 1.0)), std::sqrt(nk(it) / 2.0));
+    it.ks = std::max(1, (int)most);
+    it.split0 = splits;
+    it.partial = nullptr;
+    if (it.ks > 1) {
+      splits += gram_tiles(it);
+      it.partial = (float*)take((size_t)gram_tiles(it) * it.ks * kTile * kTile * sizeof(float));
+    }
+  }
+  t->ctrl_ints = kCtrlSplit + splits;
+  t->ctrl = (int*)take(t->ctrl_ints * sizeof(int));
   return off;
 }
 
@@ -595,14 +870,14 @@ struct Schedule {
 };
 
 yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, char* ws) {
-  place(&t, ws);
+  place(&t, ctx->num_sms, ws);
   auto half_up = [](int v) { return (v + 1) / 2; };
   for (int m = 0; m < 3; ++m) t.tiles[m][0] = 0;
   t.blocks[0] = t.chunks[0] = 0;
   for (int k = 0; k < t.count; ++k) {
     const Item& it = t.it[k];
     const int mt = half_up(it.mb);
-    t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + mt * (mt + 1) / 2;
+    t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + mt * (mt + 1) / 2 * it.ks;
     t.tiles[SQUARE][k + 1] = t.tiles[SQUARE][k] + mt * (mt + 1) / 2;
     t.tiles[UPDATE][k + 1] = t.tiles[UPDATE][k] + half_up(it.rb) * half_up(it.cb);
     t.blocks[k + 1] = t.blocks[k] + it.rb * it.cb;
@@ -617,22 +892,22 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   }
   ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0]);
   YL_TRY(check_launch("ns_split_kernel"));
-  YL_CUDA(cudaFuncSetAttribute(ns_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  YL_CUDA(cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kSmemBytes));
+  Steps st;
+  st.n = s.steps;
   for (int k = 0; k < s.steps; ++k) {
-    const float a = s.q[3 * k], b = s.q[3 * k + 1], c = s.q[3 * k + 2];
     const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
-    const bool last = k + 1 == s.steps;
-    Phase ph[3] = {{GRAM, k & 1, 0, 0.f, 0.f, sa / (sx * sx)},
-                   {SQUARE, k & 1, 0, a * sp, b * sp / sa, c * sp / (sa * sa)},
-                   {UPDATE, k & 1, last, 0.f, 0.f, (last ? 1.f : s.sx[k + 1]) / (sp * sx)}};
-    for (const Phase& f : ph) {
-      const int grid = std::min(t.tiles[f.mode][t.count], ctx->num_sms);
-      ns_product_kernel<<<grid, kProductThreads, kSmemBytes, ctx->stream>>>(dt, f, u, ctx->dev_err);
-      YL_TRY(check_launch("ns_product_kernel"));
-    }
+    st.g2[k] = sa / (sx * sx);
+    st.s0[k] = s.q[3 * k] * sp;
+    st.s1[k] = s.q[3 * k + 1] * sp / sa;
+    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa);
+    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx);
   }
-  return YL_OK;
+  const int widest = std::max(t.tiles[GRAM][t.count], t.tiles[UPDATE][t.count]);
+  ns_steps_kernel<<<std::min(widest, ctx->num_sms), kProductThreads, kSmemBytes, ctx->stream>>>(
+      dt, st, u, ctx->dev_err);
+  return check_launch("ns_steps_kernel");
 }
 
 // All tables of a call, one after the other in the same workspace.
@@ -646,13 +921,13 @@ yl_status run_items(yl_ctx* ctx, std::vector<Item>& items, const Update& u, cons
   }
   return YL_OK;
 }
-size_t items_bytes(std::vector<Item>& items) {
+size_t items_bytes(yl_ctx* ctx, std::vector<Item>& items) {
   size_t most = 0;
   auto t = std::make_unique<Table>();
   for (size_t base = 0; base < items.size(); base += kMaxItems) {
     t->count = (int)std::min<size_t>(kMaxItems, items.size() - base);
     std::copy_n(items.begin() + base, t->count, t->it);
-    most = std::max(most, place(t.get(), nullptr));
+    most = std::max(most, place(t.get(), ctx->num_sms, nullptr));
   }
   return most;
 }
@@ -774,7 +1049,7 @@ yl_status newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int s
   u.eps = eps;
   Workspace work;
   char* ws = nullptr;
-  YL_TRY(work.get(ctx, items_bytes(items), &ws));
+  YL_TRY(work.get(ctx, items_bytes(ctx, items), &ws));
   YL_TRY(run_items(ctx, items, u, q, ws));
   return work.done();
 }
@@ -845,7 +1120,7 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
   ScratchCarver carve;
   const size_t o_norm = carve.take(sizeof(float)), o_parts = carve.take(parts * sizeof(double));
   carve.offset = (carve.offset + 1023) & ~(size_t)1023;
-  const size_t o_items = carve.take(items_bytes(items));
+  const size_t o_items = carve.take(items_bytes(ctx, items));
   Workspace work;
   char* ws = nullptr;
   YL_TRY(work.get(ctx, carve.offset, &ws));
