@@ -421,7 +421,7 @@ __device__ __forceinline__ int load_acquire(const int* p) {
   return v;
 }
 __device__ __forceinline__ void add_release(int* p, int v) {
-  asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+  asm volatile("fence.acq_rel.gpu; red.relaxed.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
 __device__ __forceinline__ void fence_proxy_async_all() {
   asm volatile("fence.proxy.async;" ::: "memory");
@@ -631,13 +631,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         tc_fence_after();
         const uint32_t at =
             tmem + ((uint32_t)(wr * 32) << 16) + (uint32_t)(2 * buf * kTile + wc * 64);
+        // (accumulator, column half) p: the next read runs while this one is added
+        uint32_t acc[2][32];
+        tmem_ld_32x32b_x32(at, acc[0]);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {  // (accumulator, column half)
-          uint32_t acc[32];
-          tmem_ld_32x32b_x32(at + (p & 1) * kTile + (p >> 1) * 32, acc);
+        for (int p = 0; p < 4; ++p) {
           tmem_ld_wait();
+          if (p < 3) tmem_ld_32x32b_x32(at + ((p + 1) & 1) * kTile + ((p + 1) >> 1) * 32, acc[(p + 1) & 1]);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[(p >> 1) * 32 + c] += __uint_as_float(acc[c]);
+          for (int c = 0; c < 32; ++c) v[(p >> 1) * 32 + c] += __uint_as_float(acc[p & 1][c]);
         }
         tc_fence_before();
         __syncwarp();
@@ -652,20 +654,16 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         float* mine = part + (size_t)q.share * kTile * kTile;
 #pragma unroll
         for (int c = 0; c < 64; ++c) __stcg(mine + c * kTile, v[c]);
-        __threadfence();
         epilogue_sync();
         if (threadIdx.x == 0) {
-          int* arrivals = t->ctrl + kCtrlSplit + im.split0 + q.tile;
-          const int seen = atomicAdd(arrivals, 1);
+          __threadfence();  // with the barrier: all of the block's stores
+          const int seen = atomicAdd(t->ctrl + kCtrlSplit + im.split0 + q.tile, 1);
           __threadfence();
-          if (seen == im.ks - 1) atomicExch(arrivals, 0);
-          *last_share = seen == im.ks - 1;
+          *last_share = seen == im.ks * (q.step + 1) - 1;
         }
         epilogue_sync();
         const bool mine_is_last = *last_share != 0;
-        epilogue_sync();
-        if (!mine_is_last) continue;
-        __threadfence();
+        if (!mine_is_last) continue;  // thread 0 writes the flag again only behind a barrier
 #pragma unroll
         for (int c = 0; c < 64; ++c) v[c] = 0.f;
         for (int sh = 0; sh < im.ks; ++sh) {
@@ -790,8 +788,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         if (lane == 0) bulk_wait_group_all();
       }
       // everything this block wrote of the tile is in memory before the count says so
-      fence_proxy_async_all();
-      __threadfence();
+      if (sq && q.i != q.j) fence_proxy_async_all();  // the mirrored blocks' plain stores
       epilogue_sync();
       if (threadIdx.x == 0) add_release(t->ctrl + kCtrlDone + 3 * q.item + q.mode, 1);
     }
