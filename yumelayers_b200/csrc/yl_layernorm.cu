@@ -385,8 +385,8 @@ __device__ __forceinline__ void flush_groups(const Bwd& p, long long part, int l
   for (int k = 0; k < PER; ++k) dg[k] = db[k] = 0.f;
 }
 
-template <int THREADS, int LANES, int PER, int D>
-__global__ void __launch_bounds__(THREADS) ln_bwd_ring_kernel(const __grid_constant__ Bwd p) {
+template <int THREADS, int LANES, int PER, int D, int MIN_BLOCKS>
+__global__ void __launch_bounds__(THREADS, MIN_BLOCKS) ln_bwd_ring_kernel(const __grid_constant__ Bwd p) {
   using R = Row<LANES, PER, true>;
   using Q = Ring<THREADS, LANES, PER, 3, D>;
   extern __shared__ __align__(16) uint8_t ring[];
@@ -660,23 +660,23 @@ auto fwd_plain(int cols, F f) {
   if (cols <= 16384) return f(ln_fwd_block_kernel<1024, 16, false>, 1024, 1, 1, 0);
   return f(ln_fwd_long_kernel, kLong, 1, 1, 0);
 }
-template <int THREADS, int LANES, int PER, int D, class F>
+template <int THREADS, int LANES, int PER, int D, int MIN_BLOCKS, class F>
 auto bwd_ring(F f) {
-  return f(ln_bwd_ring_kernel<THREADS, LANES, PER, D>, THREADS, THREADS / LANES, 1,
+  return f(ln_bwd_ring_kernel<THREADS, LANES, PER, D, MIN_BLOCKS>, THREADS, THREADS / LANES, 1,
            Ring<THREADS, LANES, PER, 3, D>::kBytes);
 }
 template <class F>
 auto bwd_aligned(int cols, F f) {
-  if (cols <= 16) return bwd_ring<256, 4, 4, 3>(f);
-  if (cols <= 32) return bwd_ring<256, 4, 8, 2>(f);
-  if (cols <= 64) return bwd_ring<256, 8, 8, 2>(f);
-  if (cols <= 128) return bwd_ring<256, 16, 8, 2>(f);
-  if (cols <= 256) return bwd_ring<256, 32, 8, 2>(f);
-  if (cols <= 512) return bwd_ring<256, 32, 16, 2>(f);
-  if (cols <= 1024) return bwd_ring<256, 256, 4, 3>(f);
-  if (cols <= 2048) return bwd_ring<256, 256, 8, 2>(f);
-  if (cols <= 4096) return bwd_ring<512, 512, 8, 2>(f);
-  if (cols <= 8192) return bwd_ring<1024, 1024, 8, 2>(f);
+  if (cols <= 16) return bwd_ring<256, 4, 4, 3, 4>(f);
+  if (cols <= 32) return bwd_ring<256, 4, 8, 2, 3>(f);
+  if (cols <= 64) return bwd_ring<256, 8, 8, 2, 3>(f);
+  if (cols <= 128) return bwd_ring<256, 16, 8, 2, 3>(f);
+  if (cols <= 256) return bwd_ring<256, 32, 8, 2, 3>(f);
+  if (cols <= 512) return bwd_ring<256, 32, 16, 2, 2>(f);
+  if (cols <= 1024) return bwd_ring<256, 256, 4, 3, 4>(f);
+  if (cols <= 2048) return bwd_ring<256, 256, 8, 2, 3>(f);
+  if (cols <= 4096) return bwd_ring<512, 512, 8, 2, 2>(f);
+  if (cols <= 8192) return bwd_ring<1024, 1024, 8, 2, 1>(f);
   return f(ln_bwd_long_kernel, kLong, 1, 1, 0);
 }
 template <class F>
@@ -694,14 +694,15 @@ auto bwd_plain(int cols, F f) {
   return f(ln_bwd_long_kernel, kLong, 1, 1, 0);
 }
 
-// Resident blocks of a kernel on the whole device.
+// Limits a grid to the kernel's resident blocks on the whole device.
 template <class K>
 yl_status resident(yl_ctx* ctx, K kernel, int threads, int smem, long long* blocks) {
-  int per = 0;
-  if (smem > 48 * 1024 - 4096)
+  if (smem > 40 * 1024)
     YL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (*blocks <= ctx->num_sms) return YL_OK;
+  int per = 0;
   YL_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, threads, smem));
-  *blocks = (long long)std::max(per, 1) * ctx->num_sms;
+  *blocks = std::min(*blocks, (long long)std::max(per, 1) * ctx->num_sms);
   return YL_OK;
 }
 
@@ -738,9 +739,8 @@ yl_status yl_layernorm_fwd(yl_ctx* ctx, const float* x, long long ldx, long long
   const bool vec = aligned16(x) && aligned16(y) && aligned16(gamma) && aligned16(beta) &&
                    ((ldx | ldy | cols) & 3) == 0;
   auto launch = [&](auto kernel, int threads, int rows_a_block, int, int smem) -> yl_status {
-    long long most = 0;
-    YL_TRY(resident(ctx, kernel, threads, smem, &most));
-    const long long blocks = std::min((rows + rows_a_block - 1) / rows_a_block, most);
+    long long blocks = (rows + rows_a_block - 1) / rows_a_block;
+    YL_TRY(resident(ctx, kernel, threads, smem, &blocks));
     kernel<<<(unsigned)blocks, threads, smem, ctx->stream>>>(p);
     return check_launch("ln_fwd_kernel");
   };
@@ -782,9 +782,8 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
                    aligned16(dx) &&
                    ((ldx | lddy | cols | (p.addend ? ldadd : 0) | (dx ? lddx : 0)) & 3) == 0;
   auto launch = [&](auto kernel, int threads, int rows_a_block, int unr, int smem) -> yl_status {
-    long long most = 0;
-    YL_TRY(resident(ctx, kernel, threads, smem, &most));
-    const long long blocks = std::min((rows + rows_a_block - 1) / rows_a_block, most);
+    long long blocks = (rows + rows_a_block - 1) / rows_a_block;
+    YL_TRY(resident(ctx, kernel, threads, smem, &blocks));
     Workspace work;
     // rows a thread adds up per turn, turns per partial row, partial rows of a block
     const long long turns = (rows + blocks * rows_a_block - 1) / (blocks * rows_a_block);
