@@ -68,12 +68,14 @@ struct Item {
   float* partial;       // [GRAM tile][share][column][row] sums of the shares
 };
 enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
+constexpr int kPairSide = 128;
 struct Table {
   Item it[kMaxItems];
   int tiles[3][kMaxItems + 1];  // GRAM, SQUARE, UPDATE tickets before each item
   int blocks[kMaxItems + 1];    // 64 x 64 blocks of X before each item
   int chunks[kMaxItems + 1];    // norm chunks before each item
   int count;
+  int pair;                     // worked on by pairs of blocks, 256 x 256 tiles
   int* ctrl;                    // ticket counter, done[item][3], arrivals of split GRAM tiles
   int ctrl_ints;
 };
@@ -304,10 +306,10 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------- products
 // All steps of all matrices in one persistent kernel.  Its work is a list of
 // tickets, 128 x 128 tiles of
-//   GRAM    A = X X^T (X^T X for tall matrices), lower tiles, mirrored; the long
-//           side may be split into shares whose sums the last one to finish adds
-//           up in share order;
-//   SQUARE  P = a I + b A + c A A, lower tiles, mirrored;
+//   GRAM    A = X X^T (X^T X for tall matrices), tiles on and below the diagonal;
+//           the long side may be split into shares whose sums the last one to
+//           finish adds up in share order;
+//   SQUARE  P = a I + b A + c A A, tiles on and below the diagonal;
 //   UPDATE  X' = P X (X P), or in the last step the result itself,
 // step by step, phase by phase, matrix by matrix.  A thread block takes the next
 // ticket from a counter; before it loads a tile it waits until that matrix's
@@ -325,18 +327,36 @@ __global__ void __launch_bounds__(256)
 // 2e-6.  So an accumulator holds 32 terms only, its small ones (hi lo, lo hi)
 // first and two additions of hi hi last, and the sum over the row is in
 // registers with fp32's rounding.
-constexpr int kTile = 128;
+//
+// Two forms.  A single block works on 128 x 128 tiles: 12 MMAs a k-block, each
+// reading 4 KB of either side, 117 cycles each, bound by shared memory.  A pair
+// of blocks (PAIR: a cluster of two, cta_group::2) works on 256 x 256 tiles, each
+// block with half of the rows of both sides: the same 8 KB of reads for four
+// times the products, 128 cycles per block, bound by the tensor cores.
 constexpr int kStages = 3;
-constexpr int kOpBytes = 2 * kBlkBytes;       // one plane of one operand's 128 x 64
+constexpr int kOpBytes = 2 * kBlkBytes;       // one plane of one block's 128 rows x 64
 constexpr int kStageBytes = 4 * kOpBytes;     // L hi, L lo, R hi, R lo
 constexpr int kOutOff = kStages * kStageBytes;
 constexpr int kOutWarp = 4096;                // staging of one epilogue warp
 constexpr int kEpiWarps = 8;
 constexpr int kBarOff = kOutOff + kEpiWarps * kOutWarp;
 constexpr int kSmemBytes = kBarOff + 1536 + 1024;  // barriers and prefixes, alignment
-constexpr int kProductThreads = (kEpiWarps + 2) * 32;
-constexpr int kAccs = 2;  // k-blocks in TMEM, two accumulators of 128 columns each
-constexpr int kRing = 4;  // tickets on their way from the producer to the other warps
+// Three warpgroups of 168 registers a thread at launch; the two of the epilogue
+// take over what the third does not need: 2 * 216 + 72 = 3 * 168.
+constexpr int kProductThreads = 384;
+constexpr int kRegsEpilogue = 216, kRegsOthers = 72;
+constexpr int kRing = 4;     // tickets on their way from the producer to the other warps
+constexpr int kTmemCols = 512;
+
+template <bool PAIR>
+struct Form {
+  static constexpr int kCtas = PAIR ? 2 : 1;
+  static constexpr int kTile = 128 * kCtas;            // rows and columns of a tile
+  static constexpr int kSide = 2 * kCtas;              // blocks along it
+  static constexpr int kAccs = kTmemCols / kTile;      // accumulators in TMEM
+  static constexpr int kCols = kTile / 2;              // columns of one epilogue warp
+  static constexpr int kChain = PAIR ? 4 : 2;          // 16-deep products one accumulator takes
+};
 
 struct Steps {
   int n;
@@ -350,6 +370,7 @@ struct Ticket {
 };
 
 // `start` is the table's tiles[3][kMaxItems + 1] in shared memory.
+template <bool PAIR>
 __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, int count, int n) {
   Ticket q;
   const int gram = start[count], square = start[kMaxItems + 1 + count];
@@ -373,7 +394,7 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
   q.share = 0;
   q.nk = it.mb;
   if (q.mode == UPDATE) {
-    const int tn = (it.cb + 1) / 2;
+    const int tn = (it.cb + Form<PAIR>::kSide - 1) / Form<PAIR>::kSide;
     q.i = k / tn;
     q.j = k - q.i * tn;
     q.tile = k;
@@ -397,22 +418,25 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
 }
 
 // One operand: block (mn, k) of a plane is at base + (mn * smn + k * sk) blocks.
+// Of A and P (sym) only the tiles on and below the diagonal are kept: a block
+// above it is read from its mirror image, as an MN-major operand.
 struct Operand {
   const uint8_t* base;
   size_t plane;  // bytes from the hi to the lo plane
   int smn, sk, nmn;
   int mn_major;
+  int sym;
 };
 __device__ __forceinline__ Operand operand(const Item& it, int mode, int from, int right) {
   const bool tall = it.rows > it.cols;
   const uint8_t* x = it.x[from];
   const size_t xp = (size_t)it.rb * it.cb * kBlkBytes, mp = (size_t)it.mb * it.mb * kBlkBytes;
   if (mode == GRAM)  // rows of X, or columns when tall
-    return {x, xp, tall ? 1 : it.cb, tall ? it.cb : 1, it.mb, tall};
-  if (mode == SQUARE) return {it.a, mp, it.mb, 1, it.mb, 0};
+    return {x, xp, tall ? 1 : it.cb, tall ? it.cb : 1, it.mb, tall, 0};
+  if (mode == SQUARE) return {it.a, mp, it.mb, 1, it.mb, 0, 1};
   if (tall != (right != 0))  // X's rows (tall, left) or columns (wide, right)
-    return {x, xp, right ? 1 : it.cb, right ? it.cb : 1, right ? it.cb : it.rb, right};
-  return {it.p, mp, it.mb, 1, it.mb, 0};
+    return {x, xp, right ? 1 : it.cb, right ? it.cb : 1, right ? it.cb : it.rb, right, 0};
+  return {it.p, mp, it.mb, 1, it.mb, 0, 1};
 }
 
 __device__ __forceinline__ int load_acquire(const int* p) {
@@ -426,60 +450,81 @@ __device__ __forceinline__ void add_release(int* p, int v) {
 __device__ __forceinline__ void fence_proxy_async_all() {
   asm volatile("fence.proxy.async;" ::: "memory");
 }
-__device__ __forceinline__ void epilogue_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
-}
 
-// The counter a ticket waits for, and the value it must have reached.
+// The counter a ticket waits for, and the value it must have reached (every
+// block of a tile counts).
+template <bool PAIR>
 __device__ __forceinline__ const int* needs(const Table* t, const int* start, const Ticket& q,
                                             int* value) {
   const int before = (q.mode + 2) % 3;  // GRAM <- UPDATE of the step before
   const int* st = start + before * (kMaxItems + 1) + q.item;
   int tiles = st[1] - st[0];
   if (before == GRAM) tiles /= t->it[q.item].ks;  // counted once per tile
-  *value = tiles * (q.mode == GRAM ? q.step : q.step + 1);
+  *value = Form<PAIR>::kCtas * tiles * (q.mode == GRAM ? q.step : q.step + 1);
   return t->ctrl + kCtrlDone + 3 * q.item + before;
 }
 
+template <bool PAIR>
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, long long lim) {
+  return PAIR ? mbar_wait_cluster(bar, parity, lim) : mbar_wait(bar, parity, lim);
+}
+
+template <bool PAIR>
 __global__ void __launch_bounds__(kProductThreads, 1)
     ns_steps_kernel(const Table* __restrict__ t, const __grid_constant__ Steps steps,
                     const __grid_constant__ Update u, int* err) {
+  using F = Form<PAIR>;
+  constexpr int kAccs = F::kAccs, kCols = F::kCols;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);
-  uint64_t* empty = full + kStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);  // this block's copies
+  uint64_t* pfull = full + kStages;       // rank 0: the other block's copies
+  uint64_t* empty = pfull + kStages;
   uint64_t* acc_full = empty + kStages;
-  uint64_t* acc_empty = acc_full + kAccs;
+  uint64_t* acc_empty = acc_full + kAccs;  // rank 0
   uint64_t* tfull = acc_empty + kAccs;
-  uint64_t* tempty = tfull + kRing;
+  uint64_t* tempty = tfull + kRing;        // rank 0
   uint64_t* drain = tempty + kRing;
-  int* ring = reinterpret_cast<int*>(drain + 1);
+  uint64_t* esync = drain + 1;
+  int* ring = reinterpret_cast<int*>(esync + 1);
   int* last_share = ring + kRing;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last_share + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 1);  // [3][kMaxItems + 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_rank() : 0;
   const int count = t->count;
   for (int i = threadIdx.x; i < 3 * (kMaxItems + 1); i += kProductThreads)
     start[i] = (&t->tiles[0][0])[i];
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
+      mbar_init(&pfull[s], 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < kAccs; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], kEpiWarps);
+      mbar_init(&acc_empty[b], F::kCtas * kEpiWarps);
     }
     for (int b = 0; b < kRing; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 1 + kEpiWarps);
+      // rank 0: the MMA thread and the epilogue; rank 1: producer, relay, epilogue
+      mbar_init(&tempty[b], 1 + kEpiWarps + (PAIR ? 2 + kEpiWarps : 0));
     }
     mbar_init(drain, 1);
+    mbar_init(esync, kEpiWarps);
     fence_barrier_init();
   }
+  if (PAIR) {
+    __syncthreads();
+    cluster_sync_all();  // the other block's barriers are ready, and both can allocate
+  }
   if (warp == kEpiWarps + 1) {
-    tmem_alloc(tmem_slot, 2 * kAccs * kTile);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(tmem_slot, kTmemCols);
+    } else {
+      tmem_alloc(tmem_slot, kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -488,29 +533,51 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   const int total = steps.n * (start[count] + start[kMaxItems + 1 + count] +
                                start[2 * (kMaxItems + 1) + count]);
   const long long lim = wait_limit(err);
+  // arrivals on rank 0's barriers
+  auto arrive0 = [&](uint64_t* bar) {
+    if (PAIR) mbar_arrive_cluster(map_to_rank(smem_u32(bar), 0));
+    else mbar_arrive(bar);
+  };
 
+  if (warp >= kEpiWarps) {
+    reg_dec<kRegsOthers>();
   if (warp == kEpiWarps) {
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      int next = atomicAdd(t->ctrl, 1);
+      int next = rank == 0 ? atomicAdd(t->ctrl, 1) : 0;
       for (uint32_t k = 0; ok; ++k) {
-        const int n = next, slot = k % kRing;
-        if (k >= kRing && !mbar_wait(&tempty[slot], (k / kRing - 1) & 1, lim)) {
-          report_error(err, YL_DEVERR_TIMEOUT);
-          break;
+        const int slot = k % kRing;
+        int n = next;
+        if (rank == 0) {
+          if (k >= kRing && !wait<PAIR>(&tempty[slot], (k / kRing - 1) & 1, lim)) {
+            report_error(err, YL_DEVERR_TIMEOUT);
+            break;
+          }
+          ring[slot] = n;
+          mbar_arrive(&tfull[slot]);
+          if (PAIR) {
+            st_cluster_s32(map_to_rank(smem_u32(&ring[slot]), 1), n);
+            mbar_arrive_cluster(map_to_rank(smem_u32(&tfull[slot]), 1));
+          }
+          if (n < total) next = atomicAdd(t->ctrl, 1);  // on its way while this tile loads
+        } else {
+          if (!wait<PAIR>(&tfull[slot], (k / kRing) & 1, lim)) {
+            report_error(err, YL_DEVERR_TIMEOUT);
+            break;
+          }
+          n = ring[slot];
+          arrive0(&tempty[slot]);
         }
-        ring[slot] = n;
-        mbar_arrive(&tfull[slot]);
         if (n >= total) break;
-        next = atomicAdd(t->ctrl, 1);  // on its way while this tile loads
-        const Ticket q = ticket_of(t, start, count, n);
+        const Ticket q = ticket_of<PAIR>(t, start, count, n);
         const Item& im = t->it[q.item];
         const Operand L = operand(im, q.mode, q.step & 1, 0), R = operand(im, q.mode, q.step & 1, 1);
         const bool same = q.mode != UPDATE && q.i == q.j;
-        const int nl = min(2, L.nmn - 2 * q.i), nr = same ? 0 : min(2, R.nmn - 2 * q.j);
+        const int l0 = F::kSide * q.i + 2 * rank, r0 = F::kSide * q.j + 2 * rank;
+        const int nl = max(0, min(2, L.nmn - l0)), nr = same ? 0 : max(0, min(2, R.nmn - r0));
         int value;
-        const int* counter = needs(t, start, q, &value);
+        const int* counter = needs<PAIR>(t, start, q, &value);
         const long long t0 = clock64();
         while (load_acquire(counter) < value) {
           if (clock64() - t0 > lim) {
@@ -520,22 +587,37 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
         }
         if (!ok) break;
-        fence_proxy_async_all();  // other blocks' plain stores before this thread's bulk loads
-        for (int kb = 0; kb < q.nk; ++kb, ++it) {
+        const int extra = q.mode == SQUARE ? F::kCtas : 0;  // stages with the tile's own A
+        fence_proxy_async_all();  // what the acquire saw, before this thread's bulk loads
+        for (int kb = 0; kb < q.nk + extra; ++kb, ++it) {
           const int s = it % kStages;
-          if (it >= kStages && !mbar_wait(&empty[s], ((it / kStages) - 1) & 1, lim)) {
+          if (it >= kStages && !wait<PAIR>(&empty[s], ((it / kStages) - 1) & 1, lim)) {
             report_error(err, YL_DEVERR_TIMEOUT);
             ok = false;
             break;
           }
           const uint32_t dst = smem_u32(smem + s * kStageBytes);
+          if (kb >= q.nk) {  // 128 rows x 128 columns of A for the epilogue, blocks [row][column]
+            const int c0 = F::kSide * q.j + 2 * (kb - q.nk), nc = max(0, min(2, im.mb - c0));
+            mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * nl * nc) * kBlkBytes);
+            for (int b = 0; b < nl * nc; ++b) {
+              const int br = b / nc, bc = b - br * nc;
+              const uint8_t* src = im.a + ((size_t)(l0 + br) * im.mb + c0 + bc) * kBlkBytes;
+              const uint32_t d = dst + (uint32_t)((2 * br + bc) * kBlkBytes);
+              bulk_load(d, src, kBlkBytes, &full[s]);
+              bulk_load(d + 2 * kOpBytes, src + L.plane, kBlkBytes, &full[s]);
+            }
+            continue;
+          }
           mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * (nl + nr)) * kBlkBytes);
+          const int kk = q.kb0 + kb;
           for (int side = 0; side < 2; ++side) {
             const Operand& o = side ? R : L;
-            const int nb = side ? nr : nl, mn0 = 2 * (side ? q.j : q.i);
+            const int nb = side ? nr : nl, mn0 = side ? r0 : l0;
+            const bool above = o.sym && (side ? q.j : q.i) < kk / F::kSide;
+            const size_t smn = above ? o.sk : o.smn, sk = above ? o.smn : o.sk;
             for (int b = 0; b < nb; ++b) {
-              const uint8_t* src =
-                  o.base + ((size_t)(mn0 + b) * o.smn + (size_t)(q.kb0 + kb) * o.sk) * kBlkBytes;
+              const uint8_t* src = o.base + ((size_t)(mn0 + b) * smn + (size_t)kk * sk) * kBlkBytes;
               const uint32_t d = dst + (uint32_t)(side * 2 * kOpBytes + b * kBlkBytes);
               bulk_load(d, src, kBlkBytes, &full[s]);
               bulk_load(d + kOpBytes, src + o.plane, kBlkBytes, &full[s]);
@@ -543,212 +625,272 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
         }
       }
-      drain_ring(full, kStages, it);  // no copy may still be landing when the CTA exits
+      drain_ring(full, kStages, it);  // no copy may still be landing when the block exits
     }
   } else if (warp == kEpiWarps + 1) {
     if (lane == 0) {
-      uint32_t it = 0;
+      uint32_t it = 0, ci = 0;
       bool ok = true;
       for (uint32_t k = 0; ok; ++k) {
         const int slot = k % kRing;
-        if (!mbar_wait(&tfull[slot], (k / kRing) & 1, lim)) {
+        if (!wait<PAIR>(&tfull[slot], (k / kRing) & 1, lim)) {
           report_error(err, YL_DEVERR_TIMEOUT);
           break;
         }
         const int n = ring[slot];
-        mbar_arrive(&tempty[slot]);
+        arrive0(&tempty[slot]);
         if (n >= total) break;
-        const Ticket q = ticket_of(t, start, count, n);
+        const Ticket q = ticket_of<PAIR>(t, start, count, n);
+        const int extra = q.mode == SQUARE ? F::kCtas : 0;
+        if (rank != 0) {  // tell rank 0 of every stage that has landed here
+          for (int kb = 0; kb < q.nk + extra; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!mbar_wait(&full[s], (it / kStages) & 1, lim)) {
+              report_error(err, YL_DEVERR_TIMEOUT);
+              ok = false;
+              break;
+            }
+            arrive0(&pfull[s]);
+          }
+          continue;
+        }
         const Item& im = t->it[q.item];
-        const int lmn = operand(im, q.mode, 0, 0).mn_major, rmn = operand(im, q.mode, 0, 1).mn_major;
+        const Operand L = operand(im, q.mode, 0, 0), R = operand(im, q.mode, 0, 1);
         const bool same = q.mode != UPDATE && q.i == q.j;
-        const uint32_t idesc = idesc_f16(kTile, kTile, lmn, rmn);
-        // K-major: 16 of a row's 64 k are 32 bytes, 8-row groups 1 KB apart.
-        // MN-major: 16 k are two 8-row groups, 64-column blocks 8 KB apart.
-        const uint32_t lstep = lmn ? 2048 : 32, rstep = rmn ? 2048 : 32;
-        const uint32_t llbo = lmn ? kBlkBytes : 16, rlbo = rmn ? kBlkBytes : 16;
-        for (int kb = 0; kb < q.nk; ++kb, ++it) {
-          const int s = it % kStages, buf = it % kAccs;
-          if ((it >= kAccs && !mbar_wait(&acc_empty[buf], (it / kAccs - 1) & 1, lim)) ||
-              !mbar_wait(&full[s], (it / kStages) & 1, lim)) {
+        int filled = 0;  // products the current accumulator has taken
+        for (int kb = 0; ok && kb < q.nk; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&full[s], (it / kStages) & 1, lim) ||
+              (PAIR && !wait<PAIR>(&pfull[s], (it / kStages) & 1, lim))) {
             report_error(err, YL_DEVERR_TIMEOUT);
             ok = false;
             break;
           }
-          tc_fence_after();
+          const int kt = (q.kb0 + kb) / F::kSide;
+          const int lmn = L.mn_major | (L.sym & (q.i < kt)), rmn = R.mn_major | (R.sym & (q.j < kt));
+          const uint32_t idesc = idesc_f16(F::kTile, F::kTile, lmn, rmn);
+          // K-major: 16 of a row's 64 k are 32 bytes, 8-row groups 1 KB apart.
+          // MN-major: 16 k are two 8-row groups, 64-column blocks 8 KB apart.
+          const uint32_t lstep = lmn ? 2048 : 32, rstep = rmn ? 2048 : 32;
+          const uint32_t llbo = lmn ? kBlkBytes : 16, rlbo = rmn ? kBlkBytes : 16;
           const uint32_t l = smem_u32(smem + s * kStageBytes), r = same ? l : l + 2 * kOpBytes;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t dacc = tmem + (uint32_t)((2 * buf + h) * kTile);
+          constexpr int kRun = F::kChain < 4 ? F::kChain : 4;  // products of one k-block in a row
+#pragma unroll 1
+          for (int h = 0; h < 4; h += kRun) {
+            const int buf = ci % kAccs;
+            if (filled == 0 && ci >= kAccs && !wait<PAIR>(&acc_empty[buf], (ci / kAccs - 1) & 1, lim)) {
+              report_error(err, YL_DEVERR_TIMEOUT);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t dacc = tmem + (uint32_t)(buf * F::kTile);
 #pragma unroll
             for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
               const uint32_t lp = l + (part == 0 ? kOpBytes : 0);
               const uint32_t rp = r + (part == 1 ? kOpBytes : 0);
 #pragma unroll
-              for (int kk = 2 * h; kk < 2 * h + 2; ++kk)
-                umma_f16(dacc, sw128_desc(lp + kk * lstep, llbo, 1024),
-                         sw128_desc(rp + kk * rstep, rlbo, 1024), idesc,
-                         (part | (kk & 1)) != 0);
+              for (int e = 0; e < kRun; ++e) {
+                const int kk = h + e;
+                const uint64_t ld = sw128_desc(lp + kk * lstep, llbo, 1024);
+                const uint64_t rd = sw128_desc(rp + kk * rstep, rlbo, 1024);
+                if (PAIR) umma_f16_pair(dacc, ld, rd, idesc, (filled | part | e) != 0);
+                else umma_f16(dacc, ld, rd, idesc, (filled | part | e) != 0);
+              }
+            }
+            filled += kRun;
+            if (filled == F::kChain || (kb + 1 == q.nk && h + kRun == 4)) {
+              if (PAIR) umma_commit_pair(&acc_full[buf]);
+              else umma_commit(&acc_full[buf]);
+              filled = 0;
+              ++ci;
             }
           }
-          umma_commit(&empty[s]);
-          umma_commit(&acc_full[buf]);
+          if (!ok) break;
+          if (PAIR) umma_commit_pair(&empty[s]);
+          else umma_commit(&empty[s]);
         }
+        it += extra;  // the epilogue reads and frees those
       }
-      // every MMA this thread issued has completed before TMEM is released
-      umma_commit(drain);
-      mbar_wait(drain, 0);
+      // every MMA this thread issued has completed before TMEM and the other
+      // block's shared memory are released
+      if (rank == 0) {
+        if (PAIR) umma_commit_pair(drain);
+        else umma_commit(drain);
+      }
+      wait<PAIR>(drain, 0, kWaitLimitCycles);
     }
+  }
   } else {
-    // epilogue: warp w owns rows 32 (w % 4) .. + 31 (its TMEM lanes) and columns
-    // 64 (w / 4) .. + 63 of the tile
-    uint32_t it = 0;
+    reg_inc<kRegsEpilogue>();
+    // epilogue: warp w owns rows 32 (w % 4) .. + 31 of the block's 128 (its TMEM
+    // lanes) and columns kCols (w / 4) .. of the tile
+    uint32_t it = 0, ci = 0;
     uint8_t* stage = smem + kOutOff + warp * kOutWarp;
     const int wr = warp & 3, wc = warp >> 2;
+    // barrier of the epilogue warps; bounded like every wait, so that no warp is
+    // left behind when another one has given up
+    uint32_t phase = 0;
+    auto together = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(esync);
+      if (mbar_wait(esync, phase++ & 1, lim)) return true;
+      report_error(err, YL_DEVERR_TIMEOUT);
+      return false;
+    };
     for (uint32_t k = 0;; ++k) {
       const int slot = k % kRing;
-      if (!mbar_wait(&tfull[slot], (k / kRing) & 1, lim)) {
+      if (!wait<PAIR>(&tfull[slot], (k / kRing) & 1, lim)) {
         report_error(err, YL_DEVERR_TIMEOUT);
         break;
       }
       const int n = ring[slot];
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[slot]);
+      if (lane == 0) arrive0(&tempty[slot]);
       if (n >= total) break;
-      const Ticket q = ticket_of(t, start, count, n);
+      const Ticket q = ticket_of<PAIR>(t, start, count, n);
       const Item& im = t->it[q.item];
-      float v[64];
+      float v[kCols];
 #pragma unroll
-      for (int c = 0; c < 64; ++c) v[c] = 0.f;
+      for (int c = 0; c < kCols; ++c) v[c] = 0.f;
       bool ok = true;
-      for (int kb = 0; kb < q.nk; ++kb, ++it) {
-        const int buf = it % kAccs;
-        if (!mbar_wait(&acc_full[buf], (it / kAccs) & 1, lim)) {
+      for (int ch = 0; ch < (4 * q.nk + F::kChain - 1) / F::kChain; ++ch, ++ci) {
+        const int buf = ci % kAccs;
+        if (!wait<PAIR>(&acc_full[buf], (ci / kAccs) & 1, lim)) {
           report_error(err, YL_DEVERR_TIMEOUT);
           ok = false;
           break;
         }
         tc_fence_after();
         const uint32_t at =
-            tmem + ((uint32_t)(wr * 32) << 16) + (uint32_t)(2 * buf * kTile + wc * 64);
-        // (accumulator, column half) p: the next read runs while this one is added
-        uint32_t acc[2][32];
-        tmem_ld_32x32b_x32(at, acc[0]);
+            tmem + ((uint32_t)(wr * 32) << 16) + (uint32_t)(buf * F::kTile + wc * kCols);
+        // 16 columns at a time: the next read runs while this one is added
+        uint32_t acc[2][16];
+        tmem_ld_32x32b_x16(at, acc[0]);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
+        for (int p = 0; p < kCols / 16; ++p) {
           tmem_ld_wait();
-          if (p < 3) tmem_ld_32x32b_x32(at + ((p + 1) & 1) * kTile + ((p + 1) >> 1) * 32, acc[(p + 1) & 1]);
+          if (p + 1 < kCols / 16) tmem_ld_32x32b_x16(at + (p + 1) * 16, acc[(p + 1) & 1]);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[(p >> 1) * 32 + c] += __uint_as_float(acc[p & 1][c]);
+          for (int c = 0; c < 16; ++c) v[p * 16 + c] += __uint_as_float(acc[p & 1][c]);
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        if (lane == 0) arrive0(&acc_empty[buf]);
       }
       if (!ok) break;
+      it += q.nk;
       if (q.mode == GRAM && im.ks > 1) {
         // leave this share's sum; the block that finishes a tile's last share adds
         // them all, in share order whoever that is
-        float* part = im.partial + ((size_t)q.tile * im.ks) * kTile * kTile +
-                      (size_t)(wc * 64) * kTile + wr * 32 + lane;
-        float* mine = part + (size_t)q.share * kTile * kTile;
+        constexpr size_t kSlice = (size_t)F::kTile * 128;  // one block's part of a tile
+        const size_t slot0 = ((size_t)q.tile * F::kCtas + rank) * im.ks;
+        float* part = im.partial + slot0 * kSlice + (size_t)(wc * kCols) * 128 + wr * 32 + lane;
+        float* mine = part + (size_t)q.share * kSlice;
 #pragma unroll
-        for (int c = 0; c < 64; ++c) __stcg(mine + c * kTile, v[c]);
-        epilogue_sync();
+        for (int c = 0; c < kCols; ++c) __stcg(mine + c * 128, v[c]);
+        if (!together()) break;
         if (threadIdx.x == 0) {
           __threadfence();  // with the barrier: all of the block's stores
-          const int seen = atomicAdd(t->ctrl + kCtrlSplit + im.split0 + q.tile, 1);
+          const int seen = atomicAdd(
+              t->ctrl + kCtrlSplit + im.split0 + q.tile * F::kCtas + (int)rank, 1);
           __threadfence();
           *last_share = seen == im.ks * (q.step + 1) - 1;
         }
-        epilogue_sync();
+        if (!together()) break;
         const bool mine_is_last = *last_share != 0;
         if (!mine_is_last) continue;  // thread 0 writes the flag again only behind a barrier
 #pragma unroll
-        for (int c = 0; c < 64; ++c) v[c] = 0.f;
+        for (int c = 0; c < kCols; ++c) v[c] = 0.f;
         for (int sh = 0; sh < im.ks; ++sh) {
-          const float* p = part + (size_t)sh * kTile * kTile;
+          const float* p = part + (size_t)sh * kSlice;
 #pragma unroll
-          for (int c = 0; c < 64; ++c) v[c] += __ldcg(p + c * kTile);
+          for (int c = 0; c < kCols; ++c) v[c] += __ldcg(p + c * 128);
         }
       }
       const bool sq = q.mode != UPDATE, last = !sq && q.step + 1 == steps.n;
       const int rbt = sq ? im.mb : im.rb, cbt = sq ? im.mb : im.cb;
-      const int rblk = 2 * q.i + (wr >> 1), r64 = (wr & 1) * 32 + lane;  // row inside its block
-      const int cblk = 2 * q.j + wc;
+      // row block and row inside it
+      const int rblk = F::kSide * q.i + 2 * rank + (wr >> 1), r64 = (wr & 1) * 32 + lane;
       const float c2 = q.mode == GRAM     ? steps.g2[q.step]
                        : q.mode == SQUARE ? steps.s2[q.step]
                                           : steps.u2[q.step];
-      const bool inside = rblk < rbt && cblk < cbt;  // uniform in the warp
-      if (inside) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c) v[c] *= c2;
+      uint8_t* out = sq ? (q.mode == GRAM ? im.a : im.p) : im.x[(q.step & 1) ^ 1];
+      const size_t plane = (size_t)rbt * cbt * kBlkBytes;
+      const uint8_t* own = nullptr;  // this warp's 128 columns of the tile's own A
+      if (q.mode == SQUARE) {
+        const uint32_t e = it + (PAIR ? wc : 0);
+        if (!mbar_wait(&full[e % kStages], (e / kStages) & 1, lim)) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+          break;
+        }
+        own = smem + (e % kStages) * kStageBytes;
       }
-      if (inside && last) {
-        // 32 rows x 32 columns through shared memory (columns rotated by the
-        // row), then whole row pieces to the result
-        float* st = reinterpret_cast<float*>(stage);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          __syncwarp();
+      for (int slab = 0; slab < kCols / 64; ++slab) {
+        const int cblk = F::kSide * q.j + wc * (kCols / 64) + slab;
+        if (rblk >= rbt || cblk >= cbt) continue;  // uniform in the warp
+        float* w = v + slab * 64;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) st[lane * 32 + ((c + lane) & 31)] = v[half * 32 + c];
-          __syncwarp();
-          const long long r0 = (long long)rblk * kBlk + (wr & 1) * 32;
-          const long long col = (long long)cblk * kBlk + half * 32 + lane;
-          if (col < im.cols) {
-            const int nr = (int)min(32LL, im.rows - r0);
-            float* d = im.dst + r0 * im.ldd + col;
+        for (int c = 0; c < 64; ++c) w[c] *= c2;
+        if (last) {
+          // 32 rows x 32 columns through shared memory (columns rotated by the
+          // row), then whole row pieces to the result
+          float* st = reinterpret_cast<float*>(stage);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) st[lane * 32 + ((c + lane) & 31)] = w[half * 32 + c];
+            __syncwarp();
+            const long long r0 = (long long)rblk * kBlk + (wr & 1) * 32;
+            const long long col = (long long)cblk * kBlk + half * 32 + lane;
+            if (col < im.cols) {
+              const int nr = (int)min(32LL, im.rows - r0);
+              float* d = im.dst + r0 * im.ldd + col;
 #pragma unroll 1
-            for (int r1 = 0; r1 < nr; r1 += 16) {
-              float pv[16];  // the parameter's rows are all on their way before the first is used
-              if (u.muon) {
+              for (int r1 = 0; r1 < nr; r1 += 16) {
+                float pv[16];  // the parameter's rows are all on their way before the first is used
+                if (u.muon) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                  pv[r] = r1 + r < nr ? __ldcs(d + (r1 + r) * im.ldd) : 0.f;
-              }
+                  for (int r = 0; r < 16; ++r)
+                    pv[r] = r1 + r < nr ? __ldcs(d + (r1 + r) * im.ldd) : 0.f;
+                }
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                float x = st[(r1 + r) * 32 + ((lane + r1 + r) & 31)];
-                if (u.muon) x = pv[r] * (1.f - u.lr * u.decay) - u.lr * im.scale * x;
-                if (r1 + r < nr) __stcs(d + (r1 + r) * im.ldd, x);
+                for (int r = 0; r < 16; ++r) {
+                  float x = st[(r1 + r) * 32 + ((lane + r1 + r) & 31)];
+                  if (u.muon) x = pv[r] * (1.f - u.lr * u.decay) - u.lr * im.scale * x;
+                  if (r1 + r < nr) __stcs(d + (r1 + r) * im.ldd, x);
+                }
               }
             }
           }
+          continue;
         }
-      }
-      if (last) continue;  // nothing waits for the results
-      if (inside) {
-        uint8_t* out = sq ? (q.mode == GRAM ? im.a : im.p) : im.x[(q.step & 1) ^ 1];
-        const size_t plane = (size_t)rbt * cbt * kBlkBytes;
         const size_t blk = ((size_t)rblk * cbt + cblk) * kBlkBytes;
         if (q.mode == SQUARE) {
-          int value;
-          load_acquire(needs(t, start, q, &value));  // reached already; orders the reads of A
           const float s1 = steps.s1[q.step], s0 = steps.s0[q.step];
-          const uint8_t* ah = im.a + blk + r64 * 128;
+          const uint8_t* ah = own + (2 * (wr >> 1) + (PAIR ? slab : wc)) * kBlkBytes + r64 * 128;
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
             const int at = (ch ^ (r64 & 7)) << 4;
-            const uint4 h4 = __ldcg(reinterpret_cast<const uint4*>(ah + at));
-            const uint4 l4 = __ldcg(reinterpret_cast<const uint4*>(ah + plane + at));
+            const uint4 h4 = *reinterpret_cast<const uint4*>(ah + at);
+            const uint4 l4 = *reinterpret_cast<const uint4*>(ah + 2 * kOpBytes + at);
             const __half2* h = reinterpret_cast<const __half2*>(&h4);
             const __half2* l = reinterpret_cast<const __half2*>(&l4);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               const float2 hf = __half22float2(h[j]), lf = __half22float2(l[j]);
-              v[ch * 8 + 2 * j] += s1 * (hf.x + lf.x);
-              v[ch * 8 + 2 * j + 1] += s1 * (hf.y + lf.y);
+              w[ch * 8 + 2 * j] += s1 * (hf.x + lf.x);
+              w[ch * 8 + 2 * j + 1] += s1 * (hf.y + lf.y);
             }
           }
           if (rblk == cblk) {
 #pragma unroll
             for (int c = 0; c < 64; ++c)
-              if (r64 == c) v[c] += s0;
+              if (r64 == c) w[c] += s0;
           }
         }
-        const bool mirror = sq && q.i != q.j;
-        uint8_t* mir = out + ((size_t)cblk * cbt + rblk) * kBlkBytes;
 #pragma unroll
         for (int pl = 0; pl < 2; ++pl) {  // hi plane, then what is left of v as the lo plane
           if (lane == 0) bulk_wait_group_read<0>();  // the staging rows are free again
@@ -758,21 +900,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             __align__(16) __half2 h[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float* w = v + ch * 8 + 2 * j;
-              h[j] = __floats2half2_rn(w[0], w[1]);
+              float* x = w + ch * 8 + 2 * j;
+              h[j] = __floats2half2_rn(x[0], x[1]);
               if (pl == 0) {
                 const float2 f = __half22float2(h[j]);
-                w[0] -= f.x;
-                w[1] -= f.y;
-              }
-              if (mirror) {
-                const int row = ch * 8 + 2 * j;  // rows of the mirrored block; its column is r64
-                const int at = (r64 & 7) * 2;
-                *reinterpret_cast<__half*>(mir + pl * plane + row * 128 +
-                                           (((r64 >> 3) ^ (row & 7)) << 4) + at) = __low2half(h[j]);
-                *reinterpret_cast<__half*>(mir + pl * plane + (row + 1) * 128 +
-                                           (((r64 >> 3) ^ ((row + 1) & 7)) << 4) + at) =
-                    __high2half(h[j]);
+                x[0] -= f.x;
+                x[1] -= f.y;
               }
             }
             *reinterpret_cast<uint4*>(stage + lane * 128 + ((ch ^ (r64 & 7)) << 4)) =
@@ -785,20 +918,26 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             bulk_commit_group();
           }
         }
-        if (lane == 0) bulk_wait_group_all();
       }
+      if (last) continue;  // nothing waits for the results
+      if (lane == 0) bulk_wait_group_all();
       // everything this block wrote of the tile is in memory before the count says so
-      if (sq && q.i != q.j) fence_proxy_async_all();  // the mirrored blocks' plain stores
-      epilogue_sync();
+      if (!together()) break;
+      if (q.mode == SQUARE) {
+        if (threadIdx.x < F::kCtas) mbar_arrive(&empty[(it + threadIdx.x) % kStages]);
+        it += F::kCtas;
+      }
       if (threadIdx.x == 0) add_release(t->ctrl + kCtrlDone + 3 * q.item + q.mode, 1);
     }
     if (lane == 0) bulk_wait_group_all();
   }
   tc_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync_all();  // neither block's barriers or operands are used any more
   if (warp == kEpiWarps + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * kAccs * kTile);
+    if (PAIR) tmem_dealloc_pair(tmem, kTmemCols);
+    else tmem_dealloc(tmem, kTmemCols);
   }
 }
 
@@ -835,13 +974,14 @@ size_t place(Table* t, int num_sms, char* ws) {
   // per SM, and at most sqrt(nk / 2), where the sums' way through memory costs as
   // much as the k-blocks it saves (about 0.6 us a share against 0.4 us a k-block).
   auto nk = [](const Item& it) { return std::max(it.rb, it.cb); };
-  auto gram_tiles = [](const Item& it) {
-    const int mt = (it.mb + 1) / 2;
+  const int ctas = t->pair ? 2 : 1, workers = num_sms / ctas;
+  auto gram_tiles = [&](const Item& it) {
+    const int mt = (it.mb + 2 * ctas - 1) / (2 * ctas);
     return mt * (mt + 1) / 2;
   };
   double kb = 0;
   for (int k = 0; k < t->count; ++k) kb += (double)gram_tiles(t->it[k]) * nk(t->it[k]);
-  const double fair = kb / num_sms;
+  const double fair = kb / workers;
   int splits = 0;
   for (int k = 0; k < t->count; ++k) {
     Item& it = t->it[k];
@@ -850,8 +990,9 @@ size_t place(Table* t, int num_sms, char* ws) {
     it.split0 = splits;
     it.partial = nullptr;
     if (it.ks > 1) {
-      splits += gram_tiles(it);
-      it.partial = (float*)take((size_t)gram_tiles(it) * it.ks * kTile * kTile * sizeof(float));
+      splits += gram_tiles(it) * ctas;
+      const size_t tile = (size_t)128 * ctas * 128 * ctas * sizeof(float);
+      it.partial = (float*)take(gram_tiles(it) * it.ks * tile);
     }
   }
   t->ctrl_ints = kCtrlSplit + splits;
@@ -868,15 +1009,16 @@ struct Schedule {
 
 yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, char* ws) {
   place(&t, ctx->num_sms, ws);
-  auto half_up = [](int v) { return (v + 1) / 2; };
+  const int ctas = t.pair ? 2 : 1, side = 2 * ctas;
+  auto tiles = [&](int v) { return (v + side - 1) / side; };
   for (int m = 0; m < 3; ++m) t.tiles[m][0] = 0;
   t.blocks[0] = t.chunks[0] = 0;
   for (int k = 0; k < t.count; ++k) {
     const Item& it = t.it[k];
-    const int mt = half_up(it.mb);
+    const int mt = tiles(it.mb);
     t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + mt * (mt + 1) / 2 * it.ks;
     t.tiles[SQUARE][k + 1] = t.tiles[SQUARE][k] + mt * (mt + 1) / 2;
-    t.tiles[UPDATE][k + 1] = t.tiles[UPDATE][k] + half_up(it.rb) * half_up(it.cb);
+    t.tiles[UPDATE][k + 1] = t.tiles[UPDATE][k] + tiles(it.rb) * tiles(it.cb);
     t.blocks[k + 1] = t.blocks[k] + it.rb * it.cb;
     t.chunks[k + 1] = t.chunks[k] + it.chunks;
   }
@@ -889,8 +1031,6 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   }
   ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0]);
   YL_TRY(check_launch("ns_split_kernel"));
-  YL_CUDA(cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kSmemBytes));
   Steps st;
   st.n = s.steps;
   for (int k = 0; k < s.steps; ++k) {
@@ -902,30 +1042,55 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
     st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx);
   }
   const int widest = std::max(t.tiles[GRAM][t.count], t.tiles[UPDATE][t.count]);
-  ns_steps_kernel<<<std::min(widest, ctx->num_sms), kProductThreads, kSmemBytes, ctx->stream>>>(
-      dt, st, u, ctx->dev_err);
+  const int workers = std::min(widest, ctx->num_sms / ctas);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(workers * ctas);
+  cfg.blockDim = dim3(kProductThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = 2;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = t.pair ? 1 : 0;
+  auto kernel = t.pair ? ns_steps_kernel<true> : ns_steps_kernel<false>;
+  YL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+  YL_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const Table*)dt, st, u, ctx->dev_err));
   return check_launch("ns_steps_kernel");
 }
 
-// All tables of a call, one after the other in the same workspace.
-yl_status run_items(yl_ctx* ctx, std::vector<Item>& items, const Update& u, const Schedule& s,
-                    char* ws) {
+// The tables of a call: matrices for pairs of blocks first, then the others.
+// Pairs: two blocks' worth of products for the shared-memory reads of one, but a
+// shorter side up to kPairSide is mostly padding in a 256 x 256 tile.
+template <class Fn>
+yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, Fn fn) {
   auto t = std::make_unique<Table>();
-  for (size_t base = 0; base < items.size(); base += kMaxItems) {
-    t->count = (int)std::min<size_t>(kMaxItems, items.size() - base);
-    std::copy_n(items.begin() + base, t->count, t->it);
-    YL_TRY(run_table(ctx, *t, u, s, ws));
+  for (int pair = 1; pair >= 0; --pair) {
+    t->count = 0;
+    t->pair = pair;
+    for (size_t k = 0; k <= items.size(); ++k) {
+      if (t->count == kMaxItems || (k == items.size() && t->count > 0)) {
+        YL_TRY(fn(*t));
+        t->count = 0;
+      }
+      if (k < items.size() && (std::min(items[k].rows, items[k].cols) > kPairSide) == (pair != 0))
+        t->it[t->count++] = items[k];
+    }
   }
   return YL_OK;
 }
-size_t items_bytes(yl_ctx* ctx, std::vector<Item>& items) {
+// One table after the other, in the same workspace.
+yl_status run_items(yl_ctx* ctx, const std::vector<Item>& items, const Update& u,
+                    const Schedule& s, char* ws) {
+  return for_tables(ctx, items, [&](Table& t) { return run_table(ctx, t, u, s, ws); });
+}
+size_t items_bytes(yl_ctx* ctx, const std::vector<Item>& items) {
   size_t most = 0;
-  auto t = std::make_unique<Table>();
-  for (size_t base = 0; base < items.size(); base += kMaxItems) {
-    t->count = (int)std::min<size_t>(kMaxItems, items.size() - base);
-    std::copy_n(items.begin() + base, t->count, t->it);
-    most = std::max(most, place(t.get(), ctx->num_sms, nullptr));
-  }
+  for_tables(ctx, items, [&](Table& t) {
+    most = std::max(most, place(&t, ctx->num_sms, nullptr));
+    return YL_OK;
+  });
   return most;
 }
 
