@@ -85,6 +85,26 @@ def test_one_matrix(h, r, c):
     assert rel(got, ns64(x)) < (TOL if max(r, c) > 1.2 * min(r, c) or min(r, c) == 1 else TOL_SPREAD)
 
 
+@pytest.mark.parametrize("shapes", [[(4000, 3900)], [(900, 4097), (64, 700)] + [(1030, 1000)] * 14])
+def test_enough_tiles_for_pairs_of_blocks(h, shapes):
+    """Sizes that run on 256 x 256 tiles, against float64 on the device."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    xs = [torch.randn(s, generator=gen, device="cuda") for s in shapes]
+    ys = [torch.empty_like(x) for x in xs]
+    table = (NsMatrix * len(xs))(*[
+        NsMatrix(x.data_ptr(), y.data_ptr(), *x.shape, x.shape[1], x.shape[1])
+        for x, y in zip(xs, ys)])
+    call("yl_newton_schulz", h, table, len(xs), 5, None, 1e-7)
+    for x, y in zip(xs, ys):
+        z = x.double() if x.shape[0] <= x.shape[1] else x.double().T
+        z = z / (z.square().sum().sqrt() + 1e-7)
+        for _ in range(5):
+            g = z @ z.T
+            z = QUINTIC[0] * z + QUINTIC[1] * (g @ z) + QUINTIC[2] * (g @ (g @ z))
+        z = z if x.shape[0] <= x.shape[1] else z.T
+        assert float((y.double() - z).norm() / z.norm()) < TOL
+
+
 def test_singular_values_end_near_one(h):
     x = normal(0, 96, 400)
     s = np.linalg.svd(run_ns(h, [x])[0].astype(np.float64), compute_uv=False)

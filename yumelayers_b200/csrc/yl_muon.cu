@@ -14,6 +14,7 @@
 #include <cmath>
 #include <memory>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 #include "yl_internal.h"
@@ -68,7 +69,7 @@ struct Item {
   float* partial;       // [GRAM tile][share][column][row] sums of the shares
 };
 enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
-constexpr int kPairSide = 128;
+constexpr int kPairSide = 512;
 struct Table {
   Item it[kMaxItems];
   int tiles[3][kMaxItems + 1];  // GRAM, SQUARE, UPDATE tickets before each item
@@ -324,9 +325,13 @@ __global__ void __launch_bounds__(256)
 // the tile.
 // The tensor core truncates when it adds to its accumulator: kept there over a
 // whole row, a 384 x 1153 matrix ended 2.4e-5 off, where an fp32 product gives
-// 2e-6.  So an accumulator holds 32 terms only, its small ones (hi lo, lo hi)
-// first and two additions of hi hi last, and the sum over the row is in
-// registers with fp32's rounding.
+// 2e-6.  So an accumulator takes a few 16-deep products only, the small ones
+// (hi lo, lo hi) of a k-block first, and the sum over the row is in registers with
+// fp32's rounding.  What costs accuracy is a term far above the others, and A and
+// P have theirs on the diagonal: with eight products to an accumulator throughout
+// 256 x 2304 ended 7.3e-6 off, with eight in GRAM and two elsewhere 2.1e-6 (fp32:
+// 2.0e-6).  So it is two in the k-blocks that meet a diagonal tile, eight in the
+// others, whose handover then hides behind the tensor core's work.
 //
 // Two forms.  A single block works on 128 x 128 tiles: 12 MMAs a k-block, each
 // reading 4 KB of either side, 117 cycles each, bound by shared memory.  A pair
@@ -355,7 +360,6 @@ struct Form {
   static constexpr int kSide = 2 * kCtas;              // blocks along it
   static constexpr int kAccs = kTmemCols / kTile;      // accumulators in TMEM
   static constexpr int kCols = kTile / 2;              // columns of one epilogue warp
-  static constexpr int kChain = PAIR ? 4 : 2;          // 16-deep products one accumulator takes
 };
 
 struct Steps {
@@ -415,6 +419,15 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
   q.i = i;
   q.j = k - i * (i + 1) / 2;
   return q;
+}
+
+// Whether k-block kb of a ticket meets the diagonal of A or P.
+template <bool PAIR>
+__device__ __forceinline__ bool on_diagonal(const Item& it, const Ticket& q, int kb) {
+  const int kt = kb / Form<PAIR>::kSide;
+  if (q.mode == GRAM) return false;
+  if (q.mode == SQUARE) return kt == q.i || kt == q.j;
+  return kt == (it.rows > it.cols ? q.j : q.i);
 }
 
 // One operand: block (mn, k) of a plane is at base + (mn * smn + k * sk) blocks.
@@ -674,14 +687,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           const uint32_t lstep = lmn ? 2048 : 32, rstep = rmn ? 2048 : 32;
           const uint32_t llbo = lmn ? kBlkBytes : 16, rlbo = rmn ? kBlkBytes : 16;
           const uint32_t l = smem_u32(smem + s * kStageBytes), r = same ? l : l + 2 * kOpBytes;
-          constexpr int kRun = F::kChain < 4 ? F::kChain : 4;  // products of one k-block in a row
-#pragma unroll 1
-          for (int h = 0; h < 4; h += kRun) {
+          // `run` products of this k-block into the current accumulator
+          auto multiply = [&](auto run, int h) {
+            constexpr int kRun = decltype(run)::value;
             const int buf = ci % kAccs;
             if (filled == 0 && ci >= kAccs && !wait<PAIR>(&acc_empty[buf], (ci / kAccs - 1) & 1, lim)) {
               report_error(err, YL_DEVERR_TIMEOUT);
               ok = false;
-              break;
+              return;
             }
             tc_fence_after();
             const uint32_t dacc = tmem + (uint32_t)(buf * F::kTile);
@@ -699,12 +712,18 @@ __global__ void __launch_bounds__(kProductThreads, 1)
               }
             }
             filled += kRun;
-            if (filled == F::kChain || (kb + 1 == q.nk && h + kRun == 4)) {
+            if (kRun == 2 || filled == 8 || kb + 1 == q.nk || on_diagonal<PAIR>(im, q, kb + 1)) {
               if (PAIR) umma_commit_pair(&acc_full[buf]);
               else umma_commit(&acc_full[buf]);
               filled = 0;
               ++ci;
             }
+          };
+          if (on_diagonal<PAIR>(im, q, kb)) {
+            multiply(std::integral_constant<int, 2>(), 0);
+            if (ok) multiply(std::integral_constant<int, 2>(), 2);
+          } else {
+            multiply(std::integral_constant<int, 4>(), 0);
           }
           if (!ok) break;
           if (PAIR) umma_commit_pair(&empty[s]);
@@ -754,7 +773,16 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 #pragma unroll
       for (int c = 0; c < kCols; ++c) v[c] = 0.f;
       bool ok = true;
-      for (int ch = 0; ch < (4 * q.nk + F::kChain - 1) / F::kChain; ++ch, ++ci) {
+      // the accumulators of the ticket, as the MMA thread fills them
+      for (int kb = 0, filled = 0, half = 0; kb < q.nk; ++ci) {
+        if (on_diagonal<PAIR>(im, q, kb)) {
+          half ^= 1;
+          if (!half) ++kb;
+        } else {
+          do filled += 4, ++kb;
+          while (filled < 8 && kb < q.nk && !on_diagonal<PAIR>(im, q, kb));
+          filled = 0;
+        }
         const int buf = ci % kAccs;
         if (!wait<PAIR>(&acc_full[buf], (ci / kAccs) & 1, lim)) {
           report_error(err, YL_DEVERR_TIMEOUT);
@@ -1061,10 +1089,19 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
 }
 
 // The tables of a call: matrices for pairs of blocks first, then the others.
-// Pairs: two blocks' worth of products for the shared-memory reads of one, but a
-// shorter side up to kPairSide is mostly padding in a 256 x 256 tile.
+// A pair does twice the products per shared-memory read, but has half as many and
+// larger tiles to share among the SMs, so it pays only where the 128 x 128 tiles
+// would fill them several times over: 16 of 1024 x 1024 (1024 tiles of an UPDATE)
+// take 1.16 ms in pairs and 1.25 ms alone, one 4096 x 4096 (1024 tiles, longer
+// rows) 3.8 and 4.7 ms, one 2048 x 2048 (256 tiles) 1.19 and 0.94 ms.  Shorter
+// sides under kPairSide are mostly padding in a 256 x 256 tile.
 template <class Fn>
 yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, Fn fn) {
+  auto wide = [](const Item& it) { return std::min(it.rows, it.cols) >= kPairSide; };
+  long long tiles = 0;
+  for (const Item& it : items)
+    if (wide(it)) tiles += (long long)((it.rows + 127) / 128) * ((it.cols + 127) / 128);
+  const bool pairs = tiles >= 6LL * ctx->num_sms;
   auto t = std::make_unique<Table>();
   for (int pair = 1; pair >= 0; --pair) {
     t->count = 0;
@@ -1074,7 +1111,7 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, Fn fn) {
         YL_TRY(fn(*t));
         t->count = 0;
       }
-      if (k < items.size() && (std::min(items[k].rows, items[k].cols) > kPairSide) == (pair != 0))
+      if (k < items.size() && (pairs && wide(items[k])) == (pair != 0))
         t->it[t->count++] = items[k];
     }
   }
