@@ -464,6 +464,24 @@ yl_status yl_trainer_step_host(yl_trainer* tr, const float* frames_host, const f
 /* Replace the runtime options (learning rates, which parts train, profiling);
  * batch and frame size must match creation. */
 yl_status yl_trainer_set_config(yl_trainer* tr, const yl_trainer_config* cfg);
+/* Muon for the hidden weight matrices of both models: every conv and Linear
+ * weight, as oc rows of k*k*ic columns, except those of the convs that read a
+ * model's input and write its output; the other parameters stay with Adam
+ * (lr_vae / lr_motion of yl_trainer_config).  Per matrix yl_muon_multi with the
+ * quintic, eps 1e-7 and scale sqrt(max(1, oc / (k*k*ic))).  The momentum lives
+ * in the Adam m buffer (yl_trainer_buffer kind 2), v of those matrices is left
+ * alone; clip_max_norm clips by the model's whole gradient norm, as without
+ * Muon.  Takes effect with the next step; NULL goes back to Adam everywhere.
+ * The setting is not part of the buffers: set it again after restoring them.  No
+ * counterpart in the reference. */
+typedef struct yl_muon_config {
+  float lr_vae, lr_motion; /* Muon's own learning rates */
+  float momentum;          /* 0 to below 1, e.g. 0.95 */
+  int nesterov;
+  float weight_decay;
+  int steps;               /* Newton-Schulz steps, e.g. 5 */
+} yl_muon_config;
+yl_status yl_trainer_set_muon(yl_trainer* tr, const yl_muon_config* cfg_or_null);
 /* The inference path of Interpolation.swift:263-373 without the file and
  * video IO: frame_a, frame_b are device [3][height][width] frames (the
  * trainer's size), times[count] (host) the frame times in [0, 1].  Writes

@@ -52,6 +52,12 @@ class MuonTensor(C.Structure):
                 ("rows", C.c_int), ("cols", C.c_int), ("scale", C.c_float)]
 
 
+class MuonConfig(C.Structure):
+    """``yl_muon_config``."""
+    _fields_ = [("lr_vae", C.c_float), ("lr_motion", C.c_float), ("momentum", C.c_float),
+                ("nesterov", C.c_int), ("weight_decay", C.c_float), ("steps", C.c_int)]
+
+
 class TrainerConfig(C.Structure):
     """``yl_trainer_config``."""
     _fields_ = [("batch", C.c_int), ("height", C.c_int), ("width", C.c_int),
@@ -161,6 +167,7 @@ SIGNATURES: dict[str, list] = {
     "yl_trainer_step": [P, P, P, P],
     "yl_trainer_step_host": [P, P, P, P],
     "yl_trainer_set_config": [P, C.POINTER(TrainerConfig)],
+    "yl_trainer_set_muon": [P, C.POINTER(MuonConfig)],
     "yl_trainer_param_count": [P, I, C.POINTER(SZ)],
     "yl_trainer_buffer": [P, I, I, C.POINTER(P)],
     "yl_trainer_param_entry": [P, I, I, C.c_char_p, SZ, C.POINTER(SZ), C.POINTER(I)],

@@ -301,8 +301,11 @@ MOTION_ARCH = 6  # latent-space conv U-Net with time MLP (the reference's MLP is
 
 
 def save_trainer(tr, vae_path, motion_path=None, epoch=None, fingerprint=None) -> None:
-    """Both models of a Trainer with their Adam moments and step counter."""
+    """Both models of a Trainer with their Adam moments and step counter, and
+    what its Muon was set to (its momenta are in the m moments)."""
     step = tr.step
+    muon = getattr(tr, "muon", None)
+    more = {"muon": muon} if muon else {}
     for which, path in ((0, vae_path), (1, motion_path)):
         if path is None:
             continue
@@ -316,17 +319,18 @@ def save_trainer(tr, vae_path, motion_path=None, epoch=None, fingerprint=None) -
             save_state(path, mats, epoch=epoch, step=step, fingerprint=fingerprint,
                        optimizer=OptimizerState(step, moments), latent_channels=32,
                        arch_version=VAE_ARCH,
-                       extra_meta={"names": [e.name for e in table]})
+                       extra_meta={"names": [e.name for e in table], **more})
         else:
             save_state(path, mats, epoch=epoch, step=step, fingerprint=fingerprint,
                        optimizer=OptimizerState(step, moments), arch_version=MOTION_ARCH,
                        extra_meta={"format": "YumeLayers Motion UNet",
-                                   "names": [e.name for e in table]})
+                                   "names": [e.name for e in table], **more})
 
 
 def load_trainer(tr, vae_path=None, motion_path=None) -> CheckpointState | None:
     """Weights, Adam moments and step counter back into a Trainer; returns the
-    last loaded state."""
+    last loaded state.  A checkpoint of a Muon run sets Muon again, unless the
+    trainer has a setting of its own."""
     state = None
     for which, path in ((0, vae_path), (1, motion_path)):
         if path is None:
@@ -345,4 +349,7 @@ def load_trainer(tr, vae_path=None, motion_path=None) -> CheckpointState | None:
         tr.upload(which, flat, kind=0)
         if state.optimizer is not None:
             tr.step = state.optimizer.step
+            muon = state.meta.get("muon")
+            if isinstance(muon, dict) and getattr(tr, "muon", None) is None:
+                tr.set_muon(**muon)
     return state

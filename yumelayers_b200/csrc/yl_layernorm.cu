@@ -31,6 +31,9 @@ using namespace yl;
 namespace {
 
 constexpr int kSegRows = 64;  // rows a thread sums in fp32 before a partial is written
+// Backward calls whose rows one block sees in so many turns run in that block
+// alone: 32 x 512 in one kernel of 4 turns, not two kernels.
+constexpr int kAloneTurns = 4;
 
 // ---------------------------------------------------------------- row pieces
 // Element e of a lane's PER elements is column (e / 4 * LANES + lane) * 4 + e % 4
@@ -314,7 +317,14 @@ struct Bwd {
   long long ldadd;
   float* dx;
   long long lddx;
-  float* part;  // [partial][2][cols], or null when neither dgamma nor dbeta is wanted
+  // where column sums go: partial rows [partial][2][cols], or straight to dgamma
+  // and dbeta (either may be null) when one block sees all rows
+  float *part, *dgamma, *dbeta;
+  __device__ bool sums() const { return part || dgamma || dbeta; }
+  __device__ float* out_gamma(long long k) const { return part ? part + 2 * k * cols : dgamma; }
+  __device__ float* out_beta(long long k) const {
+    return part ? part + (2 * k + 1) * cols : dbeta;
+  }
 };
 
 // dx of one row, and its share of the column sums.
@@ -341,7 +351,7 @@ __device__ __forceinline__ void bwd_row(const Bwd& p, long long r, bool valid, i
     s2 *= inv;
   }
   if (!valid) return;
-  if (p.part) {
+  if (p.sums()) {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       dg[k] = fmaf(dy[k], h[k], dg[k]);
@@ -377,9 +387,10 @@ __device__ __forceinline__ void flush_groups(const Bwd& p, long long part, int l
     }
   }
   __syncthreads();
+  float *og = p.out_gamma(part), *ob = p.out_beta(part);
   for (int c = threadIdx.x; c < p.cols; c += THREADS) {
-    p.part[2 * part * p.cols + c] = sums[c];
-    p.part[(2 * part + 1) * p.cols + c] = sums[CAP + c];
+    if (og) og[c] = sums[c];
+    if (ob) ob[c] = sums[CAP + c];
   }
 #pragma unroll
   for (int k = 0; k < PER; ++k) dg[k] = db[k] = 0.f;
@@ -426,10 +437,10 @@ __global__ void __launch_bounds__(THREADS, MIN_BLOCKS) ln_bwd_ring_kernel(const 
     bwd_row<Own<THREADS, LANES>, R, PER>(p, r, r < p.rows, lane, x, dy, ga, m, rs, dg, db, red,
                                          [&](float(&o)[PER]) { Q::take(ring, d, 2, o); });
     ++held;
-    if (p.part && (held == kSegRows || it + 1 == iters)) {
+    if (p.sums() && (held == kSegRows || it + 1 == iters)) {
       if constexpr (kBlock) {
-        R::store(p.part + 2 * part * p.cols, p.cols, lane, dg);
-        R::store(p.part + (2 * part + 1) * p.cols, p.cols, lane, db);
+        if (float* og = p.out_gamma(part)) R::store(og, p.cols, lane, dg);
+        if (float* ob = p.out_beta(part)) R::store(ob, p.cols, lane, db);
 #pragma unroll
         for (int k = 0; k < PER; ++k) dg[k] = db[k] = 0.f;
       } else {
@@ -475,7 +486,7 @@ __global__ void __launch_bounds__(256) ln_bwd_group_kernel(const __grid_constant
                                       R::load(p.addend + (r0 + u * G) * p.ldadd, p.cols, lane, o);
                                     });
     held += UNR;
-    if (p.part && (held + UNR > kSegRows || it + 1 == iters)) {
+    if (p.sums() && (held + UNR > kSegRows || it + 1 == iters)) {
       flush_groups<256, LANES, PER, R>(p, part, lane, grp, dg, db, sums);
       part += gridDim.x;
       held = 0;
@@ -507,9 +518,9 @@ __global__ void __launch_bounds__(THREADS) ln_bwd_block_kernel(const __grid_cons
           [&](float(&o)[PER]) { R::load(p.addend + r * p.ldadd, p.cols, lane, o); });
     }
     ++held;
-    if (p.part && (held == kSegRows || it + 1 == iters)) {
-      R::store(p.part + 2 * part * p.cols, p.cols, lane, dg);
-      R::store(p.part + (2 * part + 1) * p.cols, p.cols, lane, db);
+    if (p.sums() && (held == kSegRows || it + 1 == iters)) {
+      if (float* og = p.out_gamma(part)) R::store(og, p.cols, lane, dg);
+      if (float* ob = p.out_beta(part)) R::store(ob, p.cols, lane, db);
 #pragma unroll
       for (int k = 0; k < PER; ++k) dg[k] = db[k] = 0.f;
       part += gridDim.x;
@@ -777,19 +788,24 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
   DeviceGuard dev(ctx->device);
   YL_CUDA(dev.status());
   Bwd p{x, dy, ldx, lddy, rows, cols, eps, gamma, mean, rstd, dx ? addend : nullptr, ldadd, dx, lddx,
-        nullptr};
+        nullptr, nullptr, nullptr};
   const bool vec = aligned16(x) && aligned16(dy) && aligned16(gamma) && aligned16(p.addend) &&
-                   aligned16(dx) &&
+                   aligned16(dx) && aligned16(dgamma) && aligned16(dbeta) &&
                    ((ldx | lddy | cols | (p.addend ? ldadd : 0) | (dx ? lddx : 0)) & 3) == 0;
   auto launch = [&](auto kernel, int threads, int rows_a_block, int unr, int smem) -> yl_status {
     long long blocks = (rows + rows_a_block - 1) / rows_a_block;
+    // a few turns of one block are quicker than a second kernel for the sums
+    if (blocks <= kAloneTurns && cols <= 8192) blocks = 1;
     YL_TRY(resident(ctx, kernel, threads, smem, &blocks));
     Workspace work;
     // rows a thread adds up per turn, turns per partial row, partial rows of a block
     const long long turns = (rows + blocks * rows_a_block - 1) / (blocks * rows_a_block);
     const long long per_part = kSegRows / unr;
     const long long parts = blocks * ((turns + per_part - 1) / per_part);
-    if (dgamma || dbeta) {
+    if (parts == 1 && cols <= 8192) {
+      p.dgamma = dgamma;
+      p.dbeta = dbeta;
+    } else if (dgamma || dbeta) {
       char* ws = nullptr;
       YL_TRY(work.get(ctx, (size_t)parts * 2 * cols * sizeof(float), &ws));
       p.part = (float*)ws;

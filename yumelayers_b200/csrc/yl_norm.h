@@ -38,10 +38,11 @@ struct AdamTensor {
 // Multi-tensor Adam.  grads are multiplied by grad_scale, non-finite values
 // are zeroed when sanitize != 0, and when clip_max_norm > 0 the global L2
 // norm is clipped (GradSanitize.swift:18-101); norm_out (device, optional)
-// receives the pre-clip norm.  Bias corrections use step t >= 1.
+// receives the pre-clip norm.  Bias corrections use step t >= 1.  norm_given
+// (device, optional) is the norm to clip by instead of this table's own.
 yl_status adam_multi(yl_ctx* ctx, const AdamTensor* tensors, int count, float lr, float b1,
                      float b2, float eps, int t, float grad_scale, float clip_max_norm,
-                     int sanitize, float* norm_out);
+                     int sanitize, float* norm_out, const float* norm_given = nullptr);
 
 // Linear: Y = X W^T + b (W is [oc][ic]); backward outputs optional; with
 // accumulate != 0 all of dX, dW, db are added to.

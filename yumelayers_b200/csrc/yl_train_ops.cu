@@ -132,14 +132,14 @@ __global__ void adam_update_kernel(const __grid_constant__ AdamPack p, float lr,
 
 yl_status adam_multi(yl_ctx* ctx, const AdamTensor* tensors, int count, float lr, float b1,
                      float b2, float eps, int t, float grad_scale, float clip_max_norm,
-                     int sanitize, float* norm_out) {
+                     int sanitize, float* norm_out, const float* norm_given) {
   YL_CHECK(count >= 0, YL_ERR_INVALID, "adam_multi: negative tensor count");
   if (t < 1) t = 1;
   const float c1 = 1.f - powf(b1, (float)t), c2 = 1.f - powf(b2, (float)t);
   const int nb = ctx->num_sms * 4;
   float* norm = norm_out;
   void* ws = nullptr;
-  const bool need_norm = clip_max_norm > 0.f || norm_out;
+  const bool need_norm = !norm_given && (clip_max_norm > 0.f || norm_out);
   if (need_norm) {
     YL_TRY(scratch_get(ctx, nb * sizeof(double) + 256, &ws));
     if (!norm) norm = (float*)((char*)ws + nb * sizeof(double));
@@ -169,7 +169,8 @@ yl_status adam_multi(yl_ctx* ctx, const AdamTensor* tensors, int count, float lr
     const long long items = p.istart[p.count];
     const int grid = (int)std::min<long long>(items, (long long)ctx->num_sms * 8);
     adam_update_kernel<<<grid, 256, 0, ctx->stream>>>(
-        p, lr, b1, b2, eps, c1, c2, grad_scale, sanitize, clip_max_norm, need_norm ? norm : nullptr);
+        p, lr, b1, b2, eps, c1, c2, grad_scale, sanitize, clip_max_norm,
+        norm_given ? norm_given : need_norm ? norm : nullptr);
     YL_TRY(check_launch("adam_update_kernel"));
   }
   return YL_OK;

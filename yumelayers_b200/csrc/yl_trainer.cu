@@ -25,6 +25,7 @@
 #include <string>
 #include <vector>
 
+#include "yl_muon.h"
 #include "yl_nets.h"
 #include "yl_norm.h"
 #include "yume_c.h"
@@ -145,6 +146,45 @@ void hook_fn(void* arg, Net* net, size_t lo) { launch_ready((Overlap*)arg, net, 
 
 }  // namespace
 
+namespace {
+// How a model's flat buffers divide between the two optimisers: the hidden
+// weight matrices (every conv and Linear weight but those of the convs that read
+// the model's input and write its output) for Muon, the ranges between them for
+// Adam.
+struct MuonTables {
+  std::vector<yl_muon_tensor> matrices;
+  std::vector<AdamTensor> rest;
+};
+
+MuonTables muon_tables_of(const Net& net, const char* first, const char* last) {
+  MuonTables t;
+  const ParamSet& p = net.params;
+  size_t at = 0;  // parameters behind this offset are not in a table yet
+  auto rest_until = [&](size_t end) {
+    if (end > at) t.rest.push_back({p.w + at, p.g + at, p.m + at, p.v + at, (long long)(end - at)});
+  };
+  for (const ParamEntry& e : net.param_table) {
+    const bool conv = e.d2 >= 1 && e.d1 >= 1 && e.name.size() > 7 &&
+                      e.name.compare(e.name.size() - 7, 7, ".weight") == 0;
+    const bool linear = e.d2 == 0;
+    if ((!conv && !linear) || e.name == std::string(first) + ".weight" ||
+        e.name == std::string(last) + ".weight")
+      continue;
+    // conv weights are stored [oc][k*k][ic rounded up to 4]; the padding's
+    // gradients are zero, and zero columns stay zero
+    const int rows = conv ? (e.d0 + 3) & ~3 : e.d0;
+    const int cols = conv ? e.d2 * e.d3 * ((e.d1 + 3) & ~3) : e.d1;
+    rest_until(e.offset);
+    const float scale =
+        std::sqrt(std::max(1.f, (float)e.d0 / (float)(conv ? e.d1 * e.d2 * e.d3 : e.d1)));
+    t.matrices.push_back({p.w + e.offset, p.g + e.offset, p.m + e.offset, rows, cols, scale});
+    at = e.offset + (size_t)rows * cols;
+  }
+  rest_until(p.count);
+  return t;
+}
+}  // namespace
+
 struct yl_trainer {
   yl_ctx* ctx = nullptr;
   yl_comm* comm = nullptr;
@@ -156,6 +196,9 @@ struct yl_trainer {
   float *ia = nullptr, *ib = nullptr;  // interpolation: latents of A and B, one copy per slot
   cudaEvent_t comm_done = nullptr;
   int64_t step = 0;
+  bool muon_on = false;  // hidden weight matrices are updated by Muon
+  yl_muon_config muon{};
+  MuonTables muon_tables[2];  // VAE, U-Net
   double prof_ms[kProfClasses] = {}, prof_flops[kProfClasses] = {}, prof_bytes[kProfClasses] = {};
   int prof_launches[kProfClasses] = {};
   double prof_exec[kProfClasses] = {};
@@ -314,7 +357,33 @@ yl_status yl_trainer_destroy(yl_trainer* tr) {
   return YL_OK;
 }
 
+// One optimiser step with Muon for the hidden matrices and Adam for the rest;
+// both clip by the model's whole gradient norm.
+static yl_status muon_step(yl_trainer* tr, Net& net, const MuonTables& t, float lr, float muon_lr,
+                           float scale) {
+  const float clip = tr->cfg.clip_max_norm;
+  const int sanitize = clip > 0.f ? 1 : 0;
+  float* norm = nullptr;
+  if (clip > 0.f) {
+    norm = tr->losses + 16;
+    YL_TRY(grad_norm(tr->ctx, net.params.g, (long long)net.params.count, scale, sanitize, norm));
+  }
+  MuonStep st;
+  st.lr = muon_lr, st.momentum = tr->muon.momentum, st.nesterov = tr->muon.nesterov != 0;
+  st.weight_decay = tr->muon.weight_decay, st.steps = tr->muon.steps;
+  st.grad_scale = scale, st.clip_max_norm = clip, st.sanitize = sanitize;
+  YL_TRY(muon_multi(tr->ctx, t.matrices.data(), (int)t.matrices.size(), st, nullptr, norm, nullptr));
+  YL_TRY(adam_multi(tr->ctx, t.rest.data(), (int)t.rest.size(), lr, 0.9f, 0.999f, 1e-8f,
+                    (int)tr->step, scale, clip, sanitize, nullptr, norm));
+  return net.prepare_weights();
+}
+
 static yl_status adam_step(yl_trainer* tr, Net& net, float lr, float scale) {
+  if (tr->muon_on) {
+    const bool vae = &net == tr->vae.get();
+    return muon_step(tr, net, tr->muon_tables[vae ? 0 : 1], lr,
+                     vae ? tr->muon.lr_vae : tr->muon.lr_motion, scale);
+  }
   AdamTensor t{net.params.w, net.params.g, net.params.m, net.params.v,
                (long long)net.params.count};
   const float clip = tr->cfg.clip_max_norm;
@@ -652,6 +721,33 @@ yl_status yl_trainer_set_config(yl_trainer* tr, const yl_trainer_config* cfg) {
                cfg->width == tr->cfg.width,
            YL_ERR_SHAPE, "yl_trainer_set_config: batch and frame size are fixed at creation");
   tr->cfg = *cfg;
+  return YL_OK;
+}
+
+yl_status yl_trainer_set_muon(yl_trainer* tr, const yl_muon_config* cfg) {
+  YL_CHECK(tr, YL_ERR_INVALID, "yl_trainer_set_muon: trainer is NULL");
+  if (!cfg) {
+    tr->muon_on = false;
+    return YL_OK;
+  }
+  YL_CHECK(std::isfinite(cfg->lr_vae) && std::isfinite(cfg->lr_motion) &&
+               std::isfinite(cfg->weight_decay) && cfg->weight_decay >= 0.f,
+           YL_ERR_INVALID, "yl_trainer_set_muon: learning rates %g, %g, weight decay %g",
+           (double)cfg->lr_vae, (double)cfg->lr_motion, (double)cfg->weight_decay);
+  YL_CHECK(cfg->momentum >= 0.f && cfg->momentum < 1.f, YL_ERR_INVALID,
+           "yl_trainer_set_muon: momentum %g (0 to below 1)", (double)cfg->momentum);
+  YL_CHECK(cfg->steps >= 1 && cfg->steps <= 32, YL_ERR_INVALID,
+           "yl_trainer_set_muon: %d steps (1 to 32)", cfg->steps);
+  try {
+    if (tr->muon_tables[0].matrices.empty()) {
+      tr->muon_tables[0] = muon_tables_of(*tr->vae, "enc.conv_in", "dec.conv_out");
+      tr->muon_tables[1] = muon_tables_of(*tr->unet, "conv_in", "conv_out");
+    }
+  } catch (const std::bad_alloc&) {
+    return set_error(YL_ERR_OOM, "yl_trainer_set_muon: no host memory");
+  }
+  tr->muon = *cfg;
+  tr->muon_on = true;
   return YL_OK;
 }
 

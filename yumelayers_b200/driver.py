@@ -101,13 +101,21 @@ def run_training(trainer, next_batch, *, epochs: int, epoch_steps: int, start_ep
     next_batch(epoch, step) -> (frames [3][B][3][H][W], t [B]) host arrays.
     save(epoch_next, step_in_epoch) writes a checkpoint (every `save_every`
     steps and after each completed epoch); it is never called after a NaN.
-    warmup_steps > 0 ramps both learning rates over the first steps of this
-    run (for resumes without optimizer state).  Cancel is checked before every
+    warmup_steps > 0 ramps all learning rates, Muon's among them, over the first
+    steps of this run (for resumes without optimizer state).  Cancel is checked before every
     step; a stopped epoch is neither reported nor checkpointed.
     """
     control = control or TrainingControl()
     res = RunResult()
     base = (trainer.cfg.lr_vae, trainer.cfg.lr_motion)
+    muon = dict(getattr(trainer, "muon", None) or {})
+
+    def set_rates(f):
+        trainer.set_config(lr_vae=base[0] * f, lr_motion=base[1] * f)
+        if muon:
+            trainer.set_muon(**{**muon, "lr_vae": muon["lr_vae"] * f,
+                                "lr_motion": muon["lr_motion"] * f})
+
     run_step = 0
     for ep in range(max(0, start_epoch), epochs):
         if control.cancelled:
@@ -123,8 +131,7 @@ def run_training(trainer, next_batch, *, epochs: int, epoch_steps: int, start_ep
                 stopped = True
                 break
             if warmup_steps > 0:
-                f = resume_warmup_factor(run_step + 1, warmup_steps)
-                trainer.set_config(lr_vae=base[0] * f, lr_motion=base[1] * f)
+                set_rates(resume_warmup_factor(run_step + 1, warmup_steps))
             t0 = time.perf_counter()
             frames, t = next_batch(ep, si)
             losses = trainer.step_host(frames, t)
@@ -149,5 +156,5 @@ def run_training(trainer, next_batch, *, epochs: int, epoch_steps: int, start_ep
         if save:
             save(ep + 1, 0)
     if warmup_steps > 0:
-        trainer.set_config(lr_vae=base[0], lr_motion=base[1])
+        set_rates(1.0)
     return res

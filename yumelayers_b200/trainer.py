@@ -13,7 +13,8 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from ._lib import KernelStats, TemplateStats, TrainerConfig, YumeError, call, lib
+from ._lib import (KernelStats, MuonConfig, TemplateStats, TrainerConfig, YumeError, call,
+                   lib)
 from .session import Context
 
 
@@ -111,6 +112,7 @@ class Trainer:
         self.ctx = ctx or Context.shared(0)
         self.cfg = cfg
         self.comm = comm
+        self.muon: dict | None = None  # what set_muon was given
         h = C.c_void_p()
         call("yl_trainer_create", self.ctx.handle, C.byref(cfg), comm.handle if comm else None,
              C.byref(h))
@@ -133,6 +135,21 @@ class Trainer:
         for k, v in kw.items():
             setattr(self.cfg, k, v)
         call("yl_trainer_set_config", self.handle, C.byref(self.cfg))
+
+    def set_muon(self, lr_vae=0.02, lr_motion=0.02, momentum=0.95, nesterov=True,
+                 weight_decay=0.0, steps=5) -> None:
+        """Muon for the hidden weight matrices from the next step on, Adam for the
+        rest (yl_trainer_set_muon)."""
+        kw = dict(lr_vae=float(lr_vae), lr_motion=float(lr_motion), momentum=float(momentum),
+                  nesterov=bool(nesterov), weight_decay=float(weight_decay), steps=int(steps))
+        cfg = MuonConfig(**{k: int(v) if k == "nesterov" else v for k, v in kw.items()})
+        call("yl_trainer_set_muon", self.handle, C.byref(cfg))
+        self.muon = kw
+
+    def unset_muon(self) -> None:
+        """Adam for every parameter again."""
+        call("yl_trainer_set_muon", self.handle, None)
+        self.muon = None
 
     # -- stepping --
     def step_device(self, frames_ptr: int, t_ptr: int, losses_ptr: int | None = None) -> None:
