@@ -332,8 +332,9 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
  * past 4 are YL_ERR_UNSUPPORTED; sides go to 65536.  y may be x itself (same
  * stride); any other overlap between a result and another matrix of the table
  * is YL_ERR_INVALID.  An empty matrix is skipped, a zero matrix gives zeros, and
- * one with a NaN or an infinity gives NaN and leaves the others alone.
- * No counterpart in the reference. */
+ * one with a NaN or an infinity gives NaN and leaves the others alone.  Equal
+ * calls give equal bits; a matrix in another table may come out with other
+ * roundings.  No counterpart in the reference. */
 typedef struct yl_ns_matrix {
   const float* x;
   float* y;
@@ -352,8 +353,9 @@ yl_status yl_newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, in
  * with NS, steps, coeffs and eps as in yl_newton_schulz.  scale is each matrix's
  * own factor on lr, e.g. sqrt(max(1, rows / cols)).  norm_out_dev (optional)
  * receives the pre-clip norm.  Parameters and momenta must not overlap anything
- * else in the table (YL_ERR_INVALID).  Summation orders are fixed: equal inputs
- * give equal bits.  No counterpart in the reference. */
+ * else in the table (YL_ERR_INVALID).  Equal calls give equal bits; a matrix in
+ * another table may come out with other roundings.  No counterpart in the
+ * reference. */
 typedef struct yl_muon_tensor {
   float* param;
   const float* grad;

@@ -77,6 +77,7 @@ struct Table {
   int chunks[kMaxItems + 1];    // norm chunks before each item
   int count;
   int pair;                     // worked on by pairs of blocks, 256 x 256 tiles
+  int chip;                     // stays in shared memory
   int* ctrl;                    // ticket counter, done[item][3], arrivals of split GRAM tiles
   int ctrl_ints;
 };
@@ -969,6 +970,433 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   }
 }
 
+// ---------------------------------------------------------------- short matrices
+// Matrices with a shorter side of at most 128 stay on the chip: a cluster of
+// blocks holds the pairs of X in shared memory, each block its share of the long
+// side, from the first read of the input to the write of the result, and one
+// launch does the norm, all steps and the update.  Per step each block multiplies
+// its share of the Gram sum, the blocks exchange the sums through distributed
+// shared memory (every block adds up a few columns in rank order and hands the
+// finished columns to all), and each forms P for itself and updates its share.
+// 128 x 1152 takes the steps kernel 15 trips through memory and its counters
+// (about 5 us each); here a step is bound by its 84 MMAs of 117 cycles and four
+// cluster barriers.
+constexpr int kChipBlocks = 4;                       // most 64-blocks of a block's share
+constexpr int kChipShare = 16;                       // most blocks of a cluster
+constexpr int kChipXPlane = kChipBlocks * 2 * kBlkBytes;
+constexpr int kChipAOff = 2 * kChipXPlane;           // A, then P; before that the Gram sums
+constexpr int kChipAPlane = 4 * kBlkBytes;
+constexpr int kChipBarOff = kChipAOff + 2 * kChipAPlane;
+constexpr int kChipSmem = kChipBarOff + 512 + 1024;  // barrier and norms, alignment
+constexpr int kChipThreads = 256;
+
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint4 v) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
+               "r"(v.z), "r"(v.w)
+               : "memory");
+}
+__device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
+}
+
+// Sums the accumulators 0 .. n-1 of a warp's 32 rows x 64 columns.
+__device__ __forceinline__ void sum_accumulators(uint32_t at, int n, float (&v)[64]) {
+#pragma unroll
+  for (int c = 0; c < 64; ++c) v[c] = 0.f;
+#pragma unroll 1
+  for (int a = 0; a < n; ++a) {
+    uint32_t acc[2][16];
+    tmem_ld_32x32b_x16(at + a * 128, acc[0]);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      tmem_ld_wait();
+      if (p < 3) tmem_ld_32x32b_x16(at + a * 128 + (p + 1) * 16, acc[(p + 1) & 1]);
+#pragma unroll
+      for (int c = 0; c < 16; ++c) v[p * 16 + c] += __uint_as_float(acc[p & 1][c]);
+    }
+  }
+}
+
+// Eight values as a 16-byte chunk of either plane.
+__device__ __forceinline__ void split8(const float* v, uint4* hi, uint4* lo) {
+  __half2 h[4], l[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+    const float2 f = __half22float2(h[j]);
+    l[j] = __floats2half2_rn(v[2 * j] - f.x, v[2 * j + 1] - f.y);
+  }
+  *hi = *reinterpret_cast<const uint4*>(h);
+  *lo = *reinterpret_cast<const uint4*>(l);
+}
+
+__global__ void __launch_bounds__(kChipThreads, 1)
+    ns_chip_kernel(const __grid_constant__ Table t, const __grid_constant__ Steps steps,
+                   const __grid_constant__ Update u, float sx0, int share, int* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint64_t* done = reinterpret_cast<uint64_t*>(smem + kChipBarOff);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  double* norms = reinterpret_cast<double*>(smem + kChipBarOff + 64);  // [kChipShare]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wr = warp & 3, wc = warp >> 2;
+  const int rank = (int)cluster_rank();
+  const Item& it = t.it[blockIdx.x / share];
+  const bool tall = it.rows > it.cols;
+  const int mb = it.mb, nb = max(it.rb, it.cb);
+  const int w = (nb + share - 1) / share;  // blocks of a share
+  const int first = rank * w, mw = max(0, min(w, nb - first));
+  const long long lim = wait_limit(err);
+  if (tid == 0) {
+    mbar_init(done, 1);
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+
+  // ---- the input: momentum step, norm, pairs.  A unit is 8 columns of a row;
+  // a thread keeps all of its units in registers between the two.
+  constexpr int kUnits = kChipBlocks * 2 * 64 * 8 / kChipThreads;
+  float v[kUnits][8];
+  const float clipf = u.muon ? clip_factor(u) : 1.f;
+  // blocks of the share, in rows and in columns
+  const int brows = tall ? mw : mb, bcols = tall ? mb : mw;
+  const long long row0 = tall ? (long long)first * kBlk : 0;
+  const long long col0 = tall ? 0 : (long long)first * kBlk;
+  const int units = brows * kBlk * bcols * 8;
+  double sq = 0.0;
+#pragma unroll
+  for (int e = 0; e < kUnits; ++e) {
+    const int un = tid + e * kChipThreads;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[e][j] = 0.f;
+    if (un >= units) continue;
+    const int rr = un / (bcols * 8), cc = un - rr * bcols * 8;
+    const long long r = row0 + rr, c = col0 + cc * 8;
+    if (r >= it.rows || c >= it.cols) continue;
+    const float* x = it.src + r * it.lds + c;
+    const int n = (int)min(8LL, it.cols - c);
+    float g[8], m[8];
+    const bool vec = it.vec && n == 8;
+    if (vec) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(x) + q);
+        g[4 * q] = f.x, g[4 * q + 1] = f.y, g[4 * q + 2] = f.z, g[4 * q + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = j < n ? __ldg(x + j) : 0.f;
+    }
+    if (!u.muon) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[e][j] = g[j];
+      continue;
+    }
+    float* mo = it.mom + r * it.cols + c;
+    if (vec) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const float4 f = reinterpret_cast<const float4*>(mo)[q];
+        m[4 * q] = f.x, m[4 * q + 1] = f.y, m[4 * q + 2] = f.z, m[4 * q + 3] = f.w;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m[j] = j < n ? mo[j] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float gv = clean(g[j], u, clipf);
+      m[j] = u.mu * m[j] + gv;
+      v[e][j] = j < n ? (u.nesterov ? gv + u.mu * m[j] : m[j]) : 0.f;
+    }
+    if (vec) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        reinterpret_cast<float4*>(mo)[q] =
+            make_float4(m[4 * q], m[4 * q + 1], m[4 * q + 2], m[4 * q + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < n) mo[j] = m[j];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kUnits; ++e)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sq += (double)v[e][j] * v[e][j];
+  sq = block_sum256(sq);
+  cluster_arrive();  // every block of the cluster runs: its shared memory can be written
+  cluster_wait();
+  if (tid < share) st_cluster_f64(map_to_rank(smem_u32(norms + rank), tid), sq);
+  cluster_arrive();
+  cluster_wait();
+  double total = 0.0;
+  for (int r = 0; r < share; ++r) total += norms[r];
+  const float inv = (float)(1.0 / (sqrt(total) + (double)u.eps));
+
+  // Block (long, short) of the share: a wide X keeps its two row blocks together
+  // (128 rows of a K-major operand), a tall one its row blocks.
+  auto xoff = [&](int lb, int sb) {
+    return (uint32_t)((tall ? sb * kChipBlocks + lb : lb * 2 + sb) * kBlkBytes);
+  };
+#pragma unroll
+  for (int e = 0; e < kUnits; ++e) {
+    const int un = tid + e * kChipThreads;
+    if (un >= units) continue;
+    const int rr = un / (bcols * 8), cc = un - rr * bcols * 8;
+    const int rblk = rr >> 6, r = rr & 63, cblk = cc >> 3, ch = cc & 7;
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = v[e][j] * inv * sx0;
+    uint4 hi, lo;
+    split8(x, &hi, &lo);
+    uint8_t* at = smem + (tall ? xoff(rblk, cblk) : xoff(cblk, rblk)) + r * 128 + ((ch ^ (r & 7)) << 4);
+    *reinterpret_cast<uint4*>(at) = hi;
+    *reinterpret_cast<uint4*>(at + kChipXPlane) = lo;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t lanes = tmem + ((uint32_t)(wr * 32) << 16) + (uint32_t)(wc * 64);
+  const uint32_t xs = smem_u32(smem), as = smem_u32(smem + kChipAOff);
+  uint32_t waits = 0;
+
+  // Products of `kks` 16-deep slices, `chain` to an accumulator; operand(kk) gives
+  // the hi plane's two descriptors, the lo planes lie `lplane`, `rplane` bytes on.
+  auto multiply = [&](int kks, int chain, uint32_t idesc, uint32_t lplane, uint32_t rplane,
+                      auto descriptors) {
+    fence_proxy_async_all();  // shared memory written by this block's threads
+    __syncthreads();
+    if (tid == 0) {
+      tc_fence_after();
+      for (int k0 = 0, a = 0; k0 < kks; k0 += chain, ++a) {
+        const int k1 = min(kks, k0 + chain);
+#pragma unroll 1
+        for (int part = 0; part < 3; ++part)  // lo hi, hi lo, hi hi
+          for (int kk = k0; kk < k1; ++kk) {
+            uint64_t ld, rd;
+            descriptors(kk, &ld, &rd);
+            ld += part == 0 ? lplane >> 4 : 0;
+            rd += part == 1 ? rplane >> 4 : 0;
+            umma_f16(tmem + a * 128, ld, rd, idesc, (part | (kk - k0)) != 0);
+          }
+      }
+      umma_commit(done);
+    }
+    const uint32_t parity = waits++ & 1;
+    if (!mbar_wait(done, parity, lim)) {
+      // too slow for the caller's limit: say so, but let the products finish, since
+      // they still read this block's shared memory
+      report_error(err, YL_DEVERR_TIMEOUT);
+      mbar_wait(done, parity);
+    }
+    tc_fence_after();
+  };
+  // accumulators are read again before the next multiply overwrites them
+  auto drained = [&]() { tc_fence_before(); };
+
+  const int per = max(1, 8 * mb / share);  // 8-column chunks of A that a block adds up
+  for (int s = 0; s < steps.n; ++s) {
+    // ---- this share of A = X X^T (X^T X)
+    const int kks = 4 * mw, gchain = max(1, (kks + 3) / 4);
+    if (kks > 0)
+      multiply(kks, gchain, idesc_f16(128, mb * 64, tall, tall), kChipXPlane, kChipXPlane,
+               [&](int kk, uint64_t* l, uint64_t* r) {
+                 const uint32_t at = xs + xoff(kk >> 2, 0) + (kk & 3) * (tall ? 2048 : 32);
+                 *l = *r = sw128_desc(at, tall ? kChipBlocks * kBlkBytes : 16, 1024);
+               });
+    float p[64];
+    sum_accumulators(lanes, kks > 0 ? (kks + gchain - 1) / gchain : 0, p);
+    drained();
+    if (s > 0) cluster_wait();  // no block needs its P any more
+    else {
+      cluster_arrive();
+      cluster_wait();
+    }
+    // ---- sums to the blocks that add them up: [rank][chunk][row][8]
+    if (wc < mb) {
+#pragma unroll
+      for (int ch = 0; ch < 8; ++ch) {
+        const int c = wc * 8 + ch, owner = c / per;
+        const uint32_t to = map_to_rank(
+            as + (uint32_t)(((rank * per + (c - owner * per)) * 128 + wr * 32 + lane) * 32), owner);
+        st_cluster_v4(to, *reinterpret_cast<const uint4*>(p + ch * 8));
+        st_cluster_v4(to + 16, *reinterpret_cast<const uint4*>(p + ch * 8 + 4));
+      }
+    }
+    cluster_arrive();
+    cluster_wait();
+    const int row = tid & 127;
+    const bool adds = row < mb * 64;
+    uint4 hi[8], lo[8];  // this thread's chunks: at most 16 of a single block, two threads a row
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int lc = (tid >> 7) + 2 * i;
+      if (!adds || lc >= per || rank * per + lc >= 8 * mb) continue;
+      float a[8] = {};
+      for (int r = 0; r < share; ++r) {
+        const float4* q =
+            reinterpret_cast<const float4*>(smem + kChipAOff + ((r * per + lc) * 128 + row) * 32);
+        const float4 x = q[0], y = q[1];
+        a[0] += x.x, a[1] += x.y, a[2] += x.z, a[3] += x.w;
+        a[4] += y.x, a[5] += y.y, a[6] += y.z, a[7] += y.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] *= steps.g2[s];
+      split8(a, &hi[i], &lo[i]);
+    }
+    cluster_arrive();  // every block has read its sums
+    cluster_wait();
+    // ---- finished columns to every block: A's blocks [column block][row block]
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int lc = (tid >> 7) + 2 * i, c = rank * per + lc;
+      if (!adds || lc >= per || c >= 8 * mb) continue;
+      const uint32_t at = as + (uint32_t)(((c >> 3) * 2 + (row >> 6)) * kBlkBytes + (row & 63) * 128 +
+                                          (((c & 7) ^ (row & 7)) << 4));
+      for (int r = 0; r < share; ++r) {
+        const uint32_t to = map_to_rank(at, r);
+        st_cluster_v4(to, hi[i]);
+        st_cluster_v4(to + kChipAPlane, lo[i]);
+      }
+    }
+    fence_proxy_async_all();
+    cluster_arrive();
+    cluster_wait();
+    // ---- P = s0 I + s1 A + s2 A A, over A
+    multiply(4 * mb, 2, idesc_f16(128, mb * 64, 0, 0), kChipAPlane, kChipAPlane,
+             [&](int kk, uint64_t* l, uint64_t* r) {
+               *l = *r = sw128_desc(as + (kk >> 2) * 2 * kBlkBytes + (kk & 3) * 32, 16, 1024);
+             });
+    sum_accumulators(lanes, 2 * mb, p);
+    drained();
+    if (wc < mb && (wr >> 1) < mb) {
+      const int r64 = (wr & 1) * 32 + lane;
+      uint8_t* blk = smem + kChipAOff + (wc * 2 + (wr >> 1)) * kBlkBytes + r64 * 128;
+      const float s0 = steps.s0[s], s1 = steps.s1[s], s2 = steps.s2[s];
+#pragma unroll
+      for (int ch = 0; ch < 8; ++ch) {
+        uint8_t* at = blk + ((ch ^ (r64 & 7)) << 4);
+        const uint4 h4 = *reinterpret_cast<const uint4*>(at);
+        const uint4 l4 = *reinterpret_cast<const uint4*>(at + kChipAPlane);
+        const __half2* h = reinterpret_cast<const __half2*>(&h4);
+        const __half2* l = reinterpret_cast<const __half2*>(&l4);
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 hf = __half22float2(h[j]), lf = __half22float2(l[j]);
+          o[2 * j] = s2 * p[ch * 8 + 2 * j] + s1 * (hf.x + lf.x);
+          o[2 * j + 1] = s2 * p[ch * 8 + 2 * j + 1] + s1 * (hf.y + lf.y);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (wc == (wr >> 1) && r64 == ch * 8 + j) o[j] += s0;
+        uint4 a, b;
+        split8(o, &a, &b);
+        *reinterpret_cast<uint4*>(at) = a;
+        *reinterpret_cast<uint4*>(at + kChipAPlane) = b;
+      }
+    }
+    // ---- X' = P X (X P), two blocks of the long side at a time
+    const bool last = s + 1 == steps.n;
+    for (int hf = 0; 2 * hf < mw; ++hf) {
+      const int hb = min(2, mw - 2 * hf);
+      const uint32_t idesc =
+          tall ? idesc_f16(128, mb * 64, 0, 0) : idesc_f16(128, hb * 64, 0, 1);
+      multiply(4 * mb, 2, idesc, tall ? kChipXPlane : kChipAPlane, tall ? kChipAPlane : kChipXPlane,
+               [&](int kk, uint64_t* l, uint64_t* r) {
+                 const int sb = kk >> 2, q = kk & 3;
+                 const uint64_t pd = sw128_desc(as + sb * 2 * kBlkBytes + q * 32, 16, 1024);
+                 if (tall) {
+                   *l = sw128_desc(xs + xoff(2 * hf, sb) + q * 32, 16, 1024);
+                   *r = pd;
+                 } else {
+                   *l = pd;
+                   *r = sw128_desc(xs + xoff(2 * hf, sb) + q * 2048, 2 * kBlkBytes, 1024);
+                 }
+               });
+      sum_accumulators(lanes, 2 * mb, p);
+      drained();
+      const int lrow = tall ? 2 * hf + (wr >> 1) : (wr >> 1);  // row and column block of the share
+      const int lcol = tall ? wc : 2 * hf + wc;
+      const bool inside = lrow < brows && lcol < bcols;
+      const float c2 = steps.u2[s];
+      if (inside) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) p[c] *= c2;
+      }
+      if (!last) {
+        if (inside) {
+          const int r64 = (wr & 1) * 32 + lane;
+          uint8_t* blk = smem + (tall ? xoff(lrow, lcol) : xoff(lcol, lrow)) + r64 * 128;
+#pragma unroll
+          for (int ch = 0; ch < 8; ++ch) {
+            uint4 a, b;
+            split8(p + ch * 8, &a, &b);
+            uint8_t* at = blk + ((ch ^ (r64 & 7)) << 4);
+            *reinterpret_cast<uint4*>(at) = a;
+            *reinterpret_cast<uint4*>(at + kChipXPlane) = b;
+          }
+        }
+        continue;
+      }
+      // the result, 32 rows x 32 columns at a time through this half's own blocks
+      if (inside) {
+        float* st = reinterpret_cast<float*>(
+            smem + (tall ? (wc * kChipBlocks + 2 * hf) * kBlkBytes + wr * 4096
+                         : hf * 4 * kBlkBytes + warp * 4096));
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) st[lane * 32 + ((c + lane) & 31)] = p[half * 32 + c];
+          __syncwarp();
+          const long long r0 = row0 + lrow * kBlk + (wr & 1) * 32;
+          const long long col = col0 + lcol * kBlk + half * 32 + lane;
+          if (col < it.cols) {
+            const int nr = (int)max(0LL, min(32LL, it.rows - r0));
+            float* d = it.dst + r0 * it.ldd + col;
+#pragma unroll 1
+            for (int r1 = 0; r1 < nr; r1 += 16) {
+              float pv[16];
+              if (u.muon) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  pv[r] = r1 + r < nr ? __ldcs(d + (r1 + r) * it.ldd) : 0.f;
+              }
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                float x = st[(r1 + r) * 32 + ((lane + r1 + r) & 31)];
+                if (u.muon) x = pv[r] * (1.f - u.lr * u.decay) - u.lr * it.scale * x;
+                if (r1 + r < nr) __stcs(d + (r1 + r) * it.ldd, x);
+              }
+            }
+          }
+        }
+      }
+    }
+    __syncthreads();
+    cluster_arrive();  // this block's P may be overwritten; waited for in the next step
+  }
+  cluster_wait();  // no block leaves while another may still write to it
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
 // ---------------------------------------------------------------- host side
 // Sizes the table's workspace, or (with a base address) places it; returns the
 // bytes it takes.
@@ -1035,7 +1463,57 @@ struct Schedule {
   float sa[kMaxSteps], sp[kMaxSteps];
 };
 
+// Coefficients with the scales of the pairs folded in.
+Steps scaled_steps(const Schedule& s) {
+  Steps st;
+  st.n = s.steps;
+  for (int k = 0; k < s.steps; ++k) {
+    const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
+    st.g2[k] = sa / (sx * sx);
+    st.s0[k] = s.q[3 * k] * sp;
+    st.s1[k] = s.q[3 * k + 1] * sp / sa;
+    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa);
+    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx);
+  }
+  return st;
+}
+
+// Whether a matrix can stay on the chip.
+bool on_chip(const Item& it) {
+  return std::min(it.rows, it.cols) <= 2 * kBlk &&
+         std::max(it.rows, it.cols) <= kChipShare * kChipBlocks * kBlk;
+}
+
+yl_status run_chip(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s) {
+  place(&t, ctx->num_sms, nullptr);  // sizes only: nothing of these is in the workspace
+  int longest = 0;
+  for (int k = 0; k < t.count; ++k) longest = std::max({longest, t.it[k].rb, t.it[k].cb});
+  // as many blocks to a matrix as its long side needs, and more while SMs are idle
+  int share = 1;
+  while (share * kChipBlocks < longest) share *= 2;
+  while (share < 8 && share < longest && 2 * share * t.count <= ctx->num_sms) share *= 2;
+  YL_CUDA(cudaFuncSetAttribute(ns_chip_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kChipSmem));
+  if (share > 8)
+    YL_CUDA(cudaFuncSetAttribute(ns_chip_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(t.count * share);
+  cfg.blockDim = dim3(kChipThreads);
+  cfg.dynamicSmemBytes = kChipSmem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = share;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  YL_CUDA(cudaLaunchKernelEx(&cfg, ns_chip_kernel, t, scaled_steps(s), u, s.sx[0], share,
+                             ctx->dev_err));
+  return check_launch("ns_chip_kernel");
+}
+
 yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, char* ws) {
+  if (t.chip) return run_chip(ctx, t, u, s);
   place(&t, ctx->num_sms, ws);
   const int ctas = t.pair ? 2 : 1, side = 2 * ctas;
   auto tiles = [&](int v) { return (v + side - 1) / side; };
@@ -1059,16 +1537,7 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   }
   ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0]);
   YL_TRY(check_launch("ns_split_kernel"));
-  Steps st;
-  st.n = s.steps;
-  for (int k = 0; k < s.steps; ++k) {
-    const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
-    st.g2[k] = sa / (sx * sx);
-    st.s0[k] = s.q[3 * k] * sp;
-    st.s1[k] = s.q[3 * k + 1] * sp / sa;
-    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa);
-    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx);
-  }
+  const Steps st = scaled_steps(s);
   const int widest = std::max(t.tiles[GRAM][t.count], t.tiles[UPDATE][t.count]);
   const int workers = std::min(widest, ctx->num_sms / ctas);
   cudaLaunchConfig_t cfg = {};
@@ -1096,13 +1565,17 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
 // rows) 3.8 and 4.7 ms, one 2048 x 2048 (256 tiles) 1.19 and 0.94 ms.  Shorter
 // sides under kPairSide are mostly padding in a 256 x 256 tile.
 template <class Fn>
-yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, Fn fn) {
+yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn fn) {
   auto wide = [](const Item& it) { return std::min(it.rows, it.cols) >= kPairSide; };
   long long tiles = 0;
   for (const Item& it : items)
     if (wide(it)) tiles += (long long)((it.rows + 127) / 128) * ((it.cols + 127) / 128);
   const bool pairs = tiles >= 6LL * ctx->num_sms;
+  // With longer matrices beside them the short ones cost the steps kernel less
+  // than a launch of their own.
+  const bool chip = steps > 0 && std::all_of(items.begin(), items.end(), on_chip);
   auto t = std::make_unique<Table>();
+  t->chip = chip;
   for (int pair = 1; pair >= 0; --pair) {
     t->count = 0;
     t->pair = pair;
@@ -1120,12 +1593,13 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, Fn fn) {
 // One table after the other, in the same workspace.
 yl_status run_items(yl_ctx* ctx, const std::vector<Item>& items, const Update& u,
                     const Schedule& s, char* ws) {
-  return for_tables(ctx, items, [&](Table& t) { return run_table(ctx, t, u, s, ws); });
+  return for_tables(ctx, items, s.steps,
+                    [&](Table& t) { return run_table(ctx, t, u, s, ws); });
 }
-size_t items_bytes(yl_ctx* ctx, const std::vector<Item>& items) {
+size_t items_bytes(yl_ctx* ctx, const std::vector<Item>& items, int steps) {
   size_t most = 0;
-  for_tables(ctx, items, [&](Table& t) {
-    most = std::max(most, place(&t, ctx->num_sms, nullptr));
+  for_tables(ctx, items, steps, [&](Table& t) {
+    if (!t.chip) most = std::max(most, place(&t, ctx->num_sms, nullptr));
     return YL_OK;
   });
   return most;
@@ -1248,7 +1722,7 @@ yl_status newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int s
   u.eps = eps;
   Workspace work;
   char* ws = nullptr;
-  YL_TRY(work.get(ctx, items_bytes(ctx, items), &ws));
+  YL_TRY(work.get(ctx, items_bytes(ctx, items, q.steps), &ws));
   YL_TRY(run_items(ctx, items, u, q, ws));
   return work.done();
 }
@@ -1319,7 +1793,7 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
   ScratchCarver carve;
   const size_t o_norm = carve.take(sizeof(float)), o_parts = carve.take(parts * sizeof(double));
   carve.offset = (carve.offset + 1023) & ~(size_t)1023;
-  const size_t o_items = carve.take(items_bytes(ctx, items));
+  const size_t o_items = carve.take(items_bytes(ctx, items, q.steps));
   Workspace work;
   char* ws = nullptr;
   YL_TRY(work.get(ctx, carve.offset, &ws));
