@@ -14,7 +14,6 @@
 #include <cmath>
 #include <memory>
 #include <new>
-#include <type_traits>
 #include <vector>
 
 #include "yl_internal.h"
@@ -329,10 +328,14 @@ __global__ void __launch_bounds__(256)
 // 2e-6.  So an accumulator takes a few 16-deep products only, the small ones
 // (hi lo, lo hi) of a k-block first, and the sum over the row is in registers with
 // fp32's rounding.  What costs accuracy is a term far above the others, and A and
-// P have theirs on the diagonal: with eight products to an accumulator throughout
-// 256 x 2304 ended 7.3e-6 off, with eight in GRAM and two elsewhere 2.1e-6 (fp32:
-// 2.0e-6).  So it is two in the k-blocks that meet a diagonal tile, eight in the
-// others, whose handover then hides behind the tensor core's work.
+// P have theirs on the diagonal: with two k-blocks to an accumulator throughout
+// 256 x 2304 ended 7.3e-6 off, with two in GRAM and half a k-block elsewhere 2.1e-6
+// (fp32: 2.0e-6).  So it is one k-block where the tile meets the diagonal, two
+// elsewhere, whose handover then hides behind the tensor core's work.
+// Truncation takes off the same share on average, half a step of fp32 (2^-24) for
+// every addition at full size, and scaled_steps puts 2^-23 back in SQUARE and
+// UPDATE: the errors fell by a third to a half (256 x 2304 2.5e-6 to 1.3e-6, 1024 x
+// 1024 9.9e-7 to 7.3e-7, both with half a k-block on the diagonal).
 //
 // Two forms.  A single block works on 128 x 128 tiles: 12 MMAs a k-block, each
 // reading 4 KB of either side, 117 cycles each, bound by shared memory.  A pair
@@ -671,7 +674,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         const Item& im = t->it[q.item];
         const Operand L = operand(im, q.mode, 0, 0), R = operand(im, q.mode, 0, 1);
         const bool same = q.mode != UPDATE && q.i == q.j;
-        int filled = 0;  // products the current accumulator has taken
+        int filled = 0;  // k-blocks the current accumulator has taken
         for (int kb = 0; ok && kb < q.nk; ++kb, ++it) {
           const int s = it % kStages;
           if (!mbar_wait(&full[s], (it / kStages) & 1, lim) ||
@@ -688,43 +691,32 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           const uint32_t lstep = lmn ? 2048 : 32, rstep = rmn ? 2048 : 32;
           const uint32_t llbo = lmn ? kBlkBytes : 16, rlbo = rmn ? kBlkBytes : 16;
           const uint32_t l = smem_u32(smem + s * kStageBytes), r = same ? l : l + 2 * kOpBytes;
-          // `run` products of this k-block into the current accumulator
-          auto multiply = [&](auto run, int h) {
-            constexpr int kRun = decltype(run)::value;
-            const int buf = ci % kAccs;
-            if (filled == 0 && ci >= kAccs && !wait<PAIR>(&acc_empty[buf], (ci / kAccs - 1) & 1, lim)) {
-              report_error(err, YL_DEVERR_TIMEOUT);
-              ok = false;
-              return;
-            }
-            tc_fence_after();
-            const uint32_t dacc = tmem + (uint32_t)(buf * F::kTile);
+          const bool fine = on_diagonal<PAIR>(im, q, kb);
+          const int buf = ci % kAccs;
+          if (filled == 0 && ci >= kAccs && !wait<PAIR>(&acc_empty[buf], (ci / kAccs - 1) & 1, lim)) {
+            report_error(err, YL_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t dacc = tmem + (uint32_t)(buf * F::kTile);
 #pragma unroll
-            for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
-              const uint32_t lp = l + (part == 0 ? kOpBytes : 0);
-              const uint32_t rp = r + (part == 1 ? kOpBytes : 0);
+          for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
+            const uint32_t lp = l + (part == 0 ? kOpBytes : 0);
+            const uint32_t rp = r + (part == 1 ? kOpBytes : 0);
 #pragma unroll
-              for (int e = 0; e < kRun; ++e) {
-                const int kk = h + e;
-                const uint64_t ld = sw128_desc(lp + kk * lstep, llbo, 1024);
-                const uint64_t rd = sw128_desc(rp + kk * rstep, rlbo, 1024);
-                if (PAIR) umma_f16_pair(dacc, ld, rd, idesc, (filled | part | e) != 0);
-                else umma_f16(dacc, ld, rd, idesc, (filled | part | e) != 0);
-              }
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint64_t ld = sw128_desc(lp + kk * lstep, llbo, 1024);
+              const uint64_t rd = sw128_desc(rp + kk * rstep, rlbo, 1024);
+              if (PAIR) umma_f16_pair(dacc, ld, rd, idesc, (filled | part | kk) != 0);
+              else umma_f16(dacc, ld, rd, idesc, (filled | part | kk) != 0);
             }
-            filled += kRun;
-            if (kRun == 2 || filled == 8 || kb + 1 == q.nk || on_diagonal<PAIR>(im, q, kb + 1)) {
-              if (PAIR) umma_commit_pair(&acc_full[buf]);
-              else umma_commit(&acc_full[buf]);
-              filled = 0;
-              ++ci;
-            }
-          };
-          if (on_diagonal<PAIR>(im, q, kb)) {
-            multiply(std::integral_constant<int, 2>(), 0);
-            if (ok) multiply(std::integral_constant<int, 2>(), 2);
-          } else {
-            multiply(std::integral_constant<int, 4>(), 0);
+          }
+          if (++filled == 2 || fine || kb + 1 == q.nk || on_diagonal<PAIR>(im, q, kb + 1)) {
+            if (PAIR) umma_commit_pair(&acc_full[buf]);
+            else umma_commit(&acc_full[buf]);
+            filled = 0;
+            ++ci;
           }
           if (!ok) break;
           if (PAIR) umma_commit_pair(&empty[s]);
@@ -775,15 +767,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       for (int c = 0; c < kCols; ++c) v[c] = 0.f;
       bool ok = true;
       // the accumulators of the ticket, as the MMA thread fills them
-      for (int kb = 0, filled = 0, half = 0; kb < q.nk; ++ci) {
-        if (on_diagonal<PAIR>(im, q, kb)) {
-          half ^= 1;
-          if (!half) ++kb;
-        } else {
-          do filled += 4, ++kb;
-          while (filled < 8 && kb < q.nk && !on_diagonal<PAIR>(im, q, kb));
-          filled = 0;
-        }
+      for (int kb = 0; kb < q.nk; ++ci) {
+        const bool fine = on_diagonal<PAIR>(im, q, kb++);
+        if (!fine && kb < q.nk && !on_diagonal<PAIR>(im, q, kb)) ++kb;
         const int buf = ci % kAccs;
         if (!wait<PAIR>(&acc_full[buf], (ci / kAccs) & 1, lim)) {
           report_error(err, YL_DEVERR_TIMEOUT);
@@ -975,18 +961,16 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 // blocks holds the pairs of X in shared memory, each block its share of the long
 // side, from the first read of the input to the write of the result, and one
 // launch does the norm, all steps and the update.  Per step each block multiplies
-// its share of the Gram sum, the blocks exchange the sums through distributed
-// shared memory (every block adds up a few columns in rank order and hands the
-// finished columns to all), and each forms P for itself and updates its share.
-// 128 x 1152 takes the steps kernel 15 trips through memory and its counters
-// (about 5 us each); here a step is bound by its 84 MMAs of 117 cycles and four
-// cluster barriers.
-constexpr int kChipBlocks = 4;                       // most 64-blocks of a block's share
+// its share of the Gram sum, the blocks exchange the sums by bulk copies between
+// their shared memories (every block adds up a few rows in rank order and hands
+// the finished rows to all), and each forms P for itself and updates its share.
+constexpr int kChipBlocks = 3;                       // most 64-blocks of a block's share
 constexpr int kChipShare = 16;                       // most blocks of a cluster
 constexpr int kChipXPlane = kChipBlocks * 2 * kBlkBytes;
 constexpr int kChipAOff = 2 * kChipXPlane;           // A, then P; before that the Gram sums
 constexpr int kChipAPlane = 4 * kBlkBytes;
-constexpr int kChipBarOff = kChipAOff + 2 * kChipAPlane;
+constexpr int kChipOutOff = kChipAOff + 2 * kChipAPlane;  // what the block sends
+constexpr int kChipBarOff = kChipOutOff + 2 * kChipAPlane;
 constexpr int kChipSmem = kChipBarOff + 512 + 1024;  // barrier and norms, alignment
 constexpr int kChipThreads = 256;
 
@@ -995,11 +979,6 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void st_cluster_v4(uint32_t addr, uint4 v) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y),
-               "r"(v.z), "r"(v.w)
-               : "memory");
 }
 __device__ __forceinline__ void st_cluster_f64(uint32_t addr, double v) {
   asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(addr), "d"(v) : "memory");
@@ -1042,7 +1021,9 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint64_t* done = reinterpret_cast<uint64_t*>(smem + kChipBarOff);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  uint64_t* sums_in = done + 1;   // other blocks' sums of this block's rows
+  uint64_t* rows_in = done + 2;   // finished rows of A
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 3);
   double* norms = reinterpret_cast<double*>(smem + kChipBarOff + 64);  // [kChipShare]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp & 3, wc = warp >> 2;
@@ -1055,6 +1036,8 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   const long long lim = wait_limit(err);
   if (tid == 0) {
     mbar_init(done, 1);
+    mbar_init(sums_in, 1);
+    mbar_init(rows_in, 1);
     fence_barrier_init();
   }
   if (warp == 0) {
@@ -1205,7 +1188,15 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   // accumulators are read again before the next multiply overwrites them
   auto drained = [&]() { tc_fence_before(); };
 
-  const int per = max(1, 8 * mb / share);  // 8-column chunks of A that a block adds up
+  // Waits for copies from other blocks; one that takes too long for the caller's
+  // limit is reported and still waited for, since it writes to this block.
+  auto arrived = [&](uint64_t* bar, uint32_t parity) {
+    if (mbar_wait_cluster(bar, parity, lim)) return;
+    report_error(err, YL_DEVERR_TIMEOUT);
+    mbar_wait_cluster(bar, parity);
+  };
+  const int rows = mb * kBlk / share;  // rows of A that a block adds up
+  uint8_t* outbox = smem + kChipOutOff;
   for (int s = 0; s < steps.n; ++s) {
     // ---- this share of A = X X^T (X^T X)
     const int kks = 4 * mw, gchain = max(1, (kks + 3) / 4);
@@ -1218,75 +1209,109 @@ __global__ void __launch_bounds__(kChipThreads, 1)
     float p[64];
     sum_accumulators(lanes, kks > 0 ? (kks + gchain - 1) / gchain : 0, p);
     drained();
-    if (s > 0) cluster_wait();  // no block needs its P any more
-    else {
+    const int r64 = (wr & 1) * 32 + lane;  // this thread's row inside its block of A
+    const bool in_a = wc < mb && (wr >> 1) < mb;
+    uint8_t* a_row = smem + kChipAOff + (wc * 2 + (wr >> 1)) * kBlkBytes + r64 * 128;
+    if (share == 1) {
+      if (in_a) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c) p[c] *= steps.g2[s];
+#pragma unroll
+        for (int ch = 0; ch < 8; ++ch) {
+          uint4 hi, lo;
+          split8(p + ch * 8, &hi, &lo);
+          uint8_t* at = a_row + ((ch ^ (r64 & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = hi;
+          *reinterpret_cast<uint4*>(at + kChipAPlane) = lo;
+        }
+      }
+    } else {
+      // ---- sums to the blocks that add them up: rows of 64 mb floats, the block of
+      // row r is r / rows; 16-byte pieces rotated by the row against bank conflicts
+      const uint32_t pitch = mb * 256;
+      if (s == 0) cluster_arrive();
+      cluster_wait();  // no block needs its P any more, and all have what this one sent last
+      if (in_a) {
+        const int row = wr * 32 + lane;
+        uint8_t* to = outbox + row * pitch + wc * 256;
+#pragma unroll
+        for (int q = 0; q < 16; ++q)
+          *reinterpret_cast<float4*>(to + (((q + row) & 15) << 4)) =
+              make_float4(p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]);
+      }
+      if (tid == 0) {
+        mbar_arrive_expect_tx(sums_in, (uint32_t)(mb * kBlk) * pitch);
+        mbar_arrive_expect_tx(rows_in, (uint32_t)(2 * mb * mb) * kBlkBytes);
+      }
+      fence_proxy_async_all();
+      __syncthreads();
+      const uint32_t bytes = rows * pitch;  // to and from one block
+      if (tid < share) {
+        bulk_copy_cluster(map_to_rank(as + rank * bytes, tid),
+                          smem_u32(outbox) + tid * bytes, bytes,
+                          map_to_rank(smem_u32(sums_in), tid));
+      }
+      arrived(sums_in, s & 1);
+      // ---- this block's rows, in rank order; a piece is 8 columns of a row
+      uint4 hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int e = tid + i * kChipThreads, r = e / (8 * mb), c8 = e - r * 8 * mb;
+        if (r >= rows) continue;
+        const int row = rank * rows + r;
+        const uint8_t* from = smem + kChipAOff + r * pitch + (c8 >> 3) * 256;
+        const int q = 2 * (c8 & 7);
+        float a[8] = {};
+        for (int k = 0; k < share; ++k, from += bytes) {
+          const float4 x = *reinterpret_cast<const float4*>(from + (((q + row) & 15) << 4));
+          const float4 y = *reinterpret_cast<const float4*>(from + (((q + 1 + row) & 15) << 4));
+          a[0] += x.x, a[1] += x.y, a[2] += x.z, a[3] += x.w;
+          a[4] += y.x, a[5] += y.y, a[6] += y.z, a[7] += y.w;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] *= steps.g2[s];
+        split8(a, &hi[i], &lo[i]);
+      }
+      // ---- finished rows to every block: in both planes and each column block the
+      // rows of a block lie together.  The outbox is free again once every block has
+      // its sums, which the barrier says.
+      fence_proxy_async_all();
       cluster_arrive();
       cluster_wait();
-    }
-    // ---- sums to the blocks that add them up: [rank][chunk][row][8]
-    if (wc < mb) {
+      const uint32_t piece = rows * 128;
 #pragma unroll
-      for (int ch = 0; ch < 8; ++ch) {
-        const int c = wc * 8 + ch, owner = c / per;
-        const uint32_t to = map_to_rank(
-            as + (uint32_t)(((rank * per + (c - owner * per)) * 128 + wr * 32 + lane) * 32), owner);
-        st_cluster_v4(to, *reinterpret_cast<const uint4*>(p + ch * 8));
-        st_cluster_v4(to + 16, *reinterpret_cast<const uint4*>(p + ch * 8 + 4));
+      for (int i = 0; i < 4; ++i) {
+        const int e = tid + i * kChipThreads, r = e / (8 * mb), c8 = e - r * 8 * mb;
+        if (r >= rows) continue;
+        uint8_t* to = outbox + (c8 >> 3) * piece + r * 128 +
+                      (((c8 & 7) ^ ((rank * rows + r) & 7)) << 4);
+        *reinterpret_cast<uint4*>(to) = hi[i];
+        *reinterpret_cast<uint4*>(to + mb * piece) = lo[i];
       }
-    }
-    cluster_arrive();
-    cluster_wait();
-    const int row = tid & 127;
-    const bool adds = row < mb * 64;
-    uint4 hi[8], lo[8];  // this thread's chunks: at most 16 of a single block, two threads a row
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int lc = (tid >> 7) + 2 * i;
-      if (!adds || lc >= per || rank * per + lc >= 8 * mb) continue;
-      float a[8] = {};
-      for (int r = 0; r < share; ++r) {
-        const float4* q =
-            reinterpret_cast<const float4*>(smem + kChipAOff + ((r * per + lc) * 128 + row) * 32);
-        const float4 x = q[0], y = q[1];
-        a[0] += x.x, a[1] += x.y, a[2] += x.z, a[3] += x.w;
-        a[4] += y.x, a[5] += y.y, a[6] += y.z, a[7] += y.w;
+      fence_proxy_async_all();
+      __syncthreads();
+      const int row0a = rank * rows;
+      for (int k = tid; k < share * 2 * mb; k += kChipThreads) {
+        const int dst = k / (2 * mb), pl = (k / mb) & 1, cb = k % mb;
+        const uint32_t at = as + pl * kChipAPlane + (cb * 2 + (row0a >> 6)) * kBlkBytes +
+                            (row0a & 63) * 128;
+        bulk_copy_cluster(map_to_rank(at, dst), smem_u32(outbox) + (pl * mb + cb) * piece, piece,
+                          map_to_rank(smem_u32(rows_in), dst));
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) a[j] *= steps.g2[s];
-      split8(a, &hi[i], &lo[i]);
+      arrived(rows_in, s & 1);
     }
-    cluster_arrive();  // every block has read its sums
-    cluster_wait();
-    // ---- finished columns to every block: A's blocks [column block][row block]
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int lc = (tid >> 7) + 2 * i, c = rank * per + lc;
-      if (!adds || lc >= per || c >= 8 * mb) continue;
-      const uint32_t at = as + (uint32_t)(((c >> 3) * 2 + (row >> 6)) * kBlkBytes + (row & 63) * 128 +
-                                          (((c & 7) ^ (row & 7)) << 4));
-      for (int r = 0; r < share; ++r) {
-        const uint32_t to = map_to_rank(at, r);
-        st_cluster_v4(to, hi[i]);
-        st_cluster_v4(to + kChipAPlane, lo[i]);
-      }
-    }
-    fence_proxy_async_all();
-    cluster_arrive();
-    cluster_wait();
     // ---- P = s0 I + s1 A + s2 A A, over A
-    multiply(4 * mb, 2, idesc_f16(128, mb * 64, 0, 0), kChipAPlane, kChipAPlane,
+    multiply(4 * mb, mb, idesc_f16(128, mb * 64, 0, 0), kChipAPlane, kChipAPlane,
              [&](int kk, uint64_t* l, uint64_t* r) {
                *l = *r = sw128_desc(as + (kk >> 2) * 2 * kBlkBytes + (kk & 3) * 32, 16, 1024);
              });
-    sum_accumulators(lanes, 2 * mb, p);
+    sum_accumulators(lanes, 4, p);
     drained();
-    if (wc < mb && (wr >> 1) < mb) {
-      const int r64 = (wr & 1) * 32 + lane;
-      uint8_t* blk = smem + kChipAOff + (wc * 2 + (wr >> 1)) * kBlkBytes + r64 * 128;
+    if (in_a) {
       const float s0 = steps.s0[s], s1 = steps.s1[s], s2 = steps.s2[s];
 #pragma unroll
       for (int ch = 0; ch < 8; ++ch) {
-        uint8_t* at = blk + ((ch ^ (r64 & 7)) << 4);
+        uint8_t* at = a_row + ((ch ^ (r64 & 7)) << 4);
         const uint4 h4 = *reinterpret_cast<const uint4*>(at);
         const uint4 l4 = *reinterpret_cast<const uint4*>(at + kChipAPlane);
         const __half2* h = reinterpret_cast<const __half2*>(&h4);
@@ -1313,7 +1338,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       const int hb = min(2, mw - 2 * hf);
       const uint32_t idesc =
           tall ? idesc_f16(128, mb * 64, 0, 0) : idesc_f16(128, hb * 64, 0, 1);
-      multiply(4 * mb, 2, idesc, tall ? kChipXPlane : kChipAPlane, tall ? kChipAPlane : kChipXPlane,
+      multiply(4 * mb, mb, idesc, tall ? kChipXPlane : kChipAPlane, tall ? kChipAPlane : kChipXPlane,
                [&](int kk, uint64_t* l, uint64_t* r) {
                  const int sb = kk >> 2, q = kk & 3;
                  const uint64_t pd = sw128_desc(as + sb * 2 * kBlkBytes + q * 32, 16, 1024);
@@ -1325,7 +1350,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
                    *r = sw128_desc(xs + xoff(2 * hf, sb) + q * 2048, 2 * kBlkBytes, 1024);
                  }
                });
-      sum_accumulators(lanes, 2 * mb, p);
+      sum_accumulators(lanes, 4, p);
       drained();
       const int lrow = tall ? 2 * hf + (wr >> 1) : (wr >> 1);  // row and column block of the share
       const int lcol = tall ? wc : 2 * hf + wc;
@@ -1337,7 +1362,6 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       }
       if (!last) {
         if (inside) {
-          const int r64 = (wr & 1) * 32 + lane;
           uint8_t* blk = smem + (tall ? xoff(lrow, lcol) : xoff(lcol, lrow)) + r64 * 128;
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
@@ -1386,9 +1410,10 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       }
     }
     __syncthreads();
-    cluster_arrive();  // this block's P may be overwritten; waited for in the next step
+    // this block's P may be overwritten; waited for in the next step
+    if (share > 1) cluster_arrive();
   }
-  cluster_wait();  // no block leaves while another may still write to it
+  if (share > 1) cluster_wait();  // no block leaves while another may still write to it
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -1463,8 +1488,10 @@ struct Schedule {
   float sa[kMaxSteps], sp[kMaxSteps];
 };
 
-// Coefficients with the scales of the pairs folded in.
+// Coefficients with the scales of the pairs folded in, and in the products that
+// feed back on themselves the mean of what the tensor core's truncation takes off.
 Steps scaled_steps(const Schedule& s) {
+  constexpr float kPutBack = 1.f + 0x1p-23f;
   Steps st;
   st.n = s.steps;
   for (int k = 0; k < s.steps; ++k) {
@@ -1472,8 +1499,8 @@ Steps scaled_steps(const Schedule& s) {
     st.g2[k] = sa / (sx * sx);
     st.s0[k] = s.q[3 * k] * sp;
     st.s1[k] = s.q[3 * k + 1] * sp / sa;
-    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa);
-    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx);
+    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa) * kPutBack;
+    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx) * kPutBack;
   }
   return st;
 }
@@ -1491,7 +1518,10 @@ yl_status run_chip(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s) {
   // as many blocks to a matrix as its long side needs, and more while SMs are idle
   int share = 1;
   while (share * kChipBlocks < longest) share *= 2;
-  while (share < 8 && share < longest && 2 * share * t.count <= ctx->num_sms) share *= 2;
+  // (clusters of 16 find room for only a few of themselves)
+  while (share < longest && 2 * share * t.count <= (share < 8 ? 1.0 : 0.5) * ctx->num_sms &&
+         share < kChipShare)
+    share *= 2;
   YL_CUDA(cudaFuncSetAttribute(ns_chip_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kChipSmem));
   if (share > 8)

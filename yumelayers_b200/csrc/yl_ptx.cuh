@@ -182,13 +182,15 @@ __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t byt
                : "memory");
 }
 
-// Programmatic dependent launch: wait until the preceding kernel of the stream
-// has completed and its writes are visible / let the next one be set up early.
-__device__ __forceinline__ void grid_dep_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-__device__ __forceinline__ void grid_dep_launch() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+// Bulk copy from this CTA's shared memory to one of the cluster (dst and bar are
+// addresses in that CTA, as map_to_rank gives them).
+__device__ __forceinline__ void bulk_copy_cluster(uint32_t dst, uint32_t src, uint32_t bytes,
+                                                  uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "r"(src), "r"(bytes), "r"(bar)
+      : "memory");
 }
 
 // Hint: bring the 128-byte line holding p into L2 (no register result, no fault).
