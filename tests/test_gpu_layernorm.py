@@ -70,7 +70,7 @@ def rows_in(a, pad):
 SHAPES = [(1, 1), (3, 1), (1, 2), (5, 3), (2, 4), (33, 4), (1000, 5), (7, 31), (130, 32), (9, 33),
           (257, 64), (64, 96), (65, 127), (4099, 128), (31, 129), (100, 255), (77, 256), (3, 257),
           (515, 384), (32, 512), (50, 1000), (1, 1021), (20, 1024), (13, 2048), (6, 2049),
-          (5, 4096), (3, 5000), (2, 8192), (4, 8195), (2, 16384), (3, 20000), (1, 70001)]
+          (5, 4096), (3, 5000), (2, 8192), (4, 8195), (300, 13393), (90, 9000), (2, 16383), (2, 16384), (3, 20000), (1, 70001)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)

@@ -76,7 +76,7 @@ SHAPES = [(1, 1), (1, 2), (2, 1), (3, 3), (1, 700), (700, 1), (4, 36), (3, 1152)
           (128, 129), (128, 1152), (1152, 128), (129, 257), (257, 129), (128, 864), (192, 320),
           (256, 1000), (255, 511), (511, 255), (320, 320), (384, 1153), (2, 4096), (128, 2048),
           (2049, 120), (65, 2500), (4096, 128), (4033, 17), (64, 4097), (4200, 100), (128, 192),
-          (257, 64), (70, 513)]
+          (257, 64), (70, 513), (3785, 2), (5, 6000), (6144, 60), (60, 6145), (64, 2000), (1000, 64)]
 
 
 @pytest.mark.parametrize("r,c", SHAPES)

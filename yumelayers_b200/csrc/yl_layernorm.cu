@@ -10,13 +10,12 @@
 // A row is held in registers from its only read to its only write:
 //   up to 1024 columns   a group of 4 to 32 lanes owns a row, several rows in
 //                        flight per group where a row is short;
-//   up to 16384 columns  a block of 256 to 1024 threads owns a row (8192 backward,
-//                        whose five values a column fill the registers there);
+//   up to 16384 columns  a block of 256 to 1024 threads owns a row;
 //   longer               a block walks the row from memory again for each pass.
 // The mean of x - mean, which fp32 leaves not quite zero, is measured with the
 // variance and taken off again, so that rows far from zero keep their accuracy.
-// The column sums of the backward pass stay in the registers of the threads that
-// own the columns; after at most 64 rows they go to a block's partial row, and a
+// The column sums of the backward pass stay with the threads that own the columns
+// (in registers, past 8192 columns in shared memory); after at most 64 rows they go to a block's partial row, and a
 // second kernel adds the partial rows in double in a fixed order.
 #include <algorithm>
 #include <type_traits>
@@ -529,6 +528,78 @@ __global__ void __launch_bounds__(THREADS) ln_bwd_block_kernel(const __grid_cons
   }
 }
 
+// Rows of more columns than the column sums leave registers for: those are in
+// shared memory, each thread's own columns.
+constexpr int kWideThreads = 1024, kWidePer = 16;
+constexpr int kWideBytes = 2 * kWideThreads * kWidePer * (int)sizeof(float);
+
+template <bool VEC>
+__global__ void __launch_bounds__(kWideThreads) ln_bwd_wide_kernel(const __grid_constant__ Bwd p) {
+  using R = Row<kWideThreads, kWidePer, VEC>;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float red[64];
+  const int lane = threadIdx.x;
+  float* sums = reinterpret_cast<float*>(ring) + lane;  // [2][element][thread]
+  constexpr int kBeta = kWidePer * kWideThreads;
+#pragma unroll
+  for (int k = 0; k < kWidePer; ++k) sums[k * kWideThreads] = sums[kBeta + k * kWideThreads] = 0.f;
+  const long long iters = (p.rows + gridDim.x - 1) / gridDim.x;
+  long long part = blockIdx.x;
+  int held = 0;
+  for (long long it = 0; it < iters; ++it) {
+    const long long r = it * gridDim.x + blockIdx.x;
+    if (r < p.rows) {
+      float x[kWidePer], dy[kWidePer], w[kWidePer];
+      R::load(p.x + r * p.ldx, p.cols, lane, x);
+      R::load(p.dy + r * p.lddy, p.cols, lane, dy);
+      float m = p.mean ? __ldg(p.mean + r) : 0.f, rs = p.mean ? __ldg(p.rstd + r) : 0.f, e = 0.f;
+      if (!p.mean)
+        row_stats<Block<kWideThreads>, R, kWidePer>(x, p.cols, lane, p.eps, red, m, e, rs);
+      R::load_or(p.gamma, 1.f, p.cols, lane, w);
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int k = 0; k < kWidePer; ++k) {
+        x[k] = R::col(k, lane) < p.cols ? ((x[k] - m) - e) * rs : 0.f;
+        if (p.sums()) {
+          sums[k * kWideThreads] = fmaf(dy[k], x[k], sums[k * kWideThreads]);
+          sums[kBeta + k * kWideThreads] += dy[k];
+        }
+        dy[k] *= w[k];
+        s1 += dy[k];
+        s2 = fmaf(dy[k], x[k], s2);
+      }
+      if (p.dx) {
+        if (p.addend) R::load(p.addend + r * p.ldadd, p.cols, lane, w);
+        Block<kWideThreads>::sum2(s1, s2, red);
+        const float inv = 1.f / p.cols;
+        s1 *= inv;
+        s2 *= inv;
+#pragma unroll
+        for (int k = 0; k < kWidePer; ++k) {
+          const float v = rs * ((dy[k] - s1) - x[k] * s2);
+          w[k] = p.addend ? w[k] + v : v;
+        }
+        R::store(p.dx + r * p.lddx, p.cols, lane, w);
+      }
+    }
+    ++held;
+    if (p.sums() && (held == kSegRows || it + 1 == iters)) {
+      float *og = p.out_gamma(part), *ob = p.out_beta(part);
+#pragma unroll
+      for (int k = 0; k < kWidePer; ++k) {
+        const int c = R::col(k, lane);
+        if (c < p.cols) {
+          if (og) og[c] = sums[k * kWideThreads];
+          if (ob) ob[c] = sums[kBeta + k * kWideThreads];
+        }
+        sums[k * kWideThreads] = sums[kBeta + k * kWideThreads] = 0.f;
+      }
+      part += gridDim.x;
+      held = 0;
+    }
+  }
+}
+
 // Column sums of the partial rows, 32 columns by 32 shares of the rows a block;
 // blockIdx.y 0: dgamma, 1: dbeta.
 __global__ void __launch_bounds__(1024)
@@ -688,6 +759,7 @@ auto bwd_aligned(int cols, F f) {
   if (cols <= 2048) return bwd_ring<256, 256, 8, 2, 3>(f);
   if (cols <= 4096) return bwd_ring<512, 512, 8, 2, 2>(f);
   if (cols <= 8192) return bwd_ring<1024, 1024, 8, 2, 1>(f);
+  if (cols <= 16384) return f(ln_bwd_wide_kernel<true>, kWideThreads, 1, 1, kWideBytes);
   return f(ln_bwd_long_kernel, kLong, 1, 1, 0);
 }
 template <class F>
@@ -702,6 +774,7 @@ auto bwd_plain(int cols, F f) {
   if (cols <= 2048) return f(ln_bwd_block_kernel<256, 8, false>, 256, 1, 1, 0);
   if (cols <= 4096) return f(ln_bwd_block_kernel<512, 8, false>, 512, 1, 1, 0);
   if (cols <= 8192) return f(ln_bwd_block_kernel<1024, 8, false>, 1024, 1, 1, 0);
+  if (cols <= 16384) return f(ln_bwd_wide_kernel<false>, kWideThreads, 1, 1, kWideBytes);
   return f(ln_bwd_long_kernel, kLong, 1, 1, 0);
 }
 
@@ -795,14 +868,14 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
   auto launch = [&](auto kernel, int threads, int rows_a_block, int unr, int smem) -> yl_status {
     long long blocks = (rows + rows_a_block - 1) / rows_a_block;
     // a few turns of one block are quicker than a second kernel for the sums
-    if (blocks <= kAloneTurns && cols <= 8192) blocks = 1;
+    if (blocks <= kAloneTurns && cols <= 16384) blocks = 1;
     YL_TRY(resident(ctx, kernel, threads, smem, &blocks));
     Workspace work;
     // rows a thread adds up per turn, turns per partial row, partial rows of a block
     const long long turns = (rows + blocks * rows_a_block - 1) / (blocks * rows_a_block);
     const long long per_part = kSegRows / unr;
     const long long parts = blocks * ((turns + per_part - 1) / per_part);
-    if (parts == 1 && cols <= 8192) {
+    if (parts == 1 && cols <= 16384) {
       p.dgamma = dgamma;
       p.dbeta = dbeta;
     } else if (dgamma || dbeta) {

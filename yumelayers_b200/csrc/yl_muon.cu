@@ -964,9 +964,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 // its share of the Gram sum, the blocks exchange the sums by bulk copies between
 // their shared memories (every block adds up a few rows in rank order and hands
 // the finished rows to all), and each forms P for itself and updates its share.
-constexpr int kChipBlocks = 3;                       // most 64-blocks of a block's share
+constexpr int kChipBlocks = 6;                       // most 64 x 64 blocks of a block's share
 constexpr int kChipShare = 16;                       // most blocks of a cluster
-constexpr int kChipXPlane = kChipBlocks * 2 * kBlkBytes;
+constexpr int kChipXPlane = kChipBlocks * kBlkBytes;
 constexpr int kChipAOff = 2 * kChipXPlane;           // A, then P; before that the Gram sums
 constexpr int kChipAPlane = 4 * kBlkBytes;
 constexpr int kChipOutOff = kChipAOff + 2 * kChipAPlane;  // what the block sends
@@ -1047,7 +1047,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
 
   // ---- the input: momentum step, norm, pairs.  A unit is 8 columns of a row;
   // a thread keeps all of its units in registers between the two.
-  constexpr int kUnits = kChipBlocks * 2 * 64 * 8 / kChipThreads;
+  constexpr int kUnits = kChipBlocks * 64 * 8 / kChipThreads;
   float v[kUnits][8];
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   // blocks of the share, in rows and in columns
@@ -1126,10 +1126,13 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   for (int r = 0; r < share; ++r) total += norms[r];
   const float inv = (float)(1.0 / (sqrt(total) + (double)u.eps));
 
-  // Block (long, short) of the share: a wide X keeps its two row blocks together
-  // (128 rows of a K-major operand), a tall one its row blocks.
+  // Block (long, short) of the share: a wide X keeps its row blocks together (the
+  // 128 rows of a K-major operand), a tall one its row blocks along the long side.
+  // (Operands of 128 rows run into other blocks where there are fewer rows: what
+  // comes of those stays in rows that nothing reads.)
+  const int lmax = kChipBlocks / mb;
   auto xoff = [&](int lb, int sb) {
-    return (uint32_t)((tall ? sb * kChipBlocks + lb : lb * 2 + sb) * kBlkBytes);
+    return (uint32_t)((tall ? sb * lmax + lb : lb * mb + sb) * kBlkBytes);
   };
 #pragma unroll
   for (int e = 0; e < kUnits; ++e) {
@@ -1204,7 +1207,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       multiply(kks, gchain, idesc_f16(128, mb * 64, tall, tall), kChipXPlane, kChipXPlane,
                [&](int kk, uint64_t* l, uint64_t* r) {
                  const uint32_t at = xs + xoff(kk >> 2, 0) + (kk & 3) * (tall ? 2048 : 32);
-                 *l = *r = sw128_desc(at, tall ? kChipBlocks * kBlkBytes : 16, 1024);
+                 *l = *r = sw128_desc(at, tall ? lmax * kBlkBytes : 16, 1024);
                });
     float p[64];
     sum_accumulators(lanes, kks > 0 ? (kks + gchain - 1) / gchain : 0, p);
@@ -1347,7 +1350,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
                    *r = pd;
                  } else {
                    *l = pd;
-                   *r = sw128_desc(xs + xoff(2 * hf, sb) + q * 2048, 2 * kBlkBytes, 1024);
+                   *r = sw128_desc(xs + xoff(2 * hf, sb) + q * 2048, mb * kBlkBytes, 1024);
                  }
                });
       sum_accumulators(lanes, 4, p);
@@ -1377,8 +1380,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       // the result, 32 rows x 32 columns at a time through this half's own blocks
       if (inside) {
         float* st = reinterpret_cast<float*>(
-            smem + (tall ? (wc * kChipBlocks + 2 * hf) * kBlkBytes + wr * 4096
-                         : hf * 4 * kBlkBytes + warp * 4096));
+            smem + (tall ? xoff(2 * hf, wc) + wr * 4096 : xoff(2 * hf + wc, 0) + wr * 4096));
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           __syncwarp();
@@ -1507,17 +1509,20 @@ Steps scaled_steps(const Schedule& s) {
 
 // Whether a matrix can stay on the chip.
 bool on_chip(const Item& it) {
-  return std::min(it.rows, it.cols) <= 2 * kBlk &&
-         std::max(it.rows, it.cols) <= kChipShare * kChipBlocks * kBlk;
+  const int m = std::min(it.rows, it.cols), n = std::max(it.rows, it.cols);
+  const int mb = (m + kBlk - 1) / kBlk, nb = (n + kBlk - 1) / kBlk;
+  return mb <= 2 && nb <= kChipShare * (kChipBlocks / mb);
 }
 
 yl_status run_chip(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s) {
   place(&t, ctx->num_sms, nullptr);  // sizes only: nothing of these is in the workspace
-  int longest = 0;
-  for (int k = 0; k < t.count; ++k) longest = std::max({longest, t.it[k].rb, t.it[k].cb});
   // as many blocks to a matrix as its long side needs, and more while SMs are idle
-  int share = 1;
-  while (share * kChipBlocks < longest) share *= 2;
+  int longest = 0, share = 1;
+  for (int k = 0; k < t.count; ++k) {
+    const int nb = std::max(t.it[k].rb, t.it[k].cb);
+    longest = std::max(longest, nb);
+    while (share * (kChipBlocks / t.it[k].mb) < nb) share *= 2;
+  }
   // (clusters of 16 find room for only a few of themselves)
   while (share < longest && 2 * share * t.count <= (share < 8 ? 1.0 : 0.5) * ctx->num_sms &&
          share < kChipShare)
