@@ -562,11 +562,13 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     if (lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      int next = rank == 0 ? atomicAdd(t->ctrl, 1) : 0;
       for (uint32_t k = 0; ok; ++k) {
         const int slot = k % kRing;
-        int n = next;
+        int n;
         if (rank == 0) {
+          // taken no earlier than its loads could start: a ticket held back here is
+          // one that an idle block would have begun
+          n = atomicAdd(t->ctrl, 1);
           if (k >= kRing && !wait<PAIR>(&tempty[slot], (k / kRing - 1) & 1, lim)) {
             report_error(err, YL_DEVERR_TIMEOUT);
             break;
@@ -577,7 +579,6 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             st_cluster_s32(map_to_rank(smem_u32(&ring[slot]), 1), n);
             mbar_arrive_cluster(map_to_rank(smem_u32(&tfull[slot]), 1));
           }
-          if (n < total) next = atomicAdd(t->ctrl, 1);  // on its way while this tile loads
         } else {
           if (!wait<PAIR>(&tfull[slot], (k / kRing) & 1, lim)) {
             report_error(err, YL_DEVERR_TIMEOUT);
@@ -1573,8 +1574,12 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0]);
   YL_TRY(check_launch("ns_split_kernel"));
   const Steps st = scaled_steps(s);
-  const int widest = std::max(t.tiles[GRAM][t.count], t.tiles[UPDATE][t.count]);
-  const int workers = std::min(widest, ctx->num_sms / ctas);
+  // More blocks than a phase has tickets: they hold tickets of the phases to come,
+  // so that no block is handed two of one phase (512 x 128 and 512 x 512 in 22
+  // blocks, the most tickets of a phase: 291 us).
+  long long tickets = 0;
+  for (int m = 0; m < 3; ++m) tickets += (long long)s.steps * t.tiles[m][t.count];
+  const int workers = (int)std::min<long long>(tickets, ctx->num_sms / ctas);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(workers * ctas);
   cfg.blockDim = dim3(kProductThreads);
