@@ -763,6 +763,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       if (n >= total) break;
       const Ticket q = ticket_of<PAIR>(t, start, count, n);
       const Item& im = t->it[q.item];
+      if (u.muon && q.mode == UPDATE && q.step + 1 == steps.n) {
+        // the parameter's rows towards L2 while the products run: a row of this
+        // warp's columns per lane
+        const long long r = (long long)(F::kSide * q.i + 2 * rank) * kBlk + wr * 32 + lane;
+        const int c0 = (F::kSide * q.j) * kBlk + wc * kCols, c1 = min(c0 + kCols, im.cols);
+        if (r < im.rows)
+          for (int c = c0; c < c1; c += 32) prefetch_l2(im.dst + r * im.ldd + c);
+      }
       float v[kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) v[c] = 0.f;
