@@ -337,8 +337,10 @@ __global__ void __launch_bounds__(256)
 // UPDATE: the errors fell by a third to a half (256 x 2304 2.5e-6 to 1.3e-6, 1024 x
 // 1024 9.9e-7 to 7.3e-7, both with half a k-block on the diagonal).
 //
-// Two forms.  A single block works on 128 x 128 tiles: 12 MMAs a k-block, each
-// reading 4 KB of either side, 117 cycles each, bound by shared memory.  A pair
+// Two forms.  A single block works on 128 x 128 tiles; its MMAs are bound by their
+// reads of shared memory (12 of 128 x 128 a k-block, 8 KB each, take 117 cycles
+// each, not 64), so the left hi plane meets both right planes in one of 256 columns
+// (12 KB).  A pair
 // of blocks (PAIR: a cluster of two, cta_group::2) works on 256 x 256 tiles, each
 // block with half of the rows of both sides: the same 8 KB of reads for four
 // times the products, 128 cycles per block, bound by the tensor cores.
@@ -362,7 +364,8 @@ struct Form {
   static constexpr int kCtas = PAIR ? 2 : 1;
   static constexpr int kTile = 128 * kCtas;            // rows and columns of a tile
   static constexpr int kSide = 2 * kCtas;              // blocks along it
-  static constexpr int kAccs = kTmemCols / kTile;      // accumulators in TMEM
+  static constexpr int kAccCols = 256;                 // one accumulator in TMEM
+  static constexpr int kAccs = kTmemCols / kAccCols;
   static constexpr int kCols = kTile / 2;              // columns of one epilogue warp
 };
 
@@ -700,18 +703,30 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             break;
           }
           tc_fence_after();
-          const uint32_t dacc = tmem + (uint32_t)(buf * F::kTile);
+          const uint32_t dacc = tmem + (uint32_t)(buf * F::kAccCols);
+          if constexpr (PAIR) {
 #pragma unroll
-          for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
-            const uint32_t lp = l + (part == 0 ? kOpBytes : 0);
-            const uint32_t rp = r + (part == 1 ? kOpBytes : 0);
+            for (int part = 0; part < 3; ++part) {  // lo hi, hi lo, hi hi
+              const uint32_t lp = l + (part == 0 ? kOpBytes : 0);
+              const uint32_t rp = r + (part == 1 ? kOpBytes : 0);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) {
-              const uint64_t ld = sw128_desc(lp + kk * lstep, llbo, 1024);
-              const uint64_t rd = sw128_desc(rp + kk * rstep, rlbo, 1024);
-              if (PAIR) umma_f16_pair(dacc, ld, rd, idesc, (filled | part | kk) != 0);
-              else umma_f16(dacc, ld, rd, idesc, (filled | part | kk) != 0);
+              for (int kk = 0; kk < 4; ++kk)
+                umma_f16_pair(dacc, sw128_desc(lp + kk * lstep, llbo, 1024),
+                              sw128_desc(rp + kk * rstep, rlbo, 1024), idesc,
+                              (filled | part | kk) != 0);
             }
+          } else {
+            // both planes of the right side lie one behind the other: hi (hi | lo) is
+            // one product of 256 columns, lo hi goes to the second half of them
+            const uint32_t wide = idesc_f16(128, 256, lmn, rmn);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16(dacc, sw128_desc(l + kk * lstep, llbo, 1024),
+                       sw128_desc(r + kk * rstep, rlbo, 1024), wide, (filled | kk) != 0);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16(dacc + 128, sw128_desc(l + kOpBytes + kk * lstep, llbo, 1024),
+                       sw128_desc(r + kk * rstep, rlbo, 1024), idesc, 1);
           }
           if (++filled == 2 || fine || kb + 1 == q.nk || on_diagonal<PAIR>(im, q, kb + 1)) {
             if (PAIR) umma_commit_pair(&acc_full[buf]);
@@ -787,16 +802,20 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         tc_fence_after();
         const uint32_t at =
-            tmem + ((uint32_t)(wr * 32) << 16) + (uint32_t)(buf * F::kTile + wc * kCols);
-        // 16 columns at a time: the next read runs while this one is added
+            tmem + ((uint32_t)(wr * 32) << 16) + (uint32_t)(buf * F::kAccCols + wc * kCols);
+        // 16 columns at a time (without PAIR those of hi hi, then those of the small
+        // terms): the next read runs while this one is added
+        constexpr int kReads = 128 / 16;
+        auto col = [](int p) { return PAIR ? p * 16 : (p >> 2) * 128 + (p & 3) * 16; };
         uint32_t acc[2][16];
         tmem_ld_32x32b_x16(at, acc[0]);
 #pragma unroll
-        for (int p = 0; p < kCols / 16; ++p) {
+        for (int p = 0; p < kReads; ++p) {
           tmem_ld_wait();
-          if (p + 1 < kCols / 16) tmem_ld_32x32b_x16(at + (p + 1) * 16, acc[(p + 1) & 1]);
+          if (p + 1 < kReads) tmem_ld_32x32b_x16(at + col(p + 1), acc[(p + 1) & 1]);
 #pragma unroll
-          for (int c = 0; c < 16; ++c) v[p * 16 + c] += __uint_as_float(acc[p & 1][c]);
+          for (int c = 0; c < 16; ++c)
+            v[(PAIR ? p : p & 3) * 16 + c] += __uint_as_float(acc[p & 1][c]);
         }
         tc_fence_before();
         __syncwarp();
