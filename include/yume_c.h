@@ -306,7 +306,8 @@ yl_status yl_adam_multi(yl_ctx* ctx, const yl_adam_tensor* table, int count, flo
  * mean_out / rstd_out (rows, optional) receive the statistics for the backward
  * call.  y may be x itself (same stride); any other overlap is YL_ERR_INVALID.
  * A row with a NaN or an infinity becomes NaN; other rows do not see it.
- * Columns past cols in a padded row are neither read nor written. */
+ * Columns past cols in a padded row are neither read nor written.  cols goes to
+ * 2^29. */
 yl_status yl_layernorm_fwd(yl_ctx* ctx, const float* x, long long ldx, long long rows, int cols,
                            float eps, const float* gamma, const float* beta, float* y,
                            long long ldy, float* mean_out, float* rstd_out);

@@ -287,6 +287,24 @@ def test_offsets_past_32_bits(h):
     del buf, view
 
 
+def test_very_long_rows(h):
+    """3 million columns, 3000 of them to a thread: the row's sums are in double."""
+    rows, cols = 2, 3_000_001
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, cols, generator=gen, device="cuda") + 5.0
+    dy = torch.randn(rows, cols, generator=gen, device="cuda")
+    y, dx, dg, db = (torch.empty_like(x), torch.empty_like(x), torch.empty(cols, device="cuda"),
+                     torch.empty(cols, device="cuda"))
+    call("yl_layernorm_fwd", h, p(x), cols, rows, cols, 1e-5, None, None, p(y), cols, None, None)
+    call("yl_layernorm_bwd", h, p(x), cols, p(dy), cols, rows, cols, 1e-5, None, None, None, None, 0,
+         p(dx), cols, p(dg), p(db))
+    xn, dn = x.cpu().numpy(), dy.cpu().numpy()
+    yr, _, _ = fwd64(xn, 1.0, 0.0, 1e-5)
+    dxr, dgr, dbr = bwd64(xn, dn, 1.0, 1e-5)
+    assert rel(y.cpu(), yr) < TOL_Y and rel(dx.cpu(), dxr) < TOL_DX
+    assert rel(dg.cpu(), dgr) < TOL_SUM and rel(db.cpu(), dbr) < TOL_SUM
+
+
 def test_numpy_and_session_wrappers(ctx):
     from yumelayers_b200 import ops
     from yumelayers_b200.session import GPUTensor, GpuSession

@@ -263,7 +263,8 @@ def test_same_bits_capture_and_two_graphs(h, ctx):
             NsMatrix(x.data_ptr(), y.data_ptr(), *x.shape, x.shape[1], x.shape[1]) for x, y in s])
         call("yl_newton_schulz", h, table, len(s), 5, None, 1e-7)
 
-    sets = [make(1, (128, 700), (300, 130)), make(50, (256, 256), (90, 33))]
+    sets = [make(1, (128, 700), (300, 130)), make(50, (256, 256), (90, 33)),
+            make(80, (128, 1152), (1000, 40))]
     want = []
     for s in sets:
         step(s)
@@ -308,6 +309,84 @@ def test_two_streams_in_turn(ctx):
     ctx.set_stream(None)
     assert all(torch.equal(y, outs[0]) for y in outs)
     assert rel(outs[0].cpu(), ns64(x.cpu().numpy())) < TOL_SPREAD
+
+
+def test_zero_and_tiny_matrices_without_eps(h):
+    zero, tiny = np.zeros((30, 50), np.float32), normal(3, 40, 60) * np.float32(1e-38)
+    tiny[0, :5] = 0.0
+    for more in ([], [normal(4, 140, 150)]):
+        got = run_ns(h, [zero, tiny] + more, eps=0.0)
+        assert not got[0].any()
+        assert rel(got[1], ns64(tiny, eps=0.0)) < TOL_SPREAD
+    assert not run_ns(h, [zero], steps=0, eps=0.0)[0].any()
+    inf = normal(5, 20, 30)
+    inf[3, 3] = np.inf
+    assert np.isnan(run_ns(h, [inf], steps=0)[0]).all()
+
+
+def test_two_contexts_at_once():
+    """Two contexts on two streams, each with more blocks than fit beside the other's."""
+    from yumelayers_b200.session import Context
+    a, b = Context(0), Context(0)
+    sets = []
+    for seed, shapes in ((1, [(700, 900), (128, 300)]), (20, [(128, 1152)] * 6)):
+        xs = [torch.from_numpy(normal(seed + i, *s)).cuda() for i, s in enumerate(shapes)]
+        sets.append((xs, [torch.empty_like(x) for x in xs]))
+    tables = [(NsMatrix * len(xs))(*[
+        NsMatrix(x.data_ptr(), y.data_ptr(), *x.shape, x.shape[1], x.shape[1])
+        for x, y in zip(xs, ys)]) for xs, ys in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, t in ((a, tables[0]), (b, tables[1]), (b, tables[1])):
+            call("yl_newton_schulz", c.handle, t, len(t), 5, None, 1e-7)
+    torch.cuda.synchronize()
+    for c in (a, b):
+        c.check_device_errors()
+        call("yl_ctx_destroy", c.handle)
+    for xs, ys in sets:
+        for x, y in zip(xs, ys):
+            assert rel(y.cpu(), ns64(x.cpu().numpy())) < TOL_SPREAD
+
+
+@pytest.mark.parametrize("shapes", [[(128, 1152)], [(300, 500), (64, 64)], [(1500, 1400)] * 8],
+                         ids=["on chip", "single blocks", "pairs"])
+def test_waits_that_run_out_return_a_status(ctx, shapes):
+    """With a limit of 200 cycles the kernels' waits give up, every warp leaves, and the
+    host reads a timeout; with the default again the same call is right."""
+    xs = [torch.from_numpy(normal(7 + i, *s)).cuda() for i, s in enumerate(shapes)]
+    ys = [torch.empty_like(x) for x in xs]
+    table = (NsMatrix * len(xs))(*[
+        NsMatrix(x.data_ptr(), y.data_ptr(), *x.shape, x.shape[1], x.shape[1])
+        for x, y in zip(xs, ys)])
+    torch.cuda.synchronize()
+    ctx.set_wait_limit(200)
+    try:
+        call("yl_newton_schulz", ctx.handle, table, len(xs), 5, None, 1e-7)
+        with pytest.raises(YumeError) as e:
+            ctx.check_device_errors()
+        assert e.value.status == 3  # YL_ERR_TIMEOUT
+    finally:
+        ctx.set_wait_limit(0)
+    call("yl_newton_schulz", ctx.handle, table, len(xs), 5, None, 1e-7)
+    ctx.check_device_errors()
+    assert rel(ys[0].cpu(), ns64(xs[0].cpu().numpy())) < TOL_SPREAD
+
+
+def test_many_small_weights_with_a_clip(h):
+    """150 matrices: three tables, one norm over all of them."""
+    from yumelayers_b200 import ops
+    rng = np.random.default_rng(9)
+    shapes = [(int(rng.integers(1, 60)), int(rng.integers(1, 90))) for _ in range(150)]
+    ps, gs, ms = ([normal(1000 * k + i, *s) for i, s in enumerate(shapes)] for k in range(3))
+    p2, m2, norm = ops.muon_multi(ps, gs, ms, lr=0.01, clip_max_norm=10.0)
+    want = np.sqrt(sum((g.astype(np.float64) ** 2).sum() for g in gs))
+    assert abs(norm - want) < 1e-6 * want
+    for i in range(0, 150, 7):
+        pr, mr = muon64(ps[i], gs[i] * (10.0 / want), ms[i], 0.01, 0.95, True, 0.0,
+                        ops.muon_scale(*shapes[i]))
+        assert rel(m2[i], mr) < 5e-7
+        assert np.linalg.norm(p2[i] - pr) < TOL_SPREAD * np.linalg.norm(
+            pr - ps[i]) + 1.5e-7 * np.linalg.norm(ps[i])
 
 
 def test_refused_calls_leave_the_outputs_alone(h):

@@ -34,7 +34,7 @@ def bwd(ctx, x=BASE, ldx=64, dy=BASE + (1 << 20), lddy=64, rows=8, cols=64, eps=
 
 @pytest.mark.parametrize("bad,status", [
     (dict(x=None), INVALID), (dict(y=None), INVALID), (dict(rows=-1), SHAPE), (dict(cols=0), SHAPE),
-    (dict(ldx=63), SHAPE), (dict(ldy=63), SHAPE), (dict(eps=-1e-5), INVALID),
+    (dict(cols=(1 << 29) + 1, ldx=1 << 30, ldy=1 << 30), SHAPE), (dict(ldx=63), SHAPE), (dict(ldy=63), SHAPE), (dict(eps=-1e-5), INVALID),
     (dict(eps=float("nan")), INVALID), (dict(y=BASE + 4), INVALID),
     (dict(y=BASE, ldy=65), INVALID), (dict(y=BASE + 8 * 64 * 4 - 4), INVALID),
     (dict(ldx=100, ldy=100, y=BASE + 63 * 4), INVALID), (dict(x=BASE + 2), INVALID),
@@ -52,6 +52,17 @@ def test_layernorm_fwd_refuses(ctx, bad, status):
 ])
 def test_layernorm_bwd_refuses(ctx, bad, status):
     refused(status, *bwd(ctx, **bad))
+
+
+def test_layernorm_bwd_refuses_overlapping_results(ctx):
+    g = BASE + (4 << 20)
+    for dg, db in ((g, g), (g, g + 4 * 63), (BASE + (2 << 20), None), (None, BASE + (2 << 20) + 400)):
+        refused(INVALID, *bwd(ctx)[:-2], dg, db)
+
+
+def test_long_tables_are_checked_quickly(ctx):
+    mats = [(X + i * 4096, Y + i * 4096, 16, 64, 64, 64) for i in range(3000)]
+    refused(INVALID, *ns(ctx, *mats, (X, Y + 2999 * 4096 + 64, 4, 4, 4, 4)))
 
 
 def test_layernorm_without_rows_needs_no_data(ctx):

@@ -15,8 +15,9 @@
 // The mean of x - mean, which fp32 leaves not quite zero, is measured with the
 // variance and taken off again, so that rows far from zero keep their accuracy.
 // The column sums of the backward pass stay with the threads that own the columns
-// (in registers, past 8192 columns in shared memory); after at most 64 rows they go to a block's partial row, and a
-// second kernel adds the partial rows in double in a fixed order.
+// (in registers, past 8192 columns in shared memory); after at most 64 rows they go
+// to a block's partial row, and a second kernel adds the partial rows in double in a
+// fixed order.
 #include <algorithm>
 #include <type_traits>
 
@@ -167,9 +168,9 @@ struct Fwd {
 };
 
 // UNR rows of a group are read before the first is worked on.
-template <int LANES, int PER, bool VEC, int UNR>
+template <int LANES, int PER, int UNR>
 __global__ void __launch_bounds__(256) ln_fwd_group_kernel(const __grid_constant__ Fwd p) {
-  using R = Row<LANES, PER, VEC>;
+  using R = Row<LANES, PER, false>;
   const int lane = threadIdx.x % LANES;
   float ga[PER], be[PER];
   R::load_or(p.gamma, 1.f, p.cols, lane, ga);
@@ -201,9 +202,9 @@ __global__ void __launch_bounds__(256) ln_fwd_group_kernel(const __grid_constant
   }
 }
 
-template <int THREADS, int PER, bool VEC>
+template <int THREADS, int PER>
 __global__ void __launch_bounds__(THREADS) ln_fwd_block_kernel(const __grid_constant__ Fwd p) {
-  using R = Row<THREADS, PER, VEC>;
+  using R = Row<THREADS, PER, false>;
   __shared__ float red[64];
   const int lane = threadIdx.x;
   for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
@@ -453,9 +454,9 @@ __global__ void __launch_bounds__(THREADS, MIN_BLOCKS) ln_bwd_ring_kernel(const 
 
 // Groups take rows in turns; every kSegRows rows of a group the block adds its
 // groups' sums in order and writes a partial row.
-template <int LANES, int PER, bool VEC, int UNR>
+template <int LANES, int PER, int UNR>
 __global__ void __launch_bounds__(256) ln_bwd_group_kernel(const __grid_constant__ Bwd p) {
-  using R = Row<LANES, PER, VEC>;
+  using R = Row<LANES, PER, false>;
   constexpr int G = 256 / LANES;
   __shared__ float sums[2 * LANES * PER];
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
@@ -493,9 +494,9 @@ __global__ void __launch_bounds__(256) ln_bwd_group_kernel(const __grid_constant
   }
 }
 
-template <int THREADS, int PER, bool VEC>
+template <int THREADS, int PER>
 __global__ void __launch_bounds__(THREADS) ln_bwd_block_kernel(const __grid_constant__ Bwd p) {
-  using R = Row<THREADS, PER, VEC>;
+  using R = Row<THREADS, PER, false>;
   __shared__ float red[64];
   const int lane = threadIdx.x;
   float ga[PER], dg[PER], db[PER];
@@ -626,28 +627,49 @@ __global__ void __launch_bounds__(1024)
 }
 
 // ---------------------------------------------------------------- longer rows
+// A thread adds up any number of elements here, so the row's sums are in double.
 constexpr int kLong = 1024;
 
-__device__ __forceinline__ void long_stats(const float* x, int cols, float eps, float* red,
+__device__ __forceinline__ void long_sum2(double& a, double& b, double* red) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) {
+    red[threadIdx.x >> 5] = a;
+    red[32 + (threadIdx.x >> 5)] = b;
+  }
+  __syncthreads();
+  a = b = 0.0;
+  for (int w = 0; w < kLong / 32; ++w) {
+    a += red[w];
+    b += red[32 + w];
+  }
+}
+
+__device__ __forceinline__ void long_stats(const float* x, int cols, float eps, double* red,
                                            float& m, float& e, float& rs) {
-  float s = 0.f, s2 = 0.f;
-  for (int c = threadIdx.x; c < cols; c += kLong) s += x[c];
-  Block<kLong>::sum(s, red);
-  m = s / cols;
-  s = 0.f;
+  double s = 0.0, s2 = 0.0;
+  for (int c = threadIdx.x; c < cols; c += kLong) s += (double)x[c];
+  long_sum2(s, s2, red);
+  m = (float)(s / cols);
+  s = s2 = 0.0;
   for (int c = threadIdx.x; c < cols; c += kLong) {
     const float d = x[c] - m;
-    s += d;
-    s2 = fmaf(d, d, s2);
+    s += (double)d;
+    s2 += (double)d * d;
   }
-  Block<kLong>::sum2(s, s2, red);
-  e = s / cols;
-  rs = 1.f / sqrtf(fmaxf(s2 / cols - e * e, 0.f) + eps);
-  if (isnan(s2)) rs = s2;
+  long_sum2(s, s2, red);
+  s /= cols;
+  s2 = s2 / cols - s * s;
+  e = (float)s;
+  rs = (float)(1.0 / sqrt((s2 < 0.0 ? 0.0 : s2) + (double)eps));  // a NaN stays one
 }
 
 __global__ void __launch_bounds__(kLong) ln_fwd_long_kernel(const __grid_constant__ Fwd p) {
-  __shared__ float red[64];
+  __shared__ double red[64];
   for (long long r = blockIdx.x; r < p.rows; r += gridDim.x) {
     const float* x = p.x + r * p.ldx;
     float m, e, rs;
@@ -665,7 +687,7 @@ __global__ void __launch_bounds__(kLong) ln_fwd_long_kernel(const __grid_constan
 // A block adds each of its rows into its own partial row in memory; kSegRows
 // rows at most, as in registers.
 __global__ void __launch_bounds__(kLong) ln_bwd_long_kernel(const __grid_constant__ Bwd p) {
-  __shared__ float red[64];
+  __shared__ double red[64];
   const long long per = (p.rows + gridDim.x - 1) / gridDim.x;
   for (long long it = 0; it < per; ++it) {
     const long long r = it * gridDim.x + blockIdx.x;
@@ -674,30 +696,29 @@ __global__ void __launch_bounds__(kLong) ln_bwd_long_kernel(const __grid_constan
     const bool first = it % kSegRows == 0;
     if (r >= p.rows) {
       if (pg && first)  // a partial row without rows
-        for (int c = threadIdx.x; c < 2 * p.cols; c += kLong) pg[c] = 0.f;
+        for (long long c = threadIdx.x; c < 2LL * p.cols; c += kLong) pg[c] = 0.f;
       continue;
     }
     const float *x = p.x + r * p.ldx, *dy = p.dy + r * p.lddy;
     float m, e = 0.f, rs;
     if (p.mean) m = p.mean[r], rs = p.rstd[r];
     else long_stats(x, p.cols, p.eps, red, m, e, rs);
-    float s1 = 0.f, s2 = 0.f;
+    double s1 = 0.0, s2 = 0.0;
     for (int c = threadIdx.x; c < p.cols; c += kLong) {
       const float d = dy[c], h = ((x[c] - m) - e) * rs, t = d * (p.gamma ? p.gamma[c] : 1.f);
-      s1 += t;
-      s2 = fmaf(t, h, s2);
+      s1 += (double)t;
+      s2 += (double)t * h;
       if (pg) {
         pg[c] = first ? d * h : fmaf(d, h, pg[c]);
         pg[p.cols + c] = first ? d : pg[p.cols + c] + d;
       }
     }
     if (!p.dx) continue;
-    Block<kLong>::sum2(s1, s2, red);
-    s1 /= p.cols;
-    s2 /= p.cols;
+    long_sum2(s1, s2, red);
+    const float c1 = (float)(s1 / p.cols), c2 = (float)(s2 / p.cols);
     for (int c = threadIdx.x; c < p.cols; c += kLong) {
       const float h = ((x[c] - m) - e) * rs;
-      float v = rs * (fmaf(dy[c], p.gamma ? p.gamma[c] : 1.f, -s1) - h * s2);
+      float v = rs * (fmaf(dy[c], p.gamma ? p.gamma[c] : 1.f, -c1) - h * c2);
       if (p.addend) v += p.addend[r * p.ldadd + c];
       p.dx[r * p.lddx + c] = v;
     }
@@ -729,17 +750,17 @@ auto fwd_aligned(int cols, F f) {
 }
 template <class F>
 auto fwd_plain(int cols, F f) {
-  if (cols <= 16) return f(ln_fwd_group_kernel<4, 4, false, 2>, 256, 128, 2, 0);
-  if (cols <= 32) return f(ln_fwd_group_kernel<8, 4, false, 4>, 256, 128, 4, 0);
-  if (cols <= 64) return f(ln_fwd_group_kernel<16, 4, false, 4>, 256, 64, 4, 0);
-  if (cols <= 128) return f(ln_fwd_group_kernel<32, 4, false, 4>, 256, 32, 4, 0);
-  if (cols <= 256) return f(ln_fwd_group_kernel<32, 8, false, 2>, 256, 16, 2, 0);
-  if (cols <= 512) return f(ln_fwd_group_kernel<32, 16, false, 1>, 256, 8, 1, 0);
-  if (cols <= 1024) return f(ln_fwd_group_kernel<32, 32, false, 1>, 256, 8, 1, 0);
-  if (cols <= 2048) return f(ln_fwd_block_kernel<256, 8, false>, 256, 1, 1, 0);
-  if (cols <= 4096) return f(ln_fwd_block_kernel<512, 8, false>, 512, 1, 1, 0);
-  if (cols <= 8192) return f(ln_fwd_block_kernel<1024, 8, false>, 1024, 1, 1, 0);
-  if (cols <= 16384) return f(ln_fwd_block_kernel<1024, 16, false>, 1024, 1, 1, 0);
+  if (cols <= 16) return f(ln_fwd_group_kernel<4, 4, 2>, 256, 128, 2, 0);
+  if (cols <= 32) return f(ln_fwd_group_kernel<8, 4, 4>, 256, 128, 4, 0);
+  if (cols <= 64) return f(ln_fwd_group_kernel<16, 4, 4>, 256, 64, 4, 0);
+  if (cols <= 128) return f(ln_fwd_group_kernel<32, 4, 4>, 256, 32, 4, 0);
+  if (cols <= 256) return f(ln_fwd_group_kernel<32, 8, 2>, 256, 16, 2, 0);
+  if (cols <= 512) return f(ln_fwd_group_kernel<32, 16, 1>, 256, 8, 1, 0);
+  if (cols <= 1024) return f(ln_fwd_group_kernel<32, 32, 1>, 256, 8, 1, 0);
+  if (cols <= 2048) return f(ln_fwd_block_kernel<256, 8>, 256, 1, 1, 0);
+  if (cols <= 4096) return f(ln_fwd_block_kernel<512, 8>, 512, 1, 1, 0);
+  if (cols <= 8192) return f(ln_fwd_block_kernel<1024, 8>, 1024, 1, 1, 0);
+  if (cols <= 16384) return f(ln_fwd_block_kernel<1024, 16>, 1024, 1, 1, 0);
   return f(ln_fwd_long_kernel, kLong, 1, 1, 0);
 }
 template <int THREADS, int LANES, int PER, int D, int MIN_BLOCKS, class F>
@@ -764,16 +785,16 @@ auto bwd_aligned(int cols, F f) {
 }
 template <class F>
 auto bwd_plain(int cols, F f) {
-  if (cols <= 16) return f(ln_bwd_group_kernel<4, 4, false, 2>, 256, 128, 2, 0);
-  if (cols <= 32) return f(ln_bwd_group_kernel<8, 4, false, 2>, 256, 64, 2, 0);
-  if (cols <= 64) return f(ln_bwd_group_kernel<16, 4, false, 2>, 256, 32, 2, 0);
-  if (cols <= 128) return f(ln_bwd_group_kernel<32, 4, false, 2>, 256, 16, 2, 0);
-  if (cols <= 256) return f(ln_bwd_group_kernel<32, 8, false, 2>, 256, 16, 2, 0);
-  if (cols <= 512) return f(ln_bwd_group_kernel<32, 16, false, 1>, 256, 8, 1, 0);
-  if (cols <= 1024) return f(ln_bwd_block_kernel<256, 4, false>, 256, 1, 1, 0);
-  if (cols <= 2048) return f(ln_bwd_block_kernel<256, 8, false>, 256, 1, 1, 0);
-  if (cols <= 4096) return f(ln_bwd_block_kernel<512, 8, false>, 512, 1, 1, 0);
-  if (cols <= 8192) return f(ln_bwd_block_kernel<1024, 8, false>, 1024, 1, 1, 0);
+  if (cols <= 16) return f(ln_bwd_group_kernel<4, 4, 2>, 256, 128, 2, 0);
+  if (cols <= 32) return f(ln_bwd_group_kernel<8, 4, 2>, 256, 64, 2, 0);
+  if (cols <= 64) return f(ln_bwd_group_kernel<16, 4, 2>, 256, 32, 2, 0);
+  if (cols <= 128) return f(ln_bwd_group_kernel<32, 4, 2>, 256, 16, 2, 0);
+  if (cols <= 256) return f(ln_bwd_group_kernel<32, 8, 2>, 256, 16, 2, 0);
+  if (cols <= 512) return f(ln_bwd_group_kernel<32, 16, 1>, 256, 8, 1, 0);
+  if (cols <= 1024) return f(ln_bwd_block_kernel<256, 4>, 256, 1, 1, 0);
+  if (cols <= 2048) return f(ln_bwd_block_kernel<256, 8>, 256, 1, 1, 0);
+  if (cols <= 4096) return f(ln_bwd_block_kernel<512, 8>, 512, 1, 1, 0);
+  if (cols <= 8192) return f(ln_bwd_block_kernel<1024, 8>, 1024, 1, 1, 0);
   if (cols <= 16384) return f(ln_bwd_wide_kernel<false>, kWideThreads, 1, 1, kWideBytes);
   return f(ln_bwd_long_kernel, kLong, 1, 1, 0);
 }
@@ -790,12 +811,15 @@ yl_status resident(yl_ctx* ctx, K kernel, int threads, int smem, long long* bloc
   return YL_OK;
 }
 
+constexpr int kMaxCols = 1 << 29;  // column indexes and twice their number stay ints
+
 bool aligned4(const void* p) { return ((uintptr_t)p & 3) == 0; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 yl_status check_ln(yl_ctx* ctx, const char* who, long long rows, int cols, float eps) {
   YL_CHECK(ctx, YL_ERR_INVALID, "%s: ctx is NULL", who);
-  YL_CHECK(rows >= 0 && cols >= 1, YL_ERR_SHAPE, "%s: %lld rows of %d columns", who, rows, cols);
+  YL_CHECK(rows >= 0 && cols >= 1 && cols <= kMaxCols, YL_ERR_SHAPE,
+           "%s: %lld rows of %d columns (1 to %d)", who, rows, cols, kMaxCols);
   YL_CHECK(eps >= 0.f, YL_ERR_INVALID, "%s: eps %g is negative or NaN", who, (double)eps);
   return YL_OK;
 }
@@ -857,6 +881,10 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
                ((addend == dx && ldadd == lddx) ||
                 !rows_overlap(addend, ldadd, rows, cols, dx, lddx, rows, cols)),
            YL_ERR_INVALID, "yl_layernorm_bwd: dx overlaps an input");
+  YL_CHECK(!rows_overlap(dgamma, cols, 1, cols, dbeta, cols, 1, cols) &&
+               !rows_overlap(dx, lddx, rows, cols, dgamma, cols, 1, cols) &&
+               !rows_overlap(dx, lddx, rows, cols, dbeta, cols, 1, cols),
+           YL_ERR_INVALID, "yl_layernorm_bwd: two results overlap");
   if (!dx && !dgamma && !dbeta) return YL_OK;
   DeviceGuard dev(ctx->device);
   YL_CUDA(dev.status());

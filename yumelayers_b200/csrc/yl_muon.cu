@@ -220,6 +220,25 @@ __global__ void __launch_bounds__(256)
   s = block_sum256(s);
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
+// The same over a table's gradients.
+__global__ void __launch_bounds__(256)
+    table_square_kernel(const __grid_constant__ Table t, float scale, int sanitize,
+                        double* __restrict__ part) {
+  const int k = find_item(t.chunks, t.count, blockIdx.x);
+  const Item& it = t.it[k];
+  const long long lo = (long long)(blockIdx.x - t.chunks[k]) * it.chunk;
+  const int n = (int)min((long long)it.chunk, (long long)it.rows * it.cols - lo);
+  const float* g = it.src + lo;
+  double s = 0.0;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += 256) {
+    float v = __ldg(g + i) * scale;
+    if (sanitize && !isfinite(v)) v = 0.f;
+    s += (double)v * v;
+  }
+  s = block_sum256(s);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
 __global__ void __launch_bounds__(256)
     grad_norm_final_kernel(const double* __restrict__ part, long long n, float* norm) {
   double s = 0.0;
@@ -228,11 +247,17 @@ __global__ void __launch_bounds__(256)
   if (threadIdx.x == 0) *norm = (float)sqrt(s);
 }
 
-// 1 / (|u|_F + eps) from the item's partials.
-__device__ __forceinline__ float inverse_norm(const Item& it, float eps) {
+// 1 / (sqrt(sum of squares) + eps); 0 for a zero matrix, NaN for one with a NaN or
+// an infinity.  In double, for matrices whose norm's inverse is no float.
+__device__ __forceinline__ double inverse_norm(double squares, float eps) {
+  if (squares == 0.0) return 0.0;
+  const double norm = sqrt(squares);
+  return isinf(norm) ? __longlong_as_double(0x7ff8000000000000LL) : 1.0 / (norm + (double)eps);
+}
+__device__ __forceinline__ double inverse_norm(const Item& it, float eps) {
   double s = 0.0;
   for (int c = threadIdx.x; c < it.chunks; c += 256) s += it.part[c];
-  return (float)(1.0 / (sqrt(block_sum256(s)) + (double)eps));
+  return inverse_norm(block_sum256(s), eps);
 }
 
 __device__ __forceinline__ void split_pair(float v, __half* hi, __half* lo) {
@@ -248,7 +273,7 @@ __global__ void __launch_bounds__(256)
   const Item& it = t->it[k];
   const int b = blockIdx.x - t->blocks[k];
   const int rb = b / it.cb, cb = b - rb * it.cb;
-  const float inv = inverse_norm(it, u.eps);
+  const double inv = inverse_norm(it, u.eps);
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   uint8_t* hi = it.x[0] + (size_t)b * kBlkBytes;
   uint8_t* lo = hi + (size_t)it.rb * it.cb * kBlkBytes;
@@ -278,7 +303,7 @@ __global__ void __launch_bounds__(256)
     }
     __align__(16) __half h[8], l[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) split_pair(v[j] * inv * sx, &h[j], &l[j]);
+    for (int j = 0; j < 8; ++j) split_pair((float)(v[j] * inv) * sx, &h[j], &l[j]);
     const int at = row * 128 + ((ch ^ (row & 7)) << 4);
     *reinterpret_cast<uint4*>(hi + at) = *reinterpret_cast<const uint4*>(h);
     *reinterpret_cast<uint4*>(lo + at) = *reinterpret_cast<const uint4*>(l);
@@ -291,14 +316,14 @@ __global__ void __launch_bounds__(256)
   const int k = find_item(t->chunks, t->count, blockIdx.x);
   const Item& it = t->it[k];
   const int chunk = blockIdx.x - t->chunks[k];
-  const float inv = inverse_norm(it, u.eps);
+  const double inv = inverse_norm(it, u.eps);
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   const long long total = (long long)it.rows * it.cols;
   const long long lo = (long long)chunk * it.chunk;
   const long long hi = min(total, lo + (long long)it.chunk);
   for (long long i = lo + threadIdx.x; i < hi; i += 256) {
     const long long r = i / it.cols, c = i - r * it.cols;
-    const float v = update_value(it, u, clipf, r, c) * inv;
+    const float v = (float)(update_value(it, u, clipf, r, c) * inv);
     if (u.muon) it.dst[i] = it.dst[i] * (1.f - u.lr * u.decay) - u.lr * it.scale * v;
     else it.dst[r * it.ldd + c] = v;
   }
@@ -1152,7 +1177,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   cluster_wait();
   double total = 0.0;
   for (int r = 0; r < share; ++r) total += norms[r];
-  const float inv = (float)(1.0 / (sqrt(total) + (double)u.eps));
+  const double inv = inverse_norm(total, u.eps);
 
   // Block (long, short) of the share: a wide X keeps its row blocks together (the
   // 128 rows of a K-major operand), a tall one its row blocks along the long side.
@@ -1170,7 +1195,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
     const int rblk = rr >> 6, r = rr & 63, cblk = cc >> 3, ch = cc & 7;
     float x[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = v[e][j] * inv * sx0;
+    for (int j = 0; j < 8; ++j) x[j] = (float)(v[e][j] * inv) * sx0;
     uint4 hi, lo;
     split8(x, &hi, &lo);
     uint8_t* at = smem + (tall ? xoff(rblk, cblk) : xoff(cblk, rblk)) + r * 128 + ((ch ^ (r & 7)) << 4);
@@ -1772,15 +1797,23 @@ yl_status newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int s
     it.src = t.x, it.dst = t.y, it.lds = t.ldx, it.ldd = t.ldy, it.rows = t.rows, it.cols = t.cols;
     items.push_back(it);
   }
-  for (size_t i = 0; i < items.size(); ++i)
-    for (size_t j = 0; j < items.size(); ++j) {
-      const Item &u = items[i], &v = items[j];
-      if (i < j)
-        YL_CHECK(!rows_overlap(u.dst, u.ldd, u.rows, u.cols, v.dst, v.ldd, v.rows, v.cols),
-                 YL_ERR_INVALID, "%s: two results overlap", who);
-      if (i == j && u.src == v.dst && u.lds == v.ldd) continue;  // in place
-      YL_CHECK(!rows_overlap(u.src, u.lds, u.rows, u.cols, v.dst, v.ldd, v.rows, v.cols),
-               YL_ERR_INVALID, "%s: a result overlaps an input", who);
+  // every result against every matrix whose extent meets its own
+  struct Extent { const float *p, *end; long long ld; const Item* it; bool out; };
+  std::vector<Extent> ext;
+  for (const Item& it : items)
+    for (int out = 0; out < 2; ++out) {
+      const float* p = out ? it.dst : it.src;
+      const long long ld = out ? it.ldd : it.lds;
+      ext.push_back({p, p + (it.rows - 1) * ld + it.cols, ld, &it, out != 0});
+    }
+  std::sort(ext.begin(), ext.end(), [](const Extent& x, const Extent& y) { return x.p < y.p; });
+  for (size_t i = 0; i < ext.size(); ++i)
+    for (size_t j = i + 1; j < ext.size() && ext[j].p < ext[i].end; ++j) {
+      const Extent &x = ext[i], &y = ext[j];
+      if (!x.out && !y.out) continue;
+      if (x.it == y.it && x.p == y.p && x.ld == y.ld) continue;  // in place
+      YL_CHECK(!rows_overlap(x.p, x.ld, x.it->rows, x.it->cols, y.p, y.ld, y.it->rows, y.it->cols),
+               YL_ERR_INVALID, "%s: a result overlaps another matrix of the table", who);
     }
   if (items.empty()) return YL_OK;
   DeviceGuard dev(ctx->device);
@@ -1855,8 +1888,13 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
   DeviceGuard dev(ctx->device);
   YL_CUDA(dev.status());
   size_t parts = 0;
-  if (measure)
-    for (const Item& it : items) parts += norm_parts((long long)it.rows * it.cols);
+  if (measure) {
+    for_tables(ctx, items, st.steps, [&](Table& t) {
+      place(&t, ctx->num_sms, nullptr);
+      for (int k = 0; k < t.count; ++k) parts += t.it[k].chunks;
+      return YL_OK;
+    });
+  }
   ScratchCarver carve;
   const size_t o_norm = carve.take(sizeof(float)), o_parts = carve.take(parts * sizeof(double));
   carve.offset = (carve.offset + 1023) & ~(size_t)1023;
@@ -1867,13 +1905,15 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
   if (measure) {
     double* part = (double*)(ws + o_parts);
     float* out = norm_out ? norm_out : (float*)(ws + o_norm);
-    for (const Item& it : items) {
-      const long long n = (long long)it.rows * it.cols;
-      grad_square_kernel<<<(unsigned)norm_parts(n), 256, 0, ctx->stream>>>(it.src, n, st.grad_scale,
-                                                                           st.sanitize, part);
-      YL_TRY(check_launch("grad_square_kernel"));
-      part += norm_parts(n);
-    }
+    YL_TRY(for_tables(ctx, items, st.steps, [&](Table& t) -> yl_status {
+      place(&t, ctx->num_sms, nullptr);
+      t.chunks[0] = 0;
+      for (int k = 0; k < t.count; ++k) t.chunks[k + 1] = t.chunks[k] + t.it[k].chunks;
+      table_square_kernel<<<t.chunks[t.count], 256, 0, ctx->stream>>>(t, st.grad_scale, st.sanitize,
+                                                                     part);
+      part += t.chunks[t.count];
+      return check_launch("table_square_kernel");
+    }));
     grad_norm_final_kernel<<<1, 256, 0, ctx->stream>>>((const double*)(ws + o_parts),
                                                        (long long)parts, out);
     YL_TRY(check_launch("grad_norm_final_kernel"));
