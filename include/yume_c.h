@@ -298,9 +298,8 @@ yl_status yl_adam_multi(yl_ctx* ctx, const yl_adam_tensor* table, int count, flo
 
 /* LayerNorm over the last axis of `rows` rows of `cols` floats (ldx, ldy, ...
  * are row strides in floats, at least cols): the rows of a Linear's input, or
- * the channels of every pixel of an NHWC activation.  The reference's Swift
- * path has none; its PyTorch prototype normalises transformer rows this way
- * (src/diffusion.py:12-35).
+ * the channels of every pixel of an NHWC activation.  No counterpart in the
+ * reference.
  *   mean = sum x / cols, var = sum (x - mean)^2 / cols, r = 1 / sqrt(var + eps),
  *   y = (x - mean) r gamma + beta     (gamma NULL: 1, beta NULL: 0).
  * mean_out / rstd_out (rows, optional) receive the statistics for the backward

@@ -288,6 +288,49 @@ public final class GpuSession {
         try check(yl_adam_update(ctx, param.ptr, grad.ptr, m.ptr, v.ptr, param.n, Int32(t), lr))
     }
 
+    // ------------------------------- operators without a reference counterpart
+    /// LayerNorm of every row of `a` (gamma and beta of a.cols values, or nil).
+    public func layerNorm(_ a: GPUTensor, gamma: GPUTensor? = nil, beta: GPUTensor? = nil,
+                          eps: Float = 1e-5) throws -> GPUTensor {
+        precondition(gamma.map { $0.n == a.cols } ?? true && beta.map { $0.n == a.cols } ?? true)
+        let c = try out(a.rows, a.cols)
+        try check(yl_layernorm_fwd(ctx, a.ptr, Int64(a.cols), Int64(a.rows), Int32(a.cols), eps,
+                                   gamma?.ptr, beta?.ptr, c.ptr, Int64(a.cols), nil, nil))
+        return c
+    }
+
+    /// Gradients of layerNorm: dx, dgamma, dbeta.
+    public func encodeLayerNormGrad(x: GPUTensor, dy: GPUTensor, gamma: GPUTensor? = nil,
+                                    eps: Float = 1e-5)
+        throws -> (dx: GPUTensor, dgamma: GPUTensor, dbeta: GPUTensor) {
+        precondition(x.n == dy.n && gamma.map { $0.n == x.cols } ?? true)
+        let dx = try out(x.rows, x.cols), dg = try out(1, x.cols), db = try out(1, x.cols)
+        let ld = Int64(x.cols)
+        try check(yl_layernorm_bwd(ctx, x.ptr, ld, dy.ptr, ld, Int64(x.rows), Int32(x.cols), eps,
+                                   gamma?.ptr, nil, nil, nil, 0, dx.ptr, ld, dg.ptr, db.ptr))
+        return (dx, dg, db)
+    }
+
+    /// Newton-Schulz orthogonalisation of `a`.
+    public func orthogonalize(_ a: GPUTensor, steps: Int = 5, eps: Float = 1e-7) throws -> GPUTensor {
+        let c = try out(a.rows, a.cols)
+        var m = yl_ns_matrix(x: a.ptr, y: c.ptr, rows: Int32(a.rows), cols: Int32(a.cols),
+                             ldx: Int64(a.cols), ldy: Int64(a.cols))
+        try check(yl_newton_schulz(ctx, &m, 1, Int32(steps), nil, eps))
+        return c
+    }
+
+    /// One Muon step of one weight matrix, in place.
+    public func muonUpdate(param: GPUTensor, grad: GPUTensor, momentum: GPUTensor, lr: Float,
+                           mu: Float = 0.95, nesterov: Bool = true, weightDecay: Float = 0,
+                           scale: Float = 1) throws {
+        precondition(param.n == grad.n && param.n == momentum.n)
+        var t = yl_muon_tensor(param: param.ptr, grad: grad.ptr, momentum: momentum.ptr,
+                               rows: Int32(param.rows), cols: Int32(param.cols), scale: scale)
+        try check(yl_muon_multi(ctx, &t, 1, lr, mu, nesterov ? 1 : 0, weightDecay, 5, nil, 1e-7, 1, 0,
+                                0, nil))
+    }
+
     // ------------------------------------------------ batched B200 operators
     /// ConvLayerGPU.forward (ConvGPU.swift:57-64) over a whole NCHW batch:
     /// one implicit-GEMM launch instead of im2col + matmul + biasRow per image.
@@ -347,5 +390,15 @@ public final class JointTrainer {
             }
         }
         return (losses[0], losses[1])
+    }
+
+    /// Muon for the hidden weight matrices from the next step on, Adam for the
+    /// rest; nil goes back to Adam everywhere.
+    public func setMuon(_ config: yl_muon_config?) throws {
+        if var cfg = config {
+            try check(yl_trainer_set_muon(handle, &cfg))
+        } else {
+            try check(yl_trainer_set_muon(handle, nil))
+        }
     }
 }
