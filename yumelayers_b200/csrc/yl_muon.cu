@@ -1214,7 +1214,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   // the hi plane's two descriptors, the lo planes lie `lplane`, `rplane` bytes on.
   auto multiply = [&](int kks, int chain, uint32_t idesc, uint32_t lplane, uint32_t rplane,
                       auto descriptors) {
-    fence_proxy_async_all();  // shared memory written by this block's threads
+    fence_proxy_async_smem();  // shared memory written by this block's threads
     __syncthreads();
     if (tid == 0) {
       tc_fence_after();
@@ -1299,7 +1299,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
         mbar_arrive_expect_tx(sums_in, (uint32_t)(mb * kBlk) * pitch);
         mbar_arrive_expect_tx(rows_in, (uint32_t)(2 * mb * mb) * kBlkBytes);
       }
-      fence_proxy_async_all();
+      fence_proxy_async_smem();
       __syncthreads();
       const uint32_t bytes = rows * pitch;  // to and from one block
       if (tid < share) {
@@ -1331,7 +1331,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       // ---- finished rows to every block: in both planes and each column block the
       // rows of a block lie together.  The outbox is free again once every block has
       // its sums, which the barrier says.
-      fence_proxy_async_all();
+      fence_proxy_async_smem();
       cluster_arrive();
       cluster_wait();
       const uint32_t piece = rows * 128;
@@ -1344,7 +1344,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
         *reinterpret_cast<uint4*>(to) = hi[i];
         *reinterpret_cast<uint4*>(to + mb * piece) = lo[i];
       }
-      fence_proxy_async_all();
+      fence_proxy_async_smem();
       __syncthreads();
       const int row0a = rank * rows;
       for (int k = tid; k < share * 2 * mb; k += kChipThreads) {
@@ -1567,15 +1567,21 @@ bool on_chip(const Item& it) {
   return mb <= 2 && nb <= kChipShare * (kChipBlocks / mb);
 }
 
+// Blocks that the longest of these matrices needs for its share to fit.
+int least_share(const Item* items, int count) {
+  int share = 1;
+  for (int k = 0; k < count; ++k) {
+    const int rb = (items[k].rows + kBlk - 1) / kBlk, cb = (items[k].cols + kBlk - 1) / kBlk;
+    while (share * (kChipBlocks / std::min(rb, cb)) < std::max(rb, cb)) share *= 2;
+  }
+  return share;
+}
+
 yl_status run_chip(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s) {
   place(&t, ctx->num_sms, nullptr);  // sizes only: nothing of these is in the workspace
   // as many blocks to a matrix as its long side needs, and more while SMs are idle
-  int longest = 0, share = 1;
-  for (int k = 0; k < t.count; ++k) {
-    const int nb = std::max(t.it[k].rb, t.it[k].cb);
-    longest = std::max(longest, nb);
-    while (share * (kChipBlocks / t.it[k].mb) < nb) share *= 2;
-  }
+  int longest = 0, share = least_share(t.it, t.count);
+  for (int k = 0; k < t.count; ++k) longest = std::max({longest, t.it[k].rb, t.it[k].cb});
   // (clusters of 16 find room for only a few of themselves)
   while (share < longest && 2 * share * t.count <= (share < 8 ? 1.0 : 0.5) * ctx->num_sms &&
          share < kChipShare)
@@ -1664,8 +1670,12 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn 
     if (wide(it)) tiles += (long long)((it.rows + 127) / 128) * ((it.cols + 127) / 128);
   const bool pairs = tiles >= 6LL * ctx->num_sms;
   // With longer matrices beside them the short ones cost the steps kernel less
-  // than a launch of their own.
-  const bool chip = steps > 0 && std::all_of(items.begin(), items.end(), on_chip);
+  // than a launch of their own, and so do more clusters than the SMs hold at once
+  // (24 of 128 x 1152: 267 us in clusters of 8, 168 us in the steps kernel; 14 of
+  // them 138 and 158 us).
+  const bool chip = steps > 0 && std::all_of(items.begin(), items.end(), on_chip) &&
+                    (long long)items.size() * least_share(items.data(), (int)items.size()) <=
+                        ctx->num_sms;
   auto t = std::make_unique<Table>();
   t->chip = chip;
   for (int pair = 1; pair >= 0; --pair) {
