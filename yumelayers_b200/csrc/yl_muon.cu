@@ -1506,9 +1506,10 @@ size_t place(Table* t, int num_sms, char* ws) {
     it.p = take(mb);
     it.part = (double*)take(it.chunks * sizeof(double));
   }
-  // Shares of GRAM's long side: as many as bring its tickets down to the average
-  // per SM, and at most sqrt(nk / 2), where the sums' way through memory costs as
-  // much as the k-blocks it saves (about 0.6 us a share against 0.4 us a k-block).
+  // Shares of GRAM's long side: at most as many as bring its tickets down to the
+  // average per SM, and of those the number with the shortest way through a tile.
+  // A k-block takes about 1.1k cycles; the sums' way through memory 5k, and 1.2k
+  // more for each share that the last block reads.
   auto nk = [](const Item& it) { return std::max(it.rb, it.cb); };
   const int ctas = t->pair ? 2 : 1, workers = num_sms / ctas;
   auto gram_tiles = [&](const Item& it) {
@@ -1521,8 +1522,16 @@ size_t place(Table* t, int num_sms, char* ws) {
   int splits = 0;
   for (int k = 0; k < t->count; ++k) {
     Item& it = t->it[k];
-    const double most = std::min(std::round(nk(it) / std::max(fair, 1.0)), std::sqrt(nk(it) / 2.0));
-    it.ks = std::max(1, (int)most);
+    const int most = (int)std::round(nk(it) / std::max(fair, 1.0));
+    double best = 1.1 * nk(it);
+    it.ks = 1;
+    for (int ks = 2; ks <= std::min(most, nk(it)); ++ks) {
+      const double cost = 1.1 * nk(it) / ks + 5 + 1.2 * ks;
+      if (cost < best) {
+        best = cost;
+        it.ks = ks;
+      }
+    }
     it.split0 = splits;
     it.partial = nullptr;
     if (it.ks > 1) {
