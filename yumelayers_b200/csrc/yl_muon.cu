@@ -343,11 +343,13 @@ __global__ void __launch_bounds__(256)
 // which every tile comes after the tiles it needs, and a taken ticket belongs to
 // a running block, so the waits end however many blocks are resident.
 //
-// Warp 8 streams operand blocks (128 x 64 of either side, both planes: 64 KB a
-// stage; half of that on the diagonal, where both sides are the same) through a
-// ring of three stages, warp 9 issues the tcgen05.mma, and warps 0-7 add each
-// finished accumulator into registers (64 columns of 32 rows per warp) and write
-// the tile.
+// Warp 10 takes the tickets and works out what they are, which with its trips to
+// memory takes 2.3 us (behind warp 8's loads it held up every tile: 2048 x 2048
+// 576 us, with a warp of its own 526).  Warp 8 streams operand blocks (128 x 64 of
+// either side, both planes: 64 KB a stage; half of that on the diagonal, where both
+// sides are the same) through a ring of three stages, warp 9 issues the
+// tcgen05.mma, and warps 0-7 add each finished accumulator into registers (64
+// columns of 32 rows per warp) and write the tile.
 // The tensor core truncates when it adds to its accumulator: kept there over a
 // whole row, a 384 x 1153 matrix ended 2.4e-5 off, where an fp32 product gives
 // 2e-6.  So an accumulator takes a few 16-deep products only, the small ones
@@ -381,7 +383,10 @@ constexpr int kSmemBytes = kBarOff + 1536 + 1024;  // barriers and prefixes, ali
 // take over what the third does not need: 2 * 216 + 72 = 3 * 168.
 constexpr int kProductThreads = 384;
 constexpr int kRegsEpilogue = 216, kRegsOthers = 72;
-constexpr int kRing = 4;     // tickets on their way from the producer to the other warps
+constexpr int kRing = 4;     // tickets on their way from the scheduler to the other warps
+// k-blocks left to load when the next ticket is taken: 1 costs as much on large
+// tables and 1% more on those of many short tickets
+constexpr int kAskAhead = 4;
 constexpr int kTmemCols = 512;
 
 template <bool PAIR>
@@ -404,6 +409,7 @@ struct Steps {
 struct Ticket {
   int step, mode, item, i, j, kb0, nk, share, tile;
 };
+constexpr int kTicketInts = sizeof(Ticket) / 4, kNoTicket = -1;  // mode behind the last one
 
 // `start` is the table's tiles[3][kMaxItems + 1] in shared memory.
 template <bool PAIR>
@@ -529,10 +535,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   uint64_t* acc_empty = acc_full + kAccs;  // rank 0
   uint64_t* tfull = acc_empty + kAccs;
   uint64_t* tempty = tfull + kRing;        // rank 0
-  uint64_t* drain = tempty + kRing;
+  uint64_t* ready = tempty + kRing;        // the ticket's operands are there
+  uint64_t* ask = ready + kRing;           // rank 0
+  uint64_t* drain = ask + 1;
   uint64_t* esync = drain + 1;
-  int* ring = reinterpret_cast<int*>(esync + 1);
-  int* last_share = ring + kRing;
+  Ticket* ring = reinterpret_cast<Ticket*>(esync + 1);
+  int* last_share = reinterpret_cast<int*>(ring + kRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last_share + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 1);  // [3][kMaxItems + 1]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -552,9 +560,11 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     }
     for (int b = 0; b < kRing; ++b) {
       mbar_init(&tfull[b], 1);
-      // rank 0: the MMA thread and the epilogue; rank 1: producer, relay, epilogue
-      mbar_init(&tempty[b], 1 + kEpiWarps + (PAIR ? 2 + kEpiWarps : 0));
+      mbar_init(&ready[b], 1);
+      // rank 0: producer, MMA thread, epilogue; rank 1: these (as relay) and the scheduler
+      mbar_init(&tempty[b], 2 + kEpiWarps + (PAIR ? 3 + kEpiWarps : 0));
     }
+    mbar_init(ask, 1);
     mbar_init(drain, 1);
     mbar_init(esync, kEpiWarps);
     fence_barrier_init();
@@ -586,25 +596,30 @@ __global__ void __launch_bounds__(kProductThreads, 1)
 
   if (warp >= kEpiWarps) {
     reg_dec<kRegsOthers>();
-  if (warp == kEpiWarps) {
+  if (warp == kEpiWarps + 2) {
+    // scheduler: takes the tickets and waits until what they need is done
     if (lane == 0) {
-      uint32_t it = 0;
-      bool ok = true;
-      for (uint32_t k = 0; ok; ++k) {
+      for (uint32_t k = 0;; ++k) {
         const int slot = k % kRing;
-        int n;
+        Ticket q;
         if (rank == 0) {
-          // taken no earlier than its loads could start: a ticket held back here is
-          // one that an idle block would have begun
-          n = atomicAdd(t->ctrl, 1);
-          if (k >= kRing && !wait<PAIR>(&tempty[slot], (k / kRing - 1) & 1, lim)) {
+          // taken no earlier than its loads could nearly start: a ticket held back
+          // here is one that an idle block would have begun
+          if ((k > 0 && !mbar_wait(ask, (k - 1) & 1, lim)) ||
+              (k >= kRing && !wait<PAIR>(&tempty[slot], (k / kRing - 1) & 1, lim))) {
             report_error(err, YL_DEVERR_TIMEOUT);
             break;
           }
-          ring[slot] = n;
+          const int n = atomicAdd(t->ctrl, 1);
+          q.mode = kNoTicket;
+          if (n < total) q = ticket_of<PAIR>(t, start, count, n);
+          ring[slot] = q;
           mbar_arrive(&tfull[slot]);
           if (PAIR) {
-            st_cluster_s32(map_to_rank(smem_u32(&ring[slot]), 1), n);
+            const int* words = reinterpret_cast<const int*>(&ring[slot]);
+            const uint32_t there = map_to_rank(smem_u32(words), 1);
+#pragma unroll
+            for (int w = 0; w < kTicketInts; ++w) st_cluster_s32(there + 4 * w, words[w]);
             mbar_arrive_cluster(map_to_rank(smem_u32(&tfull[slot]), 1));
           }
         } else {
@@ -612,30 +627,49 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             report_error(err, YL_DEVERR_TIMEOUT);
             break;
           }
-          n = ring[slot];
+          q = ring[slot];
           arrive0(&tempty[slot]);
         }
-        if (n >= total) break;
-        const Ticket q = ticket_of<PAIR>(t, start, count, n);
+        if (q.mode == kNoTicket) break;
+        int value;
+        const int* counter = needs<PAIR>(t, start, q, &value);
+        const long long t0 = clock64();
+        bool ok = true;
+        while (ok && load_acquire(counter) < value) ok = clock64() - t0 <= lim;
+        if (!ok) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+          break;
+        }
+        mbar_arrive(&ready[slot]);
+      }
+    }
+  } else if (warp == kEpiWarps) {
+    if (lane == 0) {
+      uint32_t it = 0;
+      bool ok = true;
+      for (uint32_t k = 0; ok; ++k) {
+        const int slot = k % kRing;
+        if (!wait<PAIR>(&tfull[slot], (k / kRing) & 1, lim)) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+          break;
+        }
+        const Ticket q = ring[slot];
+        arrive0(&tempty[slot]);
+        if (q.mode == kNoTicket) break;
         const Item& im = t->it[q.item];
         const Operand L = operand(im, q.mode, q.step & 1, 0), R = operand(im, q.mode, q.step & 1, 1);
         const bool same = q.mode != UPDATE && q.i == q.j;
         const int l0 = F::kSide * q.i + 2 * rank, r0 = F::kSide * q.j + 2 * rank;
         const int nl = max(0, min(2, L.nmn - l0)), nr = same ? 0 : max(0, min(2, R.nmn - r0));
-        int value;
-        const int* counter = needs<PAIR>(t, start, q, &value);
-        const long long t0 = clock64();
-        while (load_acquire(counter) < value) {
-          if (clock64() - t0 > lim) {
-            report_error(err, YL_DEVERR_TIMEOUT);
-            ok = false;
-            break;
-          }
+        if (!mbar_wait(&ready[slot], (k / kRing) & 1, lim)) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+          break;
         }
-        if (!ok) break;
         const int extra = q.mode == SQUARE ? F::kCtas : 0;  // stages with the tile's own A
-        fence_proxy_async_all();  // what the acquire saw, before this thread's bulk loads
+        fence_proxy_async_all();  // what the scheduler saw, before this thread's bulk loads
+        const int ask_at = max(0, q.nk + extra - kAskAhead);
         for (int kb = 0; kb < q.nk + extra; ++kb, ++it) {
+          if (kb == ask_at && rank == 0) mbar_arrive(ask);
           const int s = it % kStages;
           if (it >= kStages && !wait<PAIR>(&empty[s], ((it / kStages) - 1) & 1, lim)) {
             report_error(err, YL_DEVERR_TIMEOUT);
@@ -683,10 +717,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           report_error(err, YL_DEVERR_TIMEOUT);
           break;
         }
-        const int n = ring[slot];
+        const Ticket q = ring[slot];
         arrive0(&tempty[slot]);
-        if (n >= total) break;
-        const Ticket q = ticket_of<PAIR>(t, start, count, n);
+        if (q.mode == kNoTicket) break;
         const int extra = q.mode == SQUARE ? F::kCtas : 0;
         if (rank != 0) {  // tell rank 0 of every stage that has landed here
           for (int kb = 0; kb < q.nk + extra; ++kb, ++it) {
@@ -797,11 +830,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         report_error(err, YL_DEVERR_TIMEOUT);
         break;
       }
-      const int n = ring[slot];
+      const Ticket q = ring[slot];
       __syncwarp();
       if (lane == 0) arrive0(&tempty[slot]);
-      if (n >= total) break;
-      const Ticket q = ticket_of<PAIR>(t, start, count, n);
+      if (q.mode == kNoTicket) break;
       const Item& im = t->it[q.item];
       if (u.muon && q.mode == UPDATE && q.step + 1 == steps.n) {
         // the parameter's rows towards L2 while the products run: a row of this
