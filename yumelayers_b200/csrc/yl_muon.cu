@@ -498,8 +498,9 @@ __device__ __forceinline__ int load_acquire(const int* p) {
 __device__ __forceinline__ void add_release(int* p, int v) {
   asm volatile("fence.acq_rel.gpu; red.relaxed.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
-__device__ __forceinline__ void fence_proxy_async_all() {
-  asm volatile("fence.proxy.async;" ::: "memory");
+// (the fence for every state space costs 0.35 us more, in front of every tile)
+__device__ __forceinline__ void fence_proxy_async_global() {
+  asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
 // The counter a ticket waits for, and the value it must have reached (every
@@ -666,7 +667,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           break;
         }
         const int extra = q.mode == SQUARE ? F::kCtas : 0;  // stages with the tile's own A
-        fence_proxy_async_all();  // what the scheduler saw, before this thread's bulk loads
+        fence_proxy_async_global();  // what the scheduler saw, before this thread's bulk loads
         const int ask_at = max(0, q.nk + extra - kAskAhead);
         for (int kb = 0; kb < q.nk + extra; ++kb, ++it) {
           if (kb == ask_at && rank == 0) mbar_arrive(ask);
