@@ -303,7 +303,8 @@ yl_status yl_adam_multi(yl_ctx* ctx, const yl_adam_tensor* table, int count, flo
  *   mean = sum x / cols, var = sum (x - mean)^2 / cols, r = 1 / sqrt(var + eps),
  *   y = (x - mean) r gamma + beta     (gamma NULL: 1, beta NULL: 0).
  * mean_out / rstd_out (rows, optional) receive the statistics for the backward
- * call.  y may be x itself (same stride); any other overlap is YL_ERR_INVALID.
+ * call.  y may be x itself (same stride); any other overlap of a result is
+ * YL_ERR_INVALID.
  * A row with a NaN or an infinity becomes NaN; other rows do not see it.
  * Columns past cols in a padded row are neither read nor written.  cols goes to
  * 2^29. */
@@ -315,8 +316,8 @@ yl_status yl_layernorm_fwd(yl_ctx* ctx, const float* x, long long ldx, long long
  *   dgamma = sum over rows of dy h, dbeta = sum over rows of dy (overwritten;
  *   zero for rows = 0; fixed summation order).
  * mean and rstd come from the forward call or are both NULL (recomputed with
- * eps).  dx, dgamma, dbeta may be NULL.  dx may be addend (same stride); it
- * must not overlap x or dy (YL_ERR_INVALID). */
+ * eps).  dx, dgamma, dbeta may be NULL.  dx may be addend (same stride); any
+ * other overlap of a result is YL_ERR_INVALID. */
 yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const float* dy,
                            long long lddy, long long rows, int cols, float eps, const float* gamma,
                            const float* mean, const float* rstd, const float* addend,
@@ -352,8 +353,8 @@ yl_status yl_newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, in
  *   param <- param (1 - lr weight_decay) - lr scale NS(u)
  * with NS, steps, coeffs and eps as in yl_newton_schulz.  scale is each matrix's
  * own factor on lr, e.g. sqrt(max(1, rows / cols)).  norm_out_dev (optional)
- * receives the pre-clip norm.  Parameters and momenta must not overlap anything
- * else in the table (YL_ERR_INVALID).  Equal calls give equal bits; a matrix in
+ * receives the pre-clip norm.  Parameters, momenta and the norm must not overlap
+ * anything else of the call (YL_ERR_INVALID).  Equal calls give equal bits; a matrix in
  * another table may come out with other roundings.  No counterpart in the
  * reference. */
 typedef struct yl_muon_tensor {

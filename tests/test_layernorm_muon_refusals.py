@@ -3,8 +3,10 @@ of them come before the first device call, so they run without a GPU on a
 stand-in for the context."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
+from yumelayers_b200 import ops
 from yumelayers_b200._lib import MuonTensor, NsMatrix, YumeError, call
 
 SHAPE, INVALID, UNSUPPORTED = 1, 7, 8
@@ -52,6 +54,28 @@ def test_layernorm_fwd_refuses(ctx, bad, status):
 ])
 def test_layernorm_bwd_refuses(ctx, bad, status):
     refused(status, *bwd(ctx, **bad))
+
+
+def test_layernorm_fwd_refuses_results_in_other_arguments(ctx):
+    c, x, ldx, rows, cols, eps, _, _, y, ldy, _, _ = fwd(ctx)[1:]
+    v = BASE + (4 << 20)
+    for gamma, beta, mean, rstd in (
+            (y + 4, None, None, None), (None, y + 400, None, None), (None, None, y, None),
+            (None, None, None, x), (None, None, v, v), (None, None, v, v + 28), (v, None, v + 252, None),
+            (None, v, None, v)):
+        refused(INVALID, "yl_layernorm_fwd", c, x, ldx, rows, cols, eps, gamma, beta, y, ldy, mean,
+                rstd)
+
+
+def test_layernorm_bwd_refuses_results_in_other_arguments(ctx):
+    v, x, dy, dx = BASE + (4 << 20), BASE, BASE + (1 << 20), BASE + (2 << 20)
+    for gamma, mean, rstd, dg, db in (
+            (v, None, None, v, None), (v, None, None, None, v + 252), (None, v, v + 64, v + 28, None),
+            (None, v, v + 64, None, v + 64), (None, None, None, x + 512, None),
+            (None, None, None, None, dy), (dx, None, None, None, None), (None, dx, v, None, None),
+            (None, v, dx + 8, None, None)):
+        refused(INVALID, "yl_layernorm_bwd", ctx, x, 64, dy, 64, 8, 64, 1e-5, gamma, mean, rstd,
+                None, 64, dx, 64, dg, db)
 
 
 def test_layernorm_bwd_refuses_overlapping_results(ctx):
@@ -103,10 +127,10 @@ def test_newton_schulz_with_nothing_to_do(ctx):
     call(*ns(ctx, (None, None, 0, 7, 7, 7), (None, None, 3, 0, 0, 0)))
 
 
-def muon(ctx, *mats, steps=5, eps=1e-7):
+def muon(ctx, *mats, steps=5, eps=1e-7, norm=None):
     table = (MuonTensor * len(mats))(*[MuonTensor(*m) for m in mats])
     return ("yl_muon_multi", ctx, table, len(mats), 0.02, 0.95, 1, 0.0, steps, None, eps, 1.0, 0.0,
-            0, None)
+            0, norm)
 
 
 P, G, M = BASE, BASE + (1 << 24), BASE + (2 << 24)
@@ -121,6 +145,9 @@ P, G, M = BASE, BASE + (1 << 24), BASE + (2 << 24)
     ([(P, G, G, 4, 4, 1.0)], {}, INVALID), ([(P, P + 32, M, 4, 4, 1.0)], {}, INVALID),
     ([(P, G, M, 4, 4, 1.0)], dict(steps=40), INVALID),
     ([(P, G, M, 4, 4, 1.0)], dict(eps=float("nan")), INVALID),
+    ([(P, G, M, 4, 4, 1.0)], dict(norm=P + 60), INVALID),
+    ([(P, G, M, 4, 4, 1.0)], dict(norm=G), INVALID),
+    ([(P, G, M, 4, 4, 1.0)], dict(norm=M + 65), INVALID),
 ])
 def test_muon_refuses(ctx, mats, kw, status):
     refused(status, *muon(ctx, *mats, **kw))
@@ -131,3 +158,25 @@ def test_null_context():
     refused(INVALID, *bwd(None))
     refused(INVALID, *ns(None))
     refused(INVALID, *muon(None))
+
+
+def test_ops_refuse_arguments_of_other_sizes():
+    x = np.zeros((3, 8), np.float32)
+    for bad in (dict(gamma=np.ones(7)), dict(beta=np.ones(9)), dict(gamma=np.ones((2, 8)))):
+        with pytest.raises(ValueError, match="values, not 8"):
+            ops.layernorm_fwd(x, **bad)
+    for bad in (dict(gamma=np.ones(4)), dict(mean=np.ones(4), rstd=np.ones(3)),
+                dict(mean=np.ones(3), rstd=np.ones(2)), dict(dy=x[:2]), dict(addend=x[:, :7])):
+        with pytest.raises(ValueError):
+            ops.layernorm_bwd(x, **{"dy": x, **bad})
+    for empty in (np.zeros((3, 0)), np.float32(1)):
+        with pytest.raises(ValueError, match="no columns"):
+            ops.layernorm_fwd(empty)
+    with pytest.raises(ValueError, match="two axes"):
+        ops.newton_schulz([x, x[0]])
+    with pytest.raises(ValueError, match="two axes"):
+        ops.muon_multi([x[0]], [x[0]], [x[0]], 0.1)
+    with pytest.raises(ValueError, match="shapes"):
+        ops.muon_multi([x], [x.T], [x], 0.1)
+    with pytest.raises(ValueError, match="scales"):
+        ops.muon_multi([x], [x], [x], 0.1, scales=[1.0, 2.0])

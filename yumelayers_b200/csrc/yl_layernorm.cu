@@ -816,6 +816,23 @@ constexpr int kMaxCols = 1 << 29;  // column indexes and twice their number stay
 bool aligned4(const void* p) { return ((uintptr_t)p & 3) == 0; }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// An argument of a call: rows of cols floats at a row stride of ld.
+struct Span {
+  const float* p;
+  long long ld, rows, cols;
+};
+// Whether one of the first `outs` spans shares an element with any other span;
+// in_place: the two of this pair may be one and the same.
+bool results_overlap(const Span* s, int outs, int count, int in_place_out, int in_place_in) {
+  for (int i = 0; i < outs; ++i)
+    for (int j = i + 1; j < count; ++j) {
+      if (i == in_place_out && j == in_place_in && s[i].p == s[j].p && s[i].ld == s[j].ld) continue;
+      if (rows_overlap(s[i].p, s[i].ld, s[i].rows, s[i].cols, s[j].p, s[j].ld, s[j].rows, s[j].cols))
+        return true;
+    }
+  return false;
+}
+
 yl_status check_ln(yl_ctx* ctx, const char* who, long long rows, int cols, float eps) {
   YL_CHECK(ctx, YL_ERR_INVALID, "%s: ctx is NULL", who);
   YL_CHECK(rows >= 0 && cols >= 1 && cols <= kMaxCols, YL_ERR_SHAPE,
@@ -839,8 +856,10 @@ yl_status yl_layernorm_fwd(yl_ctx* ctx, const float* x, long long ldx, long long
            YL_ERR_INVALID, "yl_layernorm_fwd: a pointer is not a multiple of 4 bytes");
   YL_CHECK(ldx >= cols && ldy >= cols, YL_ERR_SHAPE,
            "yl_layernorm_fwd: row strides %lld, %lld are smaller than %d columns", ldx, ldy, cols);
-  YL_CHECK((x == y && ldx == ldy) || !rows_overlap(x, ldx, rows, cols, y, ldy, rows, cols),
-           YL_ERR_INVALID, "yl_layernorm_fwd: y overlaps x");
+  const Span spans[] = {{y, ldy, rows, cols},     {mean_out, rows, 1, rows}, {rstd_out, rows, 1, rows},
+                        {x, ldx, rows, cols},     {gamma, cols, 1, cols},    {beta, cols, 1, cols}};
+  YL_CHECK(!results_overlap(spans, 3, 6, 0, 3), YL_ERR_INVALID,
+           "yl_layernorm_fwd: a result overlaps another argument");
   DeviceGuard dev(ctx->device);
   YL_CUDA(dev.status());
   const Fwd p{x, ldx, rows, cols, eps, gamma, beta, y, ldy, mean_out, rstd_out};
@@ -876,15 +895,11 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
   YL_CHECK(x && dy, YL_ERR_INVALID, "yl_layernorm_bwd: NULL argument");
   YL_CHECK(ldx >= cols && lddy >= cols && (!addend || ldadd >= cols) && (!dx || lddx >= cols),
            YL_ERR_SHAPE, "yl_layernorm_bwd: a row stride is smaller than %d columns", cols);
-  YL_CHECK(!rows_overlap(x, ldx, rows, cols, dx, lddx, rows, cols) &&
-               !rows_overlap(dy, lddy, rows, cols, dx, lddx, rows, cols) &&
-               ((addend == dx && ldadd == lddx) ||
-                !rows_overlap(addend, ldadd, rows, cols, dx, lddx, rows, cols)),
-           YL_ERR_INVALID, "yl_layernorm_bwd: dx overlaps an input");
-  YL_CHECK(!rows_overlap(dgamma, cols, 1, cols, dbeta, cols, 1, cols) &&
-               !rows_overlap(dx, lddx, rows, cols, dgamma, cols, 1, cols) &&
-               !rows_overlap(dx, lddx, rows, cols, dbeta, cols, 1, cols),
-           YL_ERR_INVALID, "yl_layernorm_bwd: two results overlap");
+  const Span spans[] = {{dx, lddx, rows, cols}, {dgamma, cols, 1, cols},   {dbeta, cols, 1, cols},
+                        {x, ldx, rows, cols},   {dy, lddy, rows, cols},    {addend, ldadd, rows, cols},
+                        {gamma, cols, 1, cols}, {mean, rows, 1, rows},     {rstd, rows, 1, rows}};
+  YL_CHECK(!results_overlap(spans, 3, 9, 0, 5), YL_ERR_INVALID,
+           "yl_layernorm_bwd: a result overlaps another argument");
   if (!dx && !dgamma && !dbeta) return YL_OK;
   DeviceGuard dev(ctx->device);
   YL_CUDA(dev.status());

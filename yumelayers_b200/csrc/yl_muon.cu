@@ -1822,6 +1822,8 @@ bool rows_overlap(const float* a, long long lda, long long rows_a, long long col
   const uintptr_t a1 = a0 + 4 * ((uintptr_t)(rows_a - 1) * lda + cols_a);
   const uintptr_t b1 = b0 + 4 * ((uintptr_t)(rows_b - 1) * ldb + cols_b);
   if (a1 <= b0 || b1 <= a0) return false;
+  if (rows_a == 1) lda = ldb;  // (a single row has no stride)
+  if (rows_b == 1) ldb = lda;
   if (lda != ldb) return true;
   // columns of one buffer side by side?  (b - a) modulo the row stride
   long long d = ((long long)(b0 - a0) / 4) % lda;
@@ -1927,11 +1929,14 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
     r.push_back({(uintptr_t)it.mom, (uintptr_t)it.mom + bytes, true});
     r.push_back({(uintptr_t)it.dst, (uintptr_t)it.dst + bytes, true});
   }
+  YL_CHECK(!((uintptr_t)norm_out & 3), YL_ERR_INVALID,
+           "%s: norm_out_dev is not a multiple of 4 bytes", who);
+  if (norm_out) r.push_back({(uintptr_t)norm_out, (uintptr_t)(norm_out + 1), true});
   std::sort(r.begin(), r.end(), [](const Range& x, const Range& y) { return x.lo < y.lo; });
   uintptr_t end = 0, wend = 0;  // behind every range so far, and every written one
   for (const Range& x : r) {
     YL_CHECK(!(x.lo < wend || (x.write && x.lo < end)), YL_ERR_INVALID,
-             "%s: a parameter or momentum overlaps another tensor of the table", who);
+             "%s: a parameter, a momentum or the norm overlaps another tensor", who);
     end = std::max(end, x.hi);
     if (x.write) wend = std::max(wend, x.hi);
   }

@@ -153,13 +153,26 @@ def adam_multi(params, grads, ms, vs, lr, t, b1=0.9, b2=0.999, eps=1e-8, grad_sc
     return out[0], out[1], out[2], float(nd.toArray()[0])
 
 
+def _rows(who, x):
+    """x as float32 with its number of rows and of columns (the last axis)."""
+    x = np.asarray(x, np.float32)
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{who}: x of shape {x.shape} has no columns")
+    return x, x.size // x.shape[-1], x.shape[-1]
+
+
+def _vectors(who, n, **vectors):
+    for name, v in vectors.items():
+        if v is not None and np.size(v) != n:
+            raise ValueError(f"{who}: {name} has {np.size(v)} values, not {n}")
+
+
 def layernorm_fwd(x, gamma=None, beta=None, eps=1e-5, ctx: Context | None = None):
     """LayerNorm over the last axis of x [..., cols] -> (y, mean, rstd); the
     statistics have x's shape without its last axis."""
+    x, rows, cols = _rows("layernorm_fwd", x)
+    _vectors("layernorm_fwd", cols, gamma=gamma, beta=beta)
     ctx = ctx or Context.shared()
-    x = np.asarray(x, np.float32)
-    cols = x.shape[-1]
-    rows = x.size // cols
     xd = _dev(ctx, x)
     gd = _dev(ctx, gamma) if gamma is not None else None
     bd = _dev(ctx, beta) if beta is not None else None
@@ -174,12 +187,12 @@ def layernorm_bwd(x, dy, gamma=None, eps=1e-5, mean=None, rstd=None, addend=None
                   ctx: Context | None = None):
     """Gradients (dx, dgamma, dbeta) of layernorm_fwd; mean and rstd from the
     forward call, or both None."""
-    ctx = ctx or Context.shared()
-    x = np.asarray(x, np.float32)
-    cols = x.shape[-1]
-    rows = x.size // cols
+    x, rows, cols = _rows("layernorm_bwd", x)
+    _vectors("layernorm_bwd", cols, gamma=gamma)
+    _vectors("layernorm_bwd", rows, mean=mean, rstd=rstd)
     if np.shape(dy) != x.shape or (addend is not None and np.shape(addend) != x.shape):
         raise ValueError(f"layernorm_bwd: dy and addend must have x's shape {x.shape}")
+    ctx = ctx or Context.shared()
     xd, dyd = _dev(ctx, x), _dev(ctx, dy)
     gd, md, rd, ad = (_dev(ctx, a) if a is not None else None
                       for a in (gamma, mean, rstd, addend))
@@ -199,10 +212,17 @@ def _coeffs(coeffs, steps):
     return (C.c_float * a.size)(*a.tolist())
 
 
+def _matrices(who, arrays):
+    shapes = [np.shape(m) for m in arrays]
+    if any(len(s) != 2 for s in shapes):
+        raise ValueError(f"{who}: shapes {shapes} are not all of two axes")
+    return shapes
+
+
 def newton_schulz(matrices, steps=5, coeffs=None, eps=1e-7, ctx: Context | None = None):
     """Newton-Schulz orthogonalisation of each 2-D array -> list of arrays."""
+    shapes = _matrices("newton_schulz", matrices)
     ctx = ctx or Context.shared()
-    shapes = [np.shape(m) for m in matrices]
     xd = [_dev(ctx, m) for m in matrices]
     yd = [_out(ctx, r * c) for r, c in shapes]
     table = (NsMatrix * len(shapes))(*[NsMatrix(x.ptr, y.ptr, r, c, c, c)
@@ -215,7 +235,7 @@ def newton_schulz(matrices, steps=5, coeffs=None, eps=1e-7, ctx: Context | None 
 def muon_scale(rows: int, cols: int) -> float:
     """sqrt(max(1, rows / cols)): a factor on lr that gives the update of a tall
     matrix the root-mean-square gain of a square one's."""
-    return float(max(1.0, rows / cols) ** 0.5)
+    return float(max(1.0, rows / max(cols, 1)) ** 0.5)
 
 
 def muon_multi(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0,
@@ -223,11 +243,13 @@ def muon_multi(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
                scales=None, ctx: Context | None = None):
     """Runs one Muon step on 2-D arrays; returns (params, momenta, norm) as numpy.
     scales: each matrix's factor on lr (None: muon_scale of its shape)."""
-    ctx = ctx or Context.shared()
-    shapes = [np.shape(p) for p in params]
+    shapes = _matrices("muon_multi", params)
     for group in (grads, momenta):
         if [np.shape(a) for a in group] != shapes:
             raise ValueError("muon_multi: gradients and momenta must have the parameters' shapes")
+    if scales is not None and len(scales) != len(shapes):
+        raise ValueError(f"muon_multi: {len(scales)} scales for {len(shapes)} matrices")
+    ctx = ctx or Context.shared()
     pd, gd, md = ([_dev(ctx, a) for a in group] for group in (params, grads, momenta))
     scales = [muon_scale(*s) for s in shapes] if scales is None else scales
     table = (MuonTensor * len(shapes))(*[
