@@ -25,3 +25,17 @@ def test_warmup_ramps_muon_rates_too():
     dv.run_training(tr, _batch, epochs=1, epoch_steps=3, warmup_steps=2)
     np.testing.assert_allclose(tr.muon_rates, [(0.01, 0.02), (0.02, 0.04), (0.02, 0.04)])
     assert tr.muon["lr_vae"] == 0.02
+
+
+def test_checkpoints_during_warmup_keep_the_full_muon_rates():
+    class WithMuon(FakeTrainer):
+        muon = dict(lr_vae=0.02, lr_motion=0.04)
+
+        def set_muon(self, **kw):
+            self.muon = kw
+
+    tr, saved = WithMuon([[1.0, 0.5]] * 4), []
+    dv.run_training(tr, _batch, epochs=2, epoch_steps=2, warmup_steps=8, save_every=1,
+                    save=lambda *at: saved.append((at, dict(tr.muon))))
+    assert [at for at, _ in saved] == [(0, 1), (1, 0), (1, 1), (2, 0)]
+    assert all(m == dict(lr_vae=0.02, lr_motion=0.04) for _, m in saved)

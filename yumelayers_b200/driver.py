@@ -102,8 +102,9 @@ def run_training(trainer, next_batch, *, epochs: int, epoch_steps: int, start_ep
     save(epoch_next, step_in_epoch) writes a checkpoint (every `save_every`
     steps and after each completed epoch); it is never called after a NaN.
     warmup_steps > 0 ramps all learning rates, Muon's among them, over the first
-    steps of this run (for resumes without optimizer state).  Cancel is checked before every
-    step; a stopped epoch is neither reported nor checkpointed.
+    steps of this run (for resumes without optimizer state); checkpoints see the
+    full rates.  Cancel is checked before every step; a stopped epoch is neither
+    reported nor checkpointed.
     """
     control = control or TrainingControl()
     res = RunResult()
@@ -115,6 +116,11 @@ def run_training(trainer, next_batch, *, epochs: int, epoch_steps: int, start_ep
         if muon:
             trainer.set_muon(**{**muon, "lr_vae": muon["lr_vae"] * f,
                                 "lr_motion": muon["lr_motion"] * f})
+
+    def checkpoint(*at):
+        if warmup_steps > 0:
+            set_rates(1.0)  # a checkpoint keeps Muon's rates
+        save(*at)
 
     run_step = 0
     for ep in range(max(0, start_epoch), epochs):
@@ -145,7 +151,7 @@ def run_training(trainer, next_batch, *, epochs: int, epoch_steps: int, start_ep
             if on_progress:
                 on_progress(ep, si, [float(v) for v in losses], time.perf_counter() - t0)
             if save and save_every > 0 and (si + 1) % save_every == 0 and si + 1 < epoch_steps:
-                save(ep, si + 1)
+                checkpoint(ep, si + 1)
         if stopped:
             res.stopped = True
             break
@@ -154,7 +160,7 @@ def run_training(trainer, next_batch, *, epochs: int, epoch_steps: int, start_ep
         if not res.plateau and plateau_detected([l[0] + l[1] for l in res.epoch_losses]):
             res.plateau = True
         if save:
-            save(ep + 1, 0)
+            checkpoint(ep + 1, 0)
     if warmup_steps > 0:
         set_rates(1.0)
     return res
