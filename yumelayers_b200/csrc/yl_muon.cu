@@ -63,6 +63,7 @@ struct Item {
   int chunks;
   int chunk;            // elements of one partial
   int vec;              // 16-byte loads of src and mom: 1 everywhere
+  int narrow;           // tiles of 64 columns, not 128
   int ks;               // GRAM: shares of the long side, each a ticket of its own
   int split0;           // its first arrival counter
   float* partial;       // [GRAM tile][share][column][row] sums of the shares
@@ -367,7 +368,10 @@ __global__ void __launch_bounds__(256)
 // Two forms.  A single block works on 128 x 128 tiles; its MMAs are bound by their
 // reads of shared memory (12 of 128 x 128 a k-block, 8 KB each, take 117 cycles
 // each, not 64), so the left hi plane meets both right planes in one of 256 columns
-// (12 KB).  A pair
+// (12 KB).  With the copies' writes (64 KB) that is 144 KB of a k-block through shared
+// memory, at 128 bytes a cycle its 1.1k cycles.  Tiles of 64 columns (`narrow`) move
+// 104 KB and take 0.8k: more per product, but twice the tiles, each sooner done,
+// where SMs are idle.  A pair
 // of blocks (PAIR: a cluster of two, cta_group::2) works on 256 x 256 tiles, each
 // block with half of the rows of both sides: the same 8 KB of reads for four
 // times the products, 128 cycles per block, bound by the tensor cores.
@@ -412,7 +416,7 @@ struct Ticket {
 constexpr int kTicketInts = sizeof(Ticket) / 4, kNoTicket = -1;  // mode behind the last one
 
 // `start` is the table's tiles[3][kMaxItems + 1] in shared memory.
-template <bool PAIR>
+template <bool PAIR, bool NARROW>
 __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, int count, int n) {
   Ticket q;
   const int gram = start[count], square = start[kMaxItems + 1 + count];
@@ -435,8 +439,9 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
   q.kb0 = 0;
   q.share = 0;
   q.nk = it.mb;
+  const bool narrow = NARROW && it.narrow;
   if (q.mode == UPDATE) {
-    const int tn = (it.cb + Form<PAIR>::kSide - 1) / Form<PAIR>::kSide;
+    const int tn = narrow ? it.cb : (it.cb + Form<PAIR>::kSide - 1) / Form<PAIR>::kSide;
     q.i = k / tn;
     q.j = k - q.i * tn;
     q.tile = k;
@@ -450,6 +455,14 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
     q.nk = (int)((long long)nk * (q.share + 1) / ks) - q.kb0;
   }
   q.tile = k;
+  if (narrow) {  // lower triangle, row by row, 2 i + 2 tiles in row i: k = i (i + 1) + j
+    int i = (int)((sqrtf(4.f * k + 1.f) - 1.f) * 0.5f);
+    while (i * (i + 1) > k) --i;
+    while ((i + 1) * (i + 2) <= k) ++i;
+    q.i = i;
+    q.j = k - i * (i + 1);
+    return q;
+  }
   // lower triangle, row by row: k = i (i + 1) / 2 + j
   int i = (int)((sqrtf(8.f * k + 1.f) - 1.f) * 0.5f);
   while (i * (i + 1) / 2 > k) --i;
@@ -459,13 +472,20 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
   return q;
 }
 
+// The row of tiles that a ticket's columns are.
+template <bool NARROW>
+__device__ __forceinline__ int column_tile(const Item& it, const Ticket& q) {
+  return NARROW && it.narrow ? q.j >> 1 : q.j;
+}
+
 // Whether k-block kb of a ticket meets the diagonal of A or P.
-template <bool PAIR>
+template <bool PAIR, bool NARROW>
 __device__ __forceinline__ bool on_diagonal(const Item& it, const Ticket& q, int kb) {
   const int kt = kb / Form<PAIR>::kSide;
   if (q.mode == GRAM) return false;
-  if (q.mode == SQUARE) return kt == q.i || kt == q.j;
-  return kt == (it.rows > it.cols ? q.j : q.i);
+  const int jt = column_tile<NARROW>(it, q);
+  if (q.mode == SQUARE) return kt == q.i || kt == jt;
+  return kt == (it.rows > it.cols ? jt : q.i);
 }
 
 // One operand: block (mn, k) of a plane is at base + (mn * smn + k * sk) blocks.
@@ -521,7 +541,8 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, long long l
   return PAIR ? mbar_wait_cluster(bar, parity, lim) : mbar_wait(bar, parity, lim);
 }
 
-template <bool PAIR>
+// NARROW: some of the table's matrices are.
+template <bool PAIR, bool NARROW>
 __global__ void __launch_bounds__(kProductThreads, 1)
     ns_steps_kernel(const Table* __restrict__ t, const __grid_constant__ Steps steps,
                     const __grid_constant__ Update u, int* err) {
@@ -613,7 +634,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
           const int n = atomicAdd(t->ctrl, 1);
           q.mode = kNoTicket;
-          if (n < total) q = ticket_of<PAIR>(t, start, count, n);
+          if (n < total) q = ticket_of<PAIR, NARROW>(t, start, count, n);
           ring[slot] = q;
           mbar_arrive(&tfull[slot]);
           if (PAIR) {
@@ -659,9 +680,12 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         if (q.mode == kNoTicket) break;
         const Item& im = t->it[q.item];
         const Operand L = operand(im, q.mode, q.step & 1, 0), R = operand(im, q.mode, q.step & 1, 1);
-        const bool same = q.mode != UPDATE && q.i == q.j;
-        const int l0 = F::kSide * q.i + 2 * rank, r0 = F::kSide * q.j + 2 * rank;
-        const int nl = max(0, min(2, L.nmn - l0)), nr = same ? 0 : max(0, min(2, R.nmn - r0));
+        const bool narrow = NARROW && im.narrow;
+        const bool same = !narrow && q.mode != UPDATE && q.i == q.j;
+        const int l0 = F::kSide * q.i + 2 * rank, r0 = narrow ? q.j : F::kSide * q.j + 2 * rank;
+        const int nl = max(0, min(2, L.nmn - l0));
+        const int nr = same ? 0 : max(0, min(narrow ? 1 : 2, R.nmn - r0));
+        const int jt = column_tile<NARROW>(im, q);
         if (!mbar_wait(&ready[slot], (k / kRing) & 1, lim)) {
           report_error(err, YL_DEVERR_TIMEOUT);
           break;
@@ -679,7 +703,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
           const uint32_t dst = smem_u32(smem + s * kStageBytes);
           if (kb >= q.nk) {  // 128 rows x 128 columns of A for the epilogue, blocks [row][column]
-            const int c0 = F::kSide * q.j + 2 * (kb - q.nk), nc = max(0, min(2, im.mb - c0));
+            const int c0 = narrow ? q.j : F::kSide * q.j + 2 * (kb - q.nk);
+            const int nc = max(0, min(narrow ? 1 : 2, im.mb - c0));
             mbar_arrive_expect_tx(&full[s], (uint32_t)(2 * nl * nc) * kBlkBytes);
             for (int b = 0; b < nl * nc; ++b) {
               const int br = b / nc, bc = b - br * nc;
@@ -695,13 +720,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           for (int side = 0; side < 2; ++side) {
             const Operand& o = side ? R : L;
             const int nb = side ? nr : nl, mn0 = side ? r0 : l0;
-            const bool above = o.sym && (side ? q.j : q.i) < kk / F::kSide;
+            const bool above = o.sym && (side ? jt : q.i) < kk / F::kSide;
+            const uint32_t lo = side && narrow ? kBlkBytes : kOpBytes;  // its lo plane
             const size_t smn = above ? o.sk : o.smn, sk = above ? o.smn : o.sk;
             for (int b = 0; b < nb; ++b) {
               const uint8_t* src = o.base + ((size_t)(mn0 + b) * smn + (size_t)kk * sk) * kBlkBytes;
               const uint32_t d = dst + (uint32_t)(side * 2 * kOpBytes + b * kBlkBytes);
               bulk_load(d, src, kBlkBytes, &full[s]);
-              bulk_load(d + kOpBytes, src + o.plane, kBlkBytes, &full[s]);
+              bulk_load(d + lo, src + o.plane, kBlkBytes, &full[s]);
             }
           }
         }
@@ -736,7 +762,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         const Item& im = t->it[q.item];
         const Operand L = operand(im, q.mode, 0, 0), R = operand(im, q.mode, 0, 1);
-        const bool same = q.mode != UPDATE && q.i == q.j;
+        const bool narrow = NARROW && im.narrow;
+        const bool same = !narrow && q.mode != UPDATE && q.i == q.j;
+        const int jt = column_tile<NARROW>(im, q);
         int filled = 0;  // k-blocks the current accumulator has taken
         for (int kb = 0; ok && kb < q.nk; ++kb, ++it) {
           const int s = it % kStages;
@@ -747,14 +775,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             break;
           }
           const int kt = (q.kb0 + kb) / F::kSide;
-          const int lmn = L.mn_major | (L.sym & (q.i < kt)), rmn = R.mn_major | (R.sym & (q.j < kt));
-          const uint32_t idesc = idesc_f16(F::kTile, F::kTile, lmn, rmn);
+          const int lmn = L.mn_major | (L.sym & (q.i < kt)), rmn = R.mn_major | (R.sym & (jt < kt));
+          const int cols = narrow ? 64 : F::kTile;
+          const uint32_t idesc = idesc_f16(F::kTile, cols, lmn, rmn);
           // K-major: 16 of a row's 64 k are 32 bytes, 8-row groups 1 KB apart.
           // MN-major: 16 k are two 8-row groups, 64-column blocks 8 KB apart.
           const uint32_t lstep = lmn ? 2048 : 32, rstep = rmn ? 2048 : 32;
           const uint32_t llbo = lmn ? kBlkBytes : 16, rlbo = rmn ? kBlkBytes : 16;
           const uint32_t l = smem_u32(smem + s * kStageBytes), r = same ? l : l + 2 * kOpBytes;
-          const bool fine = on_diagonal<PAIR>(im, q, kb);
+          const bool fine = on_diagonal<PAIR, NARROW>(im, q, kb);
           const int buf = ci % kAccs;
           if (filled == 0 && ci >= kAccs && !wait<PAIR>(&acc_empty[buf], (ci / kAccs - 1) & 1, lim)) {
             report_error(err, YL_DEVERR_TIMEOUT);
@@ -776,18 +805,18 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             }
           } else {
             // both planes of the right side lie one behind the other: hi (hi | lo) is
-            // one product of 256 columns, lo hi goes to the second half of them
-            const uint32_t wide = idesc_f16(128, 256, lmn, rmn);
+            // one product of twice the columns, lo hi goes to the second half of them
+            const uint32_t wide = idesc_f16(128, 2 * cols, lmn, rmn);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               umma_f16(dacc, sw128_desc(l + kk * lstep, llbo, 1024),
                        sw128_desc(r + kk * rstep, rlbo, 1024), wide, (filled | kk) != 0);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_f16(dacc + 128, sw128_desc(l + kOpBytes + kk * lstep, llbo, 1024),
+              umma_f16(dacc + cols, sw128_desc(l + kOpBytes + kk * lstep, llbo, 1024),
                        sw128_desc(r + kk * rstep, rlbo, 1024), idesc, 1);
           }
-          if (++filled == 2 || fine || kb + 1 == q.nk || on_diagonal<PAIR>(im, q, kb + 1)) {
+          if (++filled == 2 || fine || kb + 1 == q.nk || on_diagonal<PAIR, NARROW>(im, q, kb + 1)) {
             if (PAIR) umma_commit_pair(&acc_full[buf]);
             else umma_commit(&acc_full[buf]);
             filled = 0;
@@ -836,12 +865,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       if (lane == 0) arrive0(&tempty[slot]);
       if (q.mode == kNoTicket) break;
       const Item& im = t->it[q.item];
+      const bool narrow = NARROW && im.narrow;
+      const bool idle = narrow && wc != 0;  // 64 columns: the first four warps' alone
       if (u.muon && q.mode == UPDATE && q.step + 1 == steps.n) {
         // the parameter's rows towards L2 while the products run: a row of this
         // warp's columns per lane
         const long long r = (long long)(F::kSide * q.i + 2 * rank) * kBlk + wr * 32 + lane;
-        const int c0 = (F::kSide * q.j) * kBlk + wc * kCols, c1 = min(c0 + kCols, im.cols);
-        if (r < im.rows)
+        const int c0 = narrow ? q.j * kBlk : F::kSide * q.j * kBlk + wc * kCols;
+        const int c1 = min(c0 + kCols, im.cols);
+        if (r < im.rows && !idle)
           for (int c = c0; c < c1; c += 32) prefetch_l2(im.dst + r * im.ldd + c);
       }
       float v[kCols];
@@ -850,8 +882,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       bool ok = true;
       // the accumulators of the ticket, as the MMA thread fills them
       for (int kb = 0; kb < q.nk; ++ci) {
-        const bool fine = on_diagonal<PAIR>(im, q, kb++);
-        if (!fine && kb < q.nk && !on_diagonal<PAIR>(im, q, kb)) ++kb;
+        const bool fine = on_diagonal<PAIR, NARROW>(im, q, kb++);
+        if (!fine && kb < q.nk && !on_diagonal<PAIR, NARROW>(im, q, kb)) ++kb;
         const int buf = ci % kAccs;
         if (!wait<PAIR>(&acc_full[buf], (ci / kAccs) & 1, lim)) {
           report_error(err, YL_DEVERR_TIMEOUT);
@@ -864,16 +896,19 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         // 16 columns at a time (without PAIR those of hi hi, then those of the small
         // terms): the next read runs while this one is added
         constexpr int kReads = 128 / 16;
-        auto col = [](int p) { return PAIR ? p * 16 : (p >> 2) * 128 + (p & 3) * 16; };
-        uint32_t acc[2][16];
-        tmem_ld_32x32b_x16(at, acc[0]);
+        const int small = narrow ? 64 : 128;
+        auto col = [&](int p) { return PAIR ? p * 16 : (p >> 2) * small + (p & 3) * 16; };
+        if (!idle) {
+          uint32_t acc[2][16];
+          tmem_ld_32x32b_x16(at, acc[0]);
 #pragma unroll
-        for (int p = 0; p < kReads; ++p) {
-          tmem_ld_wait();
-          if (p + 1 < kReads) tmem_ld_32x32b_x16(at + col(p + 1), acc[(p + 1) & 1]);
+          for (int p = 0; p < kReads; ++p) {
+            tmem_ld_wait();
+            if (p + 1 < kReads) tmem_ld_32x32b_x16(at + col(p + 1), acc[(p + 1) & 1]);
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
-            v[(PAIR ? p : p & 3) * 16 + c] += __uint_as_float(acc[p & 1][c]);
+            for (int c = 0; c < 16; ++c)
+              v[(PAIR ? p : p & 3) * 16 + c] += __uint_as_float(acc[p & 1][c]);
+          }
         }
         tc_fence_before();
         __syncwarp();
@@ -884,12 +919,15 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       if (q.mode == GRAM && im.ks > 1) {
         // leave this share's sum; the block that finishes a tile's last share adds
         // them all, in share order whoever that is
-        constexpr size_t kSlice = (size_t)F::kTile * 128;  // one block's part of a tile
+        // one block's part of a tile
+        const size_t slice = (size_t)128 * (narrow ? 64 : F::kTile);
         const size_t slot0 = ((size_t)q.tile * F::kCtas + rank) * im.ks;
-        float* part = im.partial + slot0 * kSlice + (size_t)(wc * kCols) * 128 + wr * 32 + lane;
-        float* mine = part + (size_t)q.share * kSlice;
+        float* part = im.partial + slot0 * slice + (size_t)(wc * kCols) * 128 + wr * 32 + lane;
+        float* mine = part + (size_t)q.share * slice;
+        if (!idle) {
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) __stcg(mine + c * 128, v[c]);
+          for (int c = 0; c < kCols; ++c) __stcg(mine + c * 128, v[c]);
+        }
         if (!together()) break;
         if (threadIdx.x == 0) {
           __threadfence();  // with the barrier: all of the block's stores
@@ -903,8 +941,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         if (!mine_is_last) continue;  // thread 0 writes the flag again only behind a barrier
 #pragma unroll
         for (int c = 0; c < kCols; ++c) v[c] = 0.f;
-        for (int sh = 0; sh < im.ks; ++sh) {
-          const float* p = part + (size_t)sh * kSlice;
+        for (int sh = 0; sh < (idle ? 0 : im.ks); ++sh) {
+          const float* p = part + (size_t)sh * slice;
 #pragma unroll
           for (int c = 0; c < kCols; ++c) v[c] += __ldcg(p + c * 128);
         }
@@ -929,8 +967,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       }
 #pragma unroll
       for (int slab = 0; slab < kCols / 64; ++slab) {
-        const int cblk = F::kSide * q.j + wc * (kCols / 64) + slab;
-        if (rblk >= rbt || cblk >= cbt) continue;  // uniform in the warp
+        const int cblk = narrow ? q.j : F::kSide * q.j + wc * (kCols / 64) + slab;
+        if (idle || rblk >= rbt || cblk >= cbt) continue;  // uniform in the warp
         float* w = v + slab * 64;
 #pragma unroll
         for (int c = 0; c < 64; ++c) w[c] *= c2;
@@ -1511,6 +1549,45 @@ __global__ void __launch_bounds__(kChipThreads, 1)
 }
 
 // ---------------------------------------------------------------- host side
+long long update_tiles(const Item& it, int side_rows, int side_cols) {
+  const long long rb = (it.rows + kBlk - 1) / kBlk, cb = (it.cols + kBlk - 1) / kBlk;
+  return (rb + side_rows - 1) / side_rows * ((cb + side_cols - 1) / side_cols);
+}
+// Tiles of a matrix on and below the diagonal.
+int lower_tiles(const Item& it, int side) {
+  const int mt = (it.mb + side - 1) / side;
+  return it.narrow ? mt * (mt + 1) - (it.mb & 1) : mt * (mt + 1) / 2;
+}
+
+// 64-deep k-blocks of a tile's sum in SQUARE and UPDATE.
+int k_blocks(const Item& it) { return (std::min(it.rows, it.cols) + kBlk - 1) / kBlk; }
+// Time of a tile in us: 0.43 a k-block at 64 columns, 0.6 at 128, and 4.5 besides.
+double tile_time(const Item& it, bool narrow) { return 4.5 + (narrow ? 0.43 : 0.6) * k_blocks(it); }
+// That of all tiles of an UPDATE.
+double tiles_time(const Item& it, bool narrow) {
+  return tile_time(it, narrow) * update_tiles(it, 2, narrow ? 1 : 2);
+}
+
+// Tiles of 64 columns for the table's first matrices (those with the most
+// k-blocks), as far as the longest product of a phase gets shorter and the SMs
+// still hold them all (512 x 512 166 -> 146 us, 1024 x 1024 238 -> 219 us).
+void choose_narrow(Table* t, int num_sms) {
+  for (int k = 0; k < t->count; ++k) t->it[k].narrow = 0;
+  if (t->pair || t->chip) return;
+  double all = 0;
+  for (int k = 0; k < t->count; ++k) all += tiles_time(t->it[k], false);
+  double best = std::max(tile_time(t->it[0], false), all / num_sms);
+  int chosen = 0;
+  for (int n = 1; n <= t->count; ++n) {
+    all += tiles_time(t->it[n - 1], true) - tiles_time(t->it[n - 1], false);
+    const double longest =
+        std::max(tile_time(t->it[0], true), n < t->count ? tile_time(t->it[n], false) : 0.0);
+    const double now = std::max(longest, all / num_sms);
+    if (now < best) best = now, chosen = n;
+  }
+  for (int n = 0; n < chosen; ++n) t->it[n].narrow = 1;
+}
+
 // Sizes the table's workspace, or (with a base address) places it; returns the
 // bytes it takes.
 size_t place(Table* t, int num_sms, char* ws) {
@@ -1545,10 +1622,7 @@ size_t place(Table* t, int num_sms, char* ws) {
   // more for each share that the last block reads.
   auto nk = [](const Item& it) { return std::max(it.rb, it.cb); };
   const int ctas = t->pair ? 2 : 1, workers = num_sms / ctas;
-  auto gram_tiles = [&](const Item& it) {
-    const int mt = (it.mb + 2 * ctas - 1) / (2 * ctas);
-    return mt * (mt + 1) / 2;
-  };
+  auto gram_tiles = [&](const Item& it) { return lower_tiles(it, 2 * ctas); };
   double kb = 0;
   for (int k = 0; k < t->count; ++k) kb += (double)gram_tiles(t->it[k]) * nk(t->it[k]);
   const double fair = kb / workers;
@@ -1556,10 +1630,11 @@ size_t place(Table* t, int num_sms, char* ws) {
   for (int k = 0; k < t->count; ++k) {
     Item& it = t->it[k];
     const int most = (int)std::round(nk(it) / std::max(fair, 1.0));
-    double best = 1.1 * nk(it);
+    const double block = it.narrow ? 0.8 : 1.1;
+    double best = block * nk(it);
     it.ks = 1;
     for (int ks = 2; ks <= std::min(most, nk(it)); ++ks) {
-      const double cost = 1.1 * nk(it) / ks + 5 + 1.2 * ks;
+      const double cost = block * nk(it) / ks + 5 + 1.2 * ks;
       if (cost < best) {
         best = cost;
         it.ks = ks;
@@ -1652,15 +1727,15 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   if (t.chip) return run_chip(ctx, t, u, s);
   place(&t, ctx->num_sms, ws);
   const int ctas = t.pair ? 2 : 1, side = 2 * ctas;
-  auto tiles = [&](int v) { return (v + side - 1) / side; };
   for (int m = 0; m < 3; ++m) t.tiles[m][0] = 0;
   t.blocks[0] = t.chunks[0] = 0;
   for (int k = 0; k < t.count; ++k) {
     const Item& it = t.it[k];
-    const int mt = tiles(it.mb);
-    t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + mt * (mt + 1) / 2 * it.ks;
-    t.tiles[SQUARE][k + 1] = t.tiles[SQUARE][k] + mt * (mt + 1) / 2;
-    t.tiles[UPDATE][k + 1] = t.tiles[UPDATE][k] + tiles(it.rb) * tiles(it.cb);
+    const int lower = lower_tiles(it, side);
+    t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + lower * it.ks;
+    t.tiles[SQUARE][k + 1] = t.tiles[SQUARE][k] + lower;
+    t.tiles[UPDATE][k + 1] =
+        t.tiles[UPDATE][k] + (int)update_tiles(it, side, it.narrow ? 1 : side);
     t.blocks[k + 1] = t.blocks[k] + it.rb * it.cb;
     t.chunks[k + 1] = t.chunks[k] + it.chunks;
   }
@@ -1691,7 +1766,11 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cfg.attrs = &cluster;
   cfg.numAttrs = t.pair ? 1 : 0;
-  auto kernel = t.pair ? ns_steps_kernel<true> : ns_steps_kernel<false>;
+  bool narrow = false;
+  for (int k = 0; k < t.count; ++k) narrow |= t.it[k].narrow != 0;
+  auto kernel = t.pair   ? ns_steps_kernel<true, false>
+                : narrow ? ns_steps_kernel<false, true>
+                         : ns_steps_kernel<false, false>;
   YL_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
   YL_CUDA(cudaLaunchKernelEx(&cfg, kernel, (const Table*)dt, st, u, ctx->dev_err));
   return check_launch("ns_steps_kernel");
@@ -1718,6 +1797,22 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn 
   const bool chip = steps > 0 && std::all_of(items.begin(), items.end(), on_chip) &&
                     (long long)items.size() * least_share(items.data(), (int)items.size()) <=
                         ctx->num_sms;
+  // Where the tiles of a phase nearly all find an SM at once, the longest chains of
+  // products come first: what has to wait is then short (five odd shapes 245 -> 233
+  // us).  Longer tables keep the caller's order (the U-Net's 39 matrices 436 us,
+  // sorted 446).
+  std::vector<const Item*> order;
+  double all = 0, longest = 0;
+  for (const Item& it : items) {
+    order.push_back(&it);
+    all += tiles_time(it, false);
+    longest = std::max(longest, tile_time(it, false));
+  }
+  if (all <= longest * ctx->num_sms)
+    std::sort(order.begin(), order.end(), [](const Item* x, const Item* y) {
+      const int sx = k_blocks(*x), sy = k_blocks(*y);
+      return sx != sy ? sx > sy : x < y;
+    });
   auto t = std::make_unique<Table>();
   t->chip = chip;
   for (int pair = 1; pair >= 0; --pair) {
@@ -1725,11 +1820,12 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn 
     t->pair = pair;
     for (size_t k = 0; k <= items.size(); ++k) {
       if (t->count == kMaxItems || (k == items.size() && t->count > 0)) {
+        choose_narrow(t.get(), ctx->num_sms);
         YL_TRY(fn(*t));
         t->count = 0;
       }
-      if (k < items.size() && (pairs && wide(items[k])) == (pair != 0))
-        t->it[t->count++] = items[k];
+      if (k < items.size() && (pairs && wide(*order[k])) == (pair != 0))
+        t->it[t->count++] = *order[k];
     }
   }
   return YL_OK;
