@@ -87,17 +87,17 @@ def test_one_matrix(h, r, c):
     assert rel(got, ns64(x)) < (TOL if max(r, c) > 1.2 * min(r, c) or min(r, c) == 1 else TOL_SPREAD)
 
 
-@pytest.mark.parametrize("shapes", [[(4000, 3900)], [(900, 4097), (64, 700)] + [(1030, 1000)] * 14])
-def test_enough_tiles_for_pairs_of_blocks(h, shapes):
-    """Sizes that run on 256 x 256 tiles, against float64 on the device."""
+def check_on_device(h, shapes):
+    """Normal matrices, two equal calls, against float64 on the device."""
     gen = torch.Generator(device="cuda").manual_seed(5)
     xs = [torch.randn(s, generator=gen, device="cuda") for s in shapes]
-    ys = [torch.empty_like(x) for x in xs]
-    table = (NsMatrix * len(xs))(*[
-        NsMatrix(x.data_ptr(), y.data_ptr(), *x.shape, x.shape[1], x.shape[1])
-        for x, y in zip(xs, ys)])
-    call("yl_newton_schulz", h, table, len(xs), 5, None, 1e-7)
-    for x, y in zip(xs, ys):
+    ys, again = [torch.empty_like(x) for x in xs], [torch.empty_like(x) for x in xs]
+    for out in (ys, again):
+        table = (NsMatrix * len(xs))(*[
+            NsMatrix(x.data_ptr(), y.data_ptr(), *x.shape, x.shape[1], x.shape[1])
+            for x, y in zip(xs, out)])
+        call("yl_newton_schulz", h, table, len(xs), 5, None, 1e-7)
+    for x, y, y2 in zip(xs, ys, again):
         z = x.double() if x.shape[0] <= x.shape[1] else x.double().T
         z = z / (z.square().sum().sqrt() + 1e-7)
         for _ in range(5):
@@ -105,6 +105,28 @@ def test_enough_tiles_for_pairs_of_blocks(h, shapes):
             z = QUINTIC[0] * z + QUINTIC[1] * (g @ z) + QUINTIC[2] * (g @ (g @ z))
         z = z if x.shape[0] <= x.shape[1] else z.T
         assert float((y.double() - z).norm() / z.norm()) < TOL
+        assert torch.equal(y, y2)
+
+
+@pytest.mark.parametrize("shapes", [[(4000, 3900)], [(900, 4097), (64, 700)] + [(1030, 1000)] * 14])
+def test_enough_tiles_for_pairs_of_blocks(h, shapes):
+    """Sizes that run on 256 x 256 tiles."""
+    check_on_device(h, shapes)
+
+
+@pytest.mark.parametrize("shapes", [
+    [(1500, 1200)], [(1200, 1501)], [(257, 20000)], [(20000, 200)], [(150, 700)] * 70])
+def test_tiles_of_128_columns(h, shapes):
+    """More tiles of a phase than SMs, in the caller's order; with shares of a long side."""
+    check_on_device(h, shapes)
+
+
+@pytest.mark.parametrize("shapes", [
+    [(333, 2500)], [(2500, 333)], [(997, 700)], [(576, 700)], [(129, 1024), (300, 3000), (640, 900), (1024, 130)]])
+def test_tiles_of_64_columns(h, shapes):
+    """Fewer tiles than SMs, odd and even numbers of blocks; the last table has tiles of
+    both widths."""
+    check_on_device(h, shapes)
 
 
 def test_singular_values_end_near_one(h):
