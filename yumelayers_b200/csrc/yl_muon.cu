@@ -63,13 +63,14 @@ struct Item {
   int chunks;
   int chunk;            // elements of one partial
   int vec;              // 16-byte loads of src and mom: 1 everywhere
-  int narrow;           // tiles of 64 columns, not 128
+  int narrow;           // bit of a phase: its tiles have 64 columns, not 128
   int ks;               // GRAM: shares of the long side, each a ticket of its own
   int split0;           // its first arrival counter
   float* partial;       // [GRAM tile][share][column][row] sums of the shares
 };
 enum { GRAM = 0, SQUARE = 1, UPDATE = 2 };
 constexpr int kPairSide = 512;
+constexpr int kMaxShares = 64;
 struct Table {
   Item it[kMaxItems];
   int tiles[3][kMaxItems + 1];  // GRAM, SQUARE, UPDATE tickets before each item
@@ -439,7 +440,7 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
   q.kb0 = 0;
   q.share = 0;
   q.nk = it.mb;
-  const bool narrow = NARROW && it.narrow;
+  const bool narrow = NARROW && (it.narrow >> q.mode & 1);
   if (q.mode == UPDATE) {
     const int tn = narrow ? it.cb : (it.cb + Form<PAIR>::kSide - 1) / Form<PAIR>::kSide;
     q.i = k / tn;
@@ -475,7 +476,7 @@ __device__ __forceinline__ Ticket ticket_of(const Table* t, const int* start, in
 // The row of tiles that a ticket's columns are.
 template <bool NARROW>
 __device__ __forceinline__ int column_tile(const Item& it, const Ticket& q) {
-  return NARROW && it.narrow ? q.j >> 1 : q.j;
+  return NARROW && (it.narrow >> q.mode & 1) ? q.j >> 1 : q.j;
 }
 
 // Whether k-block kb of a ticket meets the diagonal of A or P.
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         if (q.mode == kNoTicket) break;
         const Item& im = t->it[q.item];
         const Operand L = operand(im, q.mode, q.step & 1, 0), R = operand(im, q.mode, q.step & 1, 1);
-        const bool narrow = NARROW && im.narrow;
+        const bool narrow = NARROW && (im.narrow >> q.mode & 1);
         const bool same = !narrow && q.mode != UPDATE && q.i == q.j;
         const int l0 = F::kSide * q.i + 2 * rank, r0 = narrow ? q.j : F::kSide * q.j + 2 * rank;
         const int nl = max(0, min(2, L.nmn - l0));
@@ -762,7 +763,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         const Item& im = t->it[q.item];
         const Operand L = operand(im, q.mode, 0, 0), R = operand(im, q.mode, 0, 1);
-        const bool narrow = NARROW && im.narrow;
+        const bool narrow = NARROW && (im.narrow >> q.mode & 1);
         const bool same = !narrow && q.mode != UPDATE && q.i == q.j;
         const int jt = column_tile<NARROW>(im, q);
         int filled = 0;  // k-blocks the current accumulator has taken
@@ -865,7 +866,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       if (lane == 0) arrive0(&tempty[slot]);
       if (q.mode == kNoTicket) break;
       const Item& im = t->it[q.item];
-      const bool narrow = NARROW && im.narrow;
+      const bool narrow = NARROW && (im.narrow >> q.mode & 1);
       const bool idle = narrow && wc != 0;  // 64 columns: the first four warps' alone
       if (u.muon && q.mode == UPDATE && q.step + 1 == steps.n) {
         // the parameter's rows towards L2 while the products run: a row of this
@@ -1553,39 +1554,75 @@ long long update_tiles(const Item& it, int side_rows, int side_cols) {
   const long long rb = (it.rows + kBlk - 1) / kBlk, cb = (it.cols + kBlk - 1) / kBlk;
   return (rb + side_rows - 1) / side_rows * ((cb + side_cols - 1) / side_cols);
 }
-// Tiles of a matrix on and below the diagonal.
-int lower_tiles(const Item& it, int side) {
-  const int mt = (it.mb + side - 1) / side;
-  return it.narrow ? mt * (mt + 1) - (it.mb & 1) : mt * (mt + 1) / 2;
+// Tiles on and below the diagonal of A and P.
+long long lower_tiles(const Item& it, int side, bool narrow) {
+  const long long mb = (std::min(it.rows, it.cols) + kBlk - 1) / kBlk, mt = (mb + side - 1) / side;
+  return narrow ? mt * (mt + 1) - (mb & 1) : mt * (mt + 1) / 2;
 }
 
 // 64-deep k-blocks of a tile's sum in SQUARE and UPDATE.
 int k_blocks(const Item& it) { return (std::min(it.rows, it.cols) + kBlk - 1) / kBlk; }
-// Time of a tile in us: 0.43 a k-block at 64 columns, 0.6 at 128, and 4.5 besides.
-double tile_time(const Item& it, bool narrow) { return 4.5 + (narrow ? 0.43 : 0.6) * k_blocks(it); }
-// That of all tiles of an UPDATE.
-double tiles_time(const Item& it, bool narrow) {
-  return tile_time(it, narrow) * update_tiles(it, 2, narrow ? 1 : 2);
+// Thousands of cycles for a k-block.
+double block_time(bool narrow) { return narrow ? 0.8 : 1.1; }
+// Shares of GRAM's long side, at most `most`: the number with the shortest way
+// through a tile.  The sums' way through memory takes 5k cycles, and 1.2k more for
+// each share that the last block reads.
+int shares(const Item& it, bool narrow, int most, double* time) {
+  const int nk = (std::max(it.rows, it.cols) + kBlk - 1) / kBlk;
+  int best = 1;
+  *time = block_time(narrow) * nk;
+  for (int ks = 2; ks <= std::min(most, nk); ++ks) {
+    const double cost = block_time(narrow) * nk / ks + 5 + 1.2 * ks;
+    if (cost < *time) *time = cost, best = ks;
+  }
+  return best;
+}
+// Thousands of cycles for a tile of a phase (about 9 beside its products), and the
+// tiles' number.
+double tile_time(const Item& it, int mode, bool narrow, long long* tiles) {
+  if (mode == UPDATE) *tiles = update_tiles(it, 2, narrow ? 1 : 2);
+  else *tiles = lower_tiles(it, 2, narrow);
+  double products = block_time(narrow) * k_blocks(it);
+  if (mode == GRAM) *tiles *= shares(it, narrow, kMaxShares, &products);
+  return 9 + products;
 }
 
-// Tiles of 64 columns for the table's first matrices (those with the most
-// k-blocks), as far as the longest product of a phase gets shorter and the SMs
-// still hold them all (512 x 512 166 -> 146 us, 1024 x 1024 238 -> 219 us).
+// Tiles of 64 columns for a phase's longest products, as far as the longest one
+// gets shorter and the SMs still hold them all (512 x 512 166 -> 146 us, 1024 x 1024
+// 238 -> 219 us; with those of GRAM and SQUARE alone 512 x 4608 221 -> 203 us).  Not
+// where the phases of many matrices overlap and leave no SM idle: the U-Net's table
+// took 460 us so, 451 without.
 void choose_narrow(Table* t, int num_sms) {
   for (int k = 0; k < t->count; ++k) t->it[k].narrow = 0;
   if (t->pair || t->chip) return;
-  double all = 0;
-  for (int k = 0; k < t->count; ++k) all += tiles_time(t->it[k], false);
-  double best = std::max(tile_time(t->it[0], false), all / num_sms);
-  int chosen = 0;
-  for (int n = 1; n <= t->count; ++n) {
-    all += tiles_time(t->it[n - 1], true) - tiles_time(t->it[n - 1], false);
-    const double longest =
-        std::max(tile_time(t->it[0], true), n < t->count ? tile_time(t->it[n], false) : 0.0);
-    const double now = std::max(longest, all / num_sms);
-    if (now < best) best = now, chosen = n;
+  for (int mode = 2; mode >= 0; --mode) {
+    int order[kMaxItems];
+    double time[kMaxItems][2], total[kMaxItems][2], all = 0;
+    for (int k = 0; k < t->count; ++k) {
+      order[k] = k;
+      for (int narrow = 0; narrow < 2; ++narrow) {
+        long long tiles;
+        time[k][narrow] = tile_time(t->it[k], mode, narrow, &tiles);
+        total[k][narrow] = time[k][narrow] * tiles;
+      }
+      all += total[k][0];
+    }
+    std::sort(order, order + t->count, [&](int x, int y) {
+      return time[x][0] != time[y][0] ? time[x][0] > time[y][0] : x < y;
+    });
+    if (mode == UPDATE && t->count > 1 && all > time[order[0]][0] * num_sms) return;
+    double best = std::max(time[order[0]][0], all / num_sms), longest = 0;
+    int chosen = 0;
+    for (int n = 1; n <= t->count; ++n) {
+      const int k = order[n - 1];
+      all += total[k][1] - total[k][0];
+      longest = std::max(longest, time[k][1]);
+      const double rest = n < t->count ? time[order[n]][0] : 0.0;
+      const double now = std::max({longest, rest, all / num_sms});
+      if (now < best) best = now, chosen = n;
+    }
+    for (int n = 0; n < chosen; ++n) t->it[order[n]].narrow |= 1 << mode;
   }
-  for (int n = 0; n < chosen; ++n) t->it[n].narrow = 1;
 }
 
 // Sizes the table's workspace, or (with a base address) places it; returns the
@@ -1617,29 +1654,21 @@ size_t place(Table* t, int num_sms, char* ws) {
     it.part = (double*)take(it.chunks * sizeof(double));
   }
   // Shares of GRAM's long side: at most as many as bring its tickets down to the
-  // average per SM, and of those the number with the shortest way through a tile.
-  // A k-block takes about 1.1k cycles; the sums' way through memory 5k, and 1.2k
-  // more for each share that the last block reads.
+  // average per SM.
   auto nk = [](const Item& it) { return std::max(it.rb, it.cb); };
   const int ctas = t->pair ? 2 : 1, workers = num_sms / ctas;
-  auto gram_tiles = [&](const Item& it) { return lower_tiles(it, 2 * ctas); };
+  auto gram_tiles = [&](const Item& it) {
+    return (int)lower_tiles(it, 2 * ctas, it.narrow >> GRAM & 1);
+  };
   double kb = 0;
   for (int k = 0; k < t->count; ++k) kb += (double)gram_tiles(t->it[k]) * nk(t->it[k]);
   const double fair = kb / workers;
   int splits = 0;
   for (int k = 0; k < t->count; ++k) {
     Item& it = t->it[k];
-    const int most = (int)std::round(nk(it) / std::max(fair, 1.0));
-    const double block = it.narrow ? 0.8 : 1.1;
-    double best = block * nk(it);
-    it.ks = 1;
-    for (int ks = 2; ks <= std::min(most, nk(it)); ++ks) {
-      const double cost = block * nk(it) / ks + 5 + 1.2 * ks;
-      if (cost < best) {
-        best = cost;
-        it.ks = ks;
-      }
-    }
+    double time;
+    it.ks = shares(it, it.narrow >> GRAM & 1,
+                   (int)std::min(std::round(nk(it) / std::max(fair, 1.0)), (double)kMaxShares), &time);
     it.split0 = splits;
     it.partial = nullptr;
     if (it.ks > 1) {
@@ -1731,11 +1760,11 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   t.blocks[0] = t.chunks[0] = 0;
   for (int k = 0; k < t.count; ++k) {
     const Item& it = t.it[k];
-    const int lower = lower_tiles(it, side);
-    t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + lower * it.ks;
-    t.tiles[SQUARE][k + 1] = t.tiles[SQUARE][k] + lower;
+    auto narrow = [&](int mode) { return (it.narrow >> mode & 1) != 0; };
+    t.tiles[GRAM][k + 1] = t.tiles[GRAM][k] + (int)lower_tiles(it, side, narrow(GRAM)) * it.ks;
+    t.tiles[SQUARE][k + 1] = t.tiles[SQUARE][k] + (int)lower_tiles(it, side, narrow(SQUARE));
     t.tiles[UPDATE][k + 1] =
-        t.tiles[UPDATE][k] + (int)update_tiles(it, side, it.narrow ? 1 : side);
+        t.tiles[UPDATE][k] + (int)update_tiles(it, side, narrow(UPDATE) ? 1 : side);
     t.blocks[k + 1] = t.blocks[k] + it.rb * it.cb;
     t.chunks[k + 1] = t.chunks[k] + it.chunks;
   }
@@ -1805,8 +1834,10 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn 
   double all = 0, longest = 0;
   for (const Item& it : items) {
     order.push_back(&it);
-    all += tiles_time(it, false);
-    longest = std::max(longest, tile_time(it, false));
+    long long tiles;
+    const double time = tile_time(it, UPDATE, false, &tiles);
+    all += time * tiles;
+    longest = std::max(longest, time);
   }
   if (all <= longest * ctx->num_sms)
     std::sort(order.begin(), order.end(), [](const Item* x, const Item* y) {
