@@ -361,10 +361,13 @@ __global__ void __launch_bounds__(256)
 // 256 x 2304 ended 7.3e-6 off, with two in GRAM and half a k-block elsewhere 2.1e-6
 // (fp32: 2.0e-6).  So it is one k-block where the tile meets the diagonal, two
 // elsewhere, whose handover then hides behind the tensor core's work.
-// Truncation takes off the same share on average, half a step of fp32 (2^-24) for
-// every addition at full size, and scaled_steps puts 2^-23 back in SQUARE and
-// UPDATE: the errors fell by a third to a half (256 x 2304 2.5e-6 to 1.3e-6, 1024 x
-// 1024 9.9e-7 to 7.3e-7, both with half a k-block on the diagonal).
+// Truncation takes off the same share on average, and scaled_steps puts it back in
+// SQUARE and UPDATE, where errors feed on themselves.  By measurement (means over
+// six seeds, in 1e-6; fp32 products in brackets): with more than 64 rows 2^-22 and
+// 2^-23 (100 x 1000 0.77, with 2^-23 twice 0.97, without 1.44 [1.24]; 200 x 3000
+// 1.85, 2.40, 3.74 [2.10]; 512 x 4608 1.49, 1.75 [2.77]); up to 64 rows, where the
+// later products of a k-block add zeros, 2^-23 and nothing (7 x 1131 0.70, with both
+// 0.99 [0.78]; 12 x 1131 0.62, 0.80 [0.88]; 64 x 100 0.53, 0.79 [1.14]).
 //
 // Two forms.  A single block works on 128 x 128 tiles; its MMAs are bound by their
 // reads of shared memory (12 of 128 x 128 a k-block, 8 KB each, take 117 cycles
@@ -407,8 +410,9 @@ struct Form {
 struct Steps {
   int n;
   float g2[kMaxSteps];                                // GRAM: A' = g2 acc
-  float s0[kMaxSteps], s1[kMaxSteps], s2[kMaxSteps];  // SQUARE: P' = s0 I + s1 A' + s2 acc
-  float u2[kMaxSteps];                                // UPDATE: X' = u2 acc
+  // with the shorter side up to one block and longer:
+  float s0[kMaxSteps], s1[kMaxSteps], s2[2][kMaxSteps];  // SQUARE: P' = s0 I + s1 A' + s2 acc
+  float u2[2][kMaxSteps];                                // UPDATE: X' = u2 acc
 };
 
 struct Ticket {
@@ -953,8 +957,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       // row block and row inside it
       const int rblk = F::kSide * q.i + 2 * rank + (wr >> 1), r64 = (wr & 1) * 32 + lane;
       const float c2 = q.mode == GRAM     ? steps.g2[q.step]
-                       : q.mode == SQUARE ? steps.s2[q.step]
-                                          : steps.u2[q.step];
+                       : q.mode == SQUARE ? steps.s2[im.mb > 1][q.step]
+                                          : steps.u2[im.mb > 1][q.step];
       uint8_t* out = sq ? (q.mode == GRAM ? im.a : im.p) : im.x[(q.step & 1) ^ 1];
       const size_t plane = (size_t)rbt * cbt * kBlkBytes;
       const uint8_t* own = nullptr;  // this warp's 128 columns of the tile's own A
@@ -1436,7 +1440,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
     sum_accumulators(lanes, 4, p);
     drained();
     if (in_a) {
-      const float s0 = steps.s0[s], s1 = steps.s1[s], s2 = steps.s2[s];
+      const float s0 = steps.s0[s], s1 = steps.s1[s], s2 = steps.s2[mb > 1][s];
 #pragma unroll
       for (int ch = 0; ch < 8; ++ch) {
         uint8_t* at = a_row + ((ch ^ (r64 & 7)) << 4);
@@ -1483,7 +1487,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       const int lrow = tall ? 2 * hf + (wr >> 1) : (wr >> 1);  // row and column block of the share
       const int lcol = tall ? wc : 2 * hf + wc;
       const bool inside = lrow < brows && lcol < bcols;
-      const float c2 = steps.u2[s];
+      const float c2 = steps.u2[mb > 1][s];
       if (inside) {
 #pragma unroll
         for (int c = 0; c < 64; ++c) p[c] *= c2;
@@ -1689,10 +1693,9 @@ struct Schedule {
   float sa[kMaxSteps], sp[kMaxSteps];
 };
 
-// Coefficients with the scales of the pairs folded in, and in the products that
-// feed back on themselves the mean of what the tensor core's truncation takes off.
+// Coefficients with the scales of the pairs folded in, and the share of its sums
+// that the tensor core's truncation takes off.
 Steps scaled_steps(const Schedule& s) {
-  constexpr float kPutBack = 1.f + 0x1p-23f;
   Steps st;
   st.n = s.steps;
   for (int k = 0; k < s.steps; ++k) {
@@ -1700,8 +1703,11 @@ Steps scaled_steps(const Schedule& s) {
     st.g2[k] = sa / (sx * sx);
     st.s0[k] = s.q[3 * k] * sp;
     st.s1[k] = s.q[3 * k + 1] * sp / sa;
-    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa) * kPutBack;
-    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx) * kPutBack;
+    for (int deep = 0; deep < 2; ++deep) {
+      const float s_back = 1.f + (deep ? 0x1p-22f : 0x1p-23f), u_back = deep ? 1.f + 0x1p-23f : 1.f;
+      st.s2[deep][k] = s.q[3 * k + 2] * sp / (sa * sa) * s_back;
+      st.u2[deep][k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx) * u_back;
+    }
   }
   return st;
 }
