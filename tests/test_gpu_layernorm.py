@@ -325,3 +325,23 @@ def test_numpy_and_session_wrappers(ctx):
     got = s.encodeLayerNormGrad(xs, t(dy, 6), gs)
     assert rel(got[0].toArray().reshape(6, 40), dxr) < TOL_DX
     assert rel(got[1].toArray(), dgr) < TOL_SUM and rel(got[2].toArray(), dbr) < TOL_SUM
+
+
+@pytest.mark.parametrize("rows,pad", [(1, 0), (300, 3), (5000, 0)])
+def test_rows_of_one_column_have_no_gradient(h, rows, pad):
+    """One value is its own mean: y = beta, and dx is zero to the last bit."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, dy, add = (torch.randn(rows, 1 + pad, generator=g, device="cuda") for _ in range(3))
+    gamma, y = torch.full((1,), 1.7, device="cuda"), torch.empty(rows, 1, device="cuda")
+    beta = torch.full((1,), -0.3, device="cuda")
+    call("yl_layernorm_fwd", h, p(x), 1 + pad, rows, 1, 1e-5, p(gamma), p(beta), p(y), 1, None, None)
+    assert torch.all(y == beta)
+    dx, dg, db = torch.empty(rows, 1, device="cuda"), torch.empty(1, device="cuda"), torch.empty(1, device="cuda")
+    for addend, want in ((None, torch.zeros_like(dx)), (add, add[:, :1])):
+        call("yl_layernorm_bwd", h, p(x), 1 + pad, p(dy), 1 + pad, rows, 1, 1e-5, p(gamma), None,
+             None, p(addend), 1 + pad, p(dx), 1, p(dg), p(db))
+        assert torch.equal(dx, want)
+        assert float(dg) == 0
+        # 64 roundings of partial sums, of 64 values at most each, in fp32 behind one another
+        exact = dy[:, 0].double()
+        assert abs(float(db) - float(exact.sum())) <= 64 * 2 ** -24 * float(exact.abs().sum())

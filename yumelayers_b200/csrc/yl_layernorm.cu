@@ -40,6 +40,7 @@ constexpr int kAloneTurns = 4;
 // with 16-byte accesses and e * LANES + lane without.
 template <int LANES, int PER, bool VEC>
 struct Row {
+  static constexpr int kCols = LANES * PER;
   static __device__ __forceinline__ int col(int e, int lane) {
     return VEC ? ((e >> 2) * LANES + lane) * 4 + (e & 3) : e * LANES + lane;
   }
@@ -334,13 +335,16 @@ __device__ __forceinline__ void bwd_row(const Bwd& p, long long r, bool valid, i
                                         const float (&x)[PER], const float (&dy)[PER],
                                         const float (&ga)[PER], float m, float rs,
                                         float (&dg)[PER], float (&db)[PER], float* red, Add add) {
+  // t rounded as in its mean, so that a row of one column gives exactly zero (in
+  // all sizes that costs 10% of 16384 x 4096)
+  constexpr bool kFew = R::kCols <= 16;
   float e = 0.f;
   if (!p.mean) row_stats<Own, R, PER>(x, p.cols, lane, p.eps, red, m, e, rs);
   float h[PER], s1 = 0.f, s2 = 0.f;
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     h[k] = R::col(k, lane) < p.cols ? ((x[k] - m) - e) * rs : 0.f;
-    const float t = dy[k] * ga[k];
+    const float t = kFew ? __fmul_rn(dy[k], ga[k]) : dy[k] * ga[k];
     s1 += t;
     s2 = fmaf(t, h[k], s2);
   }
@@ -363,17 +367,22 @@ __device__ __forceinline__ void bwd_row(const Bwd& p, long long r, bool valid, i
     if (p.addend) add(out);
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const float v = rs * (fmaf(dy[k], ga[k], -s1) - h[k] * s2);
+      const float t = kFew ? __fmul_rn(dy[k], ga[k]) - s1 : fmaf(dy[k], ga[k], -s1);
+      const float v = rs * (t - h[k] * s2);
       out[k] = p.addend ? out[k] + v : v;
     }
     R::store(p.dx + r * p.lddx, p.cols, lane, out);
   }
 }
 
-// A block adds its groups' column sums in order and writes a partial row.
+// A block adds its groups' column sums in order and writes a partial row; in double
+// where the groups are many and the columns too few to average the roundings.
+template <int LANES>
+using GroupSum = std::conditional_t<LANES <= 8, double, float>;
 template <int THREADS, int LANES, int PER, class R>
 __device__ __forceinline__ void flush_groups(const Bwd& p, long long part, int lane, int grp,
-                                             float (&dg)[PER], float (&db)[PER], float* sums) {
+                                             float (&dg)[PER], float (&db)[PER],
+                                             GroupSum<LANES>* sums) {
   constexpr int CAP = LANES * PER;
   for (int g = 0; g < THREADS / LANES; ++g) {
     __syncthreads();
@@ -389,8 +398,8 @@ __device__ __forceinline__ void flush_groups(const Bwd& p, long long part, int l
   __syncthreads();
   float *og = p.out_gamma(part), *ob = p.out_beta(part);
   for (int c = threadIdx.x; c < p.cols; c += THREADS) {
-    if (og) og[c] = sums[c];
-    if (ob) ob[c] = sums[CAP + c];
+    if (og) og[c] = (float)sums[c];
+    if (ob) ob[c] = (float)sums[CAP + c];
   }
 #pragma unroll
   for (int k = 0; k < PER; ++k) dg[k] = db[k] = 0.f;
@@ -402,7 +411,8 @@ __global__ void __launch_bounds__(THREADS, MIN_BLOCKS) ln_bwd_ring_kernel(const 
   using Q = Ring<THREADS, LANES, PER, 3, D>;
   extern __shared__ __align__(16) uint8_t ring[];
   constexpr bool kBlock = LANES > 32;
-  __shared__ float red[kBlock ? 64 : 2 * LANES * PER];
+  __shared__ float red[kBlock ? 64 : 1];
+  __shared__ GroupSum<LANES> sums[kBlock ? 1 : 2 * LANES * PER];
   constexpr int G = THREADS / LANES;
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const long long stride = (long long)gridDim.x * G;
@@ -444,7 +454,7 @@ __global__ void __launch_bounds__(THREADS, MIN_BLOCKS) ln_bwd_ring_kernel(const 
 #pragma unroll
         for (int k = 0; k < PER; ++k) dg[k] = db[k] = 0.f;
       } else {
-        flush_groups<THREADS, LANES, PER, R>(p, part, lane, grp, dg, db, red);
+        flush_groups<THREADS, LANES, PER, R>(p, part, lane, grp, dg, db, sums);
       }
       part += gridDim.x;
       held = 0;
@@ -458,7 +468,7 @@ template <int LANES, int PER, int UNR>
 __global__ void __launch_bounds__(256) ln_bwd_group_kernel(const __grid_constant__ Bwd p) {
   using R = Row<LANES, PER, false>;
   constexpr int G = 256 / LANES;
-  __shared__ float sums[2 * LANES * PER];
+  __shared__ GroupSum<LANES> sums[2 * LANES * PER];
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   float ga[PER], dg[PER], db[PER];
   R::load_or(p.gamma, 1.f, p.cols, lane, ga);
@@ -705,7 +715,8 @@ __global__ void __launch_bounds__(kLong) ln_bwd_long_kernel(const __grid_constan
     else long_stats(x, p.cols, p.eps, red, m, e, rs);
     double s1 = 0.0, s2 = 0.0;
     for (int c = threadIdx.x; c < p.cols; c += kLong) {
-      const float d = dy[c], h = ((x[c] - m) - e) * rs, t = d * (p.gamma ? p.gamma[c] : 1.f);
+      const float d = dy[c], h = ((x[c] - m) - e) * rs, 
+                  t = __fmul_rn(d, p.gamma ? p.gamma[c] : 1.f);
       s1 += (double)t;
       s2 += (double)t * h;
       if (pg) {
@@ -718,7 +729,7 @@ __global__ void __launch_bounds__(kLong) ln_bwd_long_kernel(const __grid_constan
     const float c1 = (float)(s1 / p.cols), c2 = (float)(s2 / p.cols);
     for (int c = threadIdx.x; c < p.cols; c += kLong) {
       const float h = ((x[c] - m) - e) * rs;
-      float v = rs * (fmaf(dy[c], p.gamma ? p.gamma[c] : 1.f, -c1) - h * c2);
+      float v = rs * ((__fmul_rn(dy[c], p.gamma ? p.gamma[c] : 1.f) - c1) - h * c2);
       if (p.addend) v += p.addend[r * p.ldadd + c];
       p.dx[r * p.lddx + c] = v;
     }
