@@ -22,6 +22,7 @@
 #include <thread>
 #include <map>
 #include <memory>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -372,7 +373,11 @@ static yl_status muon_step(yl_trainer* tr, Net& net, const MuonTables& t, float 
   st.lr = muon_lr, st.momentum = tr->muon.momentum, st.nesterov = tr->muon.nesterov != 0;
   st.weight_decay = tr->muon.weight_decay, st.steps = tr->muon.steps;
   st.grad_scale = scale, st.clip_max_norm = clip, st.sanitize = sanitize;
-  YL_TRY(muon_multi(tr->ctx, t.matrices.data(), (int)t.matrices.size(), st, nullptr, norm, nullptr));
+  try {
+    YL_TRY(muon_multi(tr->ctx, t.matrices.data(), (int)t.matrices.size(), st, nullptr, norm, nullptr));
+  } catch (const std::bad_alloc&) {
+    return set_error(YL_ERR_OOM, "yl_trainer_step: no host memory for Muon's tables");
+  }
   YL_TRY(adam_multi(tr->ctx, t.rest.data(), (int)t.rest.size(), lr, 0.9f, 0.999f, 1e-8f,
                     (int)tr->step, scale, clip, sanitize, nullptr, norm));
   return net.prepare_weights();
