@@ -108,7 +108,8 @@ def check_on_device(h, shapes):
         assert torch.equal(y, y2)
 
 
-@pytest.mark.parametrize("shapes", [[(4000, 3900)], [(900, 4097), (64, 700)] + [(1030, 1000)] * 14])
+@pytest.mark.parametrize("shapes", [[(4000, 3900)], [(900, 4097), (64, 700)] + [(1030, 1000)] * 14,
+                                    [(2500, 2560), (2050, 2049)]])
 def test_enough_tiles_for_pairs_of_blocks(h, shapes):
     """Sizes that run on 256 x 256 tiles."""
     check_on_device(h, shapes)
@@ -370,8 +371,8 @@ def test_two_contexts_at_once():
             assert rel(y.cpu(), ns64(x.cpu().numpy())) < TOL_SPREAD
 
 
-@pytest.mark.parametrize("shapes", [[(128, 1152)], [(300, 500), (64, 64)], [(1500, 1400)] * 8],
-                         ids=["on chip", "single blocks", "pairs"])
+@pytest.mark.parametrize("shapes", [[(128, 1152)], [(300, 500), (64, 64)], [(1500, 1400)] * 8, [(2560, 2500)] * 2],
+                         ids=["on chip", "single blocks", "many tiles", "pairs"])
 def test_waits_that_run_out_return_a_status(ctx, shapes):
     """With a limit of 200 cycles the kernels' waits give up, every warp leaves, and the
     host reads a timeout; with the default again the same call is right."""

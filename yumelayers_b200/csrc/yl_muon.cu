@@ -1811,20 +1811,56 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
   return check_launch("ns_steps_kernel");
 }
 
+// About how long a step of these matrices takes (us), by single blocks or by pairs
+// of them on SMs that are all busy: 0.72 us a k-block of a 128 x 128 tile, 1.1 us of
+// a 256 x 256 tile, and 2 and 6 us beside them.  The tiles of a single matrix go in
+// whole waves; those of several fill one another's, and take at least one tile of
+// each phase.
+double step_time(const std::vector<const Item*>& items, int num_sms, bool pair) {
+  const int side = pair ? 4 : 2, workers = pair ? num_sms / 2 : num_sms;
+  const double block = pair ? 1.1 : 0.72, rest = pair ? 6 : 2;
+  double sum = 0, chain = 0;
+  for (const Item* it : items) {
+    const double lower = (double)lower_tiles(*it, side, false);
+    const double update = (double)update_tiles(*it, side, side);
+    const double one = block * k_blocks(*it) + rest;
+    const double nk = (std::max(it->rows, it->cols) + kBlk - 1) / kBlk;
+    const double gram = block * nk + rest;
+    if (items.size() > 1) {
+      sum += (lower * gram + lower * one + update * one) / workers;
+      chain = std::max(chain, 3 * one);
+      continue;
+    }
+    // a Gram product that leaves SMs idle is shared out among them
+    sum += lower < workers ? std::min(gram, lower * block * nk / workers + rest + 5)
+                           : std::ceil(lower / workers) * gram;
+    // half as wide tiles, each sooner done, while they fit
+    const bool narrow = !pair && 2 * lower <= workers;
+    sum += std::ceil(lower / workers) * (narrow ? 0.7 * one : one);
+    sum += std::ceil(update / workers) * one;
+  }
+  return std::max(sum, chain);
+}
+
 // The tables of a call: matrices for pairs of blocks first, then the others.
 // A pair does twice the products per shared-memory read, but has half as many and
-// larger tiles to share among the SMs, so it pays only where the 128 x 128 tiles
-// would fill them several times over: 16 of 1024 x 1024 (1024 tiles of an UPDATE)
-// take 1.16 ms in pairs and 1.25 ms alone, one 4096 x 4096 (1024 tiles, longer
-// rows) 3.8 and 4.7 ms, one 2048 x 2048 (256 tiles) 1.19 and 0.94 ms.  Shorter
-// sides under kPairSide are mostly padding in a 256 x 256 tile.
+// larger tiles to share among the SMs, so it pays where those stay full: 4096 x 4096
+// 3.4 ms in pairs and 3.9 alone, 2560 x 2560 0.97 and 1.03, 8 of 1024 x 1024 0.53
+// and 0.56, but 4 of them 0.53 and 0.38, 2048 x 2048 0.59 and 0.52, 1024 x 8192 0.68 and 0.61, 16 of 600 x
+// 2400, which 256 x 256 tiles pad, 1.04 and 0.88.  (The estimates are within some
+// 6% of that: pairs have to promise as much.)  Sides under kPairSide are mostly
+// padding.  Where other matrices remain, they take a launch of their own.
 template <class Fn>
 yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn fn) {
   auto wide = [](const Item& it) { return std::min(it.rows, it.cols) >= kPairSide; };
-  long long tiles = 0;
-  for (const Item& it : items)
-    if (wide(it)) tiles += (long long)((it.rows + 127) / 128) * ((it.cols + 127) / 128);
-  const bool pairs = tiles >= 6LL * ctx->num_sms;
+  std::vector<const Item*> large;
+  double others = 0;
+  for (const Item& it : items) {
+    if (wide(it)) large.push_back(&it);
+    else others = std::max(others, 3 * (4.5 + 0.43 * k_blocks(it)));
+  }
+  const bool pairs = !large.empty() && step_time(large, ctx->num_sms, true) + others <
+                                           0.94 * step_time(large, ctx->num_sms, false);
   // With longer matrices beside them the short ones cost the steps kernel less
   // than a launch of their own, and so do more clusters than the SMs hold at once
   // (24 of 128 x 1152: 267 us in clusters of 8, 168 us in the steps kernel; 14 of
