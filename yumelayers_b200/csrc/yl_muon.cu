@@ -361,8 +361,9 @@ __global__ void __launch_bounds__(256)
 // 256 x 2304 ended 7.3e-6 off, with two in GRAM and half a k-block elsewhere 2.1e-6
 // (fp32: 2.0e-6).  So it is one k-block where the tile meets the diagonal, two
 // elsewhere, whose handover then hides behind the tensor core's work.
-// Truncation takes off the same share on average, and scaled_steps puts it back in
-// SQUARE and UPDATE, where errors feed on themselves.  By measurement (means over
+// Truncation takes off the same share on average, and scaled_steps puts it back:
+// 2^-22 in GRAM, whose diagonal adds up squares (10 x 4722 6.4e-7 to 5.6e-7, 100 x
+// 6000 1.17e-6 to 1.05e-6), and in SQUARE and UPDATE, by measurement (means over
 // six seeds, in 1e-6; fp32 products in brackets): with more than 64 rows 2^-22 and
 // 2^-23 (100 x 1000 0.77, with 2^-23 twice 0.97, without 1.44 [1.24]; 200 x 3000
 // 1.85, 2.40, 3.74 [2.10]; 512 x 4608 1.49, 1.75 [2.77]); up to 64 rows, where the
@@ -1694,13 +1695,13 @@ struct Schedule {
 };
 
 // Coefficients with the scales of the pairs folded in, and the share of its sums
-// that the tensor core's truncation takes off.
+// that the tensor core's truncation takes off each product.
 Steps scaled_steps(const Schedule& s) {
   Steps st;
   st.n = s.steps;
   for (int k = 0; k < s.steps; ++k) {
     const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
-    st.g2[k] = sa / (sx * sx);
+    st.g2[k] = sa / (sx * sx) * (1.f + 0x1p-22f);
     st.s0[k] = s.q[3 * k] * sp;
     st.s1[k] = s.q[3 * k + 1] * sp / sa;
     for (int deep = 0; deep < 2; ++deep) {
@@ -1846,8 +1847,8 @@ double step_time(const std::vector<const Item*>& items, int num_sms, bool pair) 
 // A pair does twice the products per shared-memory read, but has half as many and
 // larger tiles to share among the SMs, so it pays where those stay full: 4096 x 4096
 // 3.4 ms in pairs and 3.9 alone, 2560 x 2560 0.97 and 1.03, 8 of 1024 x 1024 0.53
-// and 0.56, but 4 of them 0.53 and 0.38, 2048 x 2048 0.59 and 0.52, 1024 x 8192 0.68 and 0.61, 16 of 600 x
-// 2400, which 256 x 256 tiles pad, 1.04 and 0.88.  (The estimates are within some
+// and 0.56, but 4 of them 0.53 and 0.38, 2048 x 2048 0.59 and 0.52, 1024 x 8192
+// 0.68 and 0.61, 16 of 600 x 2400, which 256 x 256 tiles pad, 1.04 and 0.88.  (The estimates are within some
 // 6% of that: pairs have to promise as much.)  Sides under kPairSide are mostly
 // padding.  Where other matrices remain, they take a launch of their own.
 template <class Fn>
