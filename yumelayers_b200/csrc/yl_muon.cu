@@ -1576,10 +1576,13 @@ double block_time(bool narrow) { return narrow ? 0.8 : 1.1; }
 int shares(const Item& it, bool narrow, int most, double* time) {
   const int nk = (std::max(it.rows, it.cols) + kBlk - 1) / kBlk;
   int best = 1;
+  double before = HUGE_VAL;
   *time = block_time(narrow) * nk;
   for (int ks = 2; ks <= std::min(most, nk); ++ks) {
     const double cost = block_time(narrow) * nk / ks + 5 + 1.2 * ks;
+    if (cost > before) break;  // it only grows from here
     if (cost < *time) *time = cost, best = ks;
+    before = cost;
   }
   return best;
 }
