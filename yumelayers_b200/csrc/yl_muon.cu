@@ -19,6 +19,7 @@
 #include "yl_internal.h"
 #include "yl_muon.h"
 #include "yl_ptx.cuh"
+#include "yl_ring.h"
 #include "yume_c.h"
 
 namespace yl {
@@ -745,6 +746,10 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     if (lane == 0) {
       uint32_t it = 0, ci = 0;
       bool ok = true;
+      auto commit = [&](uint64_t* bar) {
+        if (PAIR) umma_commit_pair(bar);
+        else umma_commit(bar);
+      };
       for (uint32_t k = 0; ok; ++k) {
         const int slot = k % kRing;
         if (!wait<PAIR>(&tfull[slot], (k / kRing) & 1, lim)) {
@@ -773,14 +778,13 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         const bool same = !narrow && q.mode != UPDATE && q.i == q.j;
         const int jt = column_tile<NARROW>(im, q);
         int filled = 0;  // k-blocks the current accumulator has taken
-        for (int kb = 0; ok && kb < q.nk; ++kb, ++it) {
-          const int s = it % kStages;
-          if (!mbar_wait(&full[s], (it / kStages) & 1, lim) ||
-              (PAIR && !wait<PAIR>(&pfull[s], (it / kStages) & 1, lim))) {
-            report_error(err, YL_DEVERR_TIMEOUT);
-            ok = false;
-            break;
-          }
+        auto landed = [&](uint32_t i) {
+          return mbar_wait(&full[i % kStages], (i / kStages) & 1, lim) &&
+                 (!PAIR || wait<PAIR>(&pfull[i % kStages], (i / kStages) & 1, lim));
+        };
+        StageWalk walk{q.nk, extra};
+        for (; walk.next(it, landed); walk.pass(it)) {
+          const int s = it % kStages, kb = walk.at;
           const int kt = (q.kb0 + kb) / F::kSide;
           const int lmn = L.mn_major | (L.sym & (q.i < kt)), rmn = R.mn_major | (R.sym & (jt < kt));
           const int cols = narrow ? 64 : F::kTile;
@@ -793,8 +797,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           const bool fine = on_diagonal<PAIR, NARROW>(im, q, kb);
           const int buf = ci % kAccs;
           if (filled == 0 && ci >= kAccs && !wait<PAIR>(&acc_empty[buf], (ci / kAccs - 1) & 1, lim)) {
-            report_error(err, YL_DEVERR_TIMEOUT);
-            ok = false;
+            walk.lost = true;
             break;
           }
           tc_fence_after();
@@ -823,24 +826,21 @@ __global__ void __launch_bounds__(kProductThreads, 1)
               umma_f16(dacc + cols, sw128_desc(l + kOpBytes + kk * lstep, llbo, 1024),
                        sw128_desc(r + kk * rstep, rlbo, 1024), idesc, 1);
           }
-          if (++filled == 2 || fine || kb + 1 == q.nk || on_diagonal<PAIR, NARROW>(im, q, kb + 1)) {
-            if (PAIR) umma_commit_pair(&acc_full[buf]);
-            else umma_commit(&acc_full[buf]);
+          if (kb + 1 < q.nk && (++filled == 2 || fine || on_diagonal<PAIR, NARROW>(im, q, kb + 1))) {
+            commit(&acc_full[buf]);
             filled = 0;
             ++ci;
           }
-          if (!ok) break;
-          if (PAIR) umma_commit_pair(&empty[s]);
-          else umma_commit(&empty[s]);
+          commit(&empty[s]);
         }
-        it += extra;  // the epilogue reads and frees those
+        // the last one behind the walk, which has then seen the epilogue's own stages
+        ok = !walk.lost;
+        if (ok) commit(&acc_full[ci++ % kAccs]);
+        else report_error(err, YL_DEVERR_TIMEOUT);
       }
       // every MMA this thread issued has completed before TMEM and the other
       // block's shared memory are released
-      if (rank == 0) {
-        if (PAIR) umma_commit_pair(drain);
-        else umma_commit(drain);
-      }
+      if (rank == 0) commit(drain);
       wait<PAIR>(drain, 0, kWaitLimitCycles);
     }
   }
