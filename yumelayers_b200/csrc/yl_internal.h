@@ -78,11 +78,10 @@ struct yl_ctx {
   void* scratch[3] = {nullptr, nullptr, nullptr};
   size_t scratch_bytes[3] = {0, 0, 0};
   // workspace of the operators that take theirs through yl::Workspace, with an
-  // event behind its last use and the stream of that use
+  // event behind its last use
   void* work = nullptr;
   size_t work_bytes = 0;
   cudaEvent_t work_ev = nullptr;
-  cudaStream_t work_stream = nullptr;
   bool work_used = false;
 };
 
@@ -117,9 +116,11 @@ class DeviceGuard {
 };
 
 // Temporaries of one operator call.  Outside a stream capture they live in the
-// context's workspace, and a call on another stream than the last one's waits
-// for that call's work first.  Inside a capture they are allocated and freed by
-// nodes of the graph itself, so a graph neither keeps a pointer into the
+// context's workspace, and every call's work waits for that of the last one: by an
+// event, whatever the stream handles, since a destroyed stream's handle may be given
+// out again while its work still runs, and the per-thread default stream's is
+// another stream in every host thread.  Inside a capture they are allocated and
+// freed by nodes of the graph itself, so a graph neither keeps a pointer into the
 // context's workspace (which may grow) nor shares it with another graph.
 class Workspace {
  public:

@@ -70,8 +70,8 @@ yl_status Workspace::get(yl_ctx* ctx, size_t bytes, char** out) {
     return YL_OK;
   }
   if (!ctx->work_ev) YL_CUDA(cudaEventCreateWithFlags(&ctx->work_ev, cudaEventDisableTiming));
-  if (ctx->work_used && ctx->work_stream != ctx->stream)
-    YL_CUDA(cudaStreamWaitEvent(ctx->stream, ctx->work_ev, 0));
+  // on equal handles too: a handle does not name a stream for good
+  if (ctx->work_used) YL_CUDA(cudaStreamWaitEvent(ctx->stream, ctx->work_ev, 0));
   if (bytes > ctx->work_bytes) {
     if (ctx->work) YL_CUDA(cudaFreeAsync(ctx->work, ctx->stream));
     ctx->work = nullptr;
@@ -100,7 +100,6 @@ yl_status Workspace::done() {
     return YL_OK;
   }
   YL_CUDA(cudaEventRecord(ctx->work_ev, ctx->stream));
-  ctx->work_stream = ctx->stream;
   ctx->work_used = true;
   return YL_OK;
 }
