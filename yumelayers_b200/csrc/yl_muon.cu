@@ -569,7 +569,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   uint64_t* ask = ready + kRing;           // rank 0
   uint64_t* drain = ask + 1;
   uint64_t* esync = drain + 1;
-  Ticket* ring = reinterpret_cast<Ticket*>(esync + 1);
+  uint64_t* seen = esync + 1;              // [2]: a SQUARE tile's own A may be freed
+  Ticket* ring = reinterpret_cast<Ticket*>(seen + 2);
   int* last_share = reinterpret_cast<int*>(ring + kRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last_share + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 1);  // [3][kMaxItems + 1]
@@ -597,6 +598,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     mbar_init(ask, 1);
     mbar_init(drain, 1);
     mbar_init(esync, kEpiWarps);
+    for (int b = 0; b < 2; ++b) mbar_init(&seen[b], 1);
     fence_barrier_init();
   }
   if (PAIR) {
@@ -744,7 +746,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     }
   } else if (warp == kEpiWarps + 1) {
     if (lane == 0) {
-      uint32_t it = 0, ci = 0;
+      uint32_t it = 0, ci = 0, squares = 0;
       bool ok = true;
       auto commit = [&](uint64_t* bar) {
         if (PAIR) umma_commit_pair(bar);
@@ -778,13 +780,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         const bool same = !narrow && q.mode != UPDATE && q.i == q.j;
         const int jt = column_tile<NARROW>(im, q);
         int filled = 0;  // k-blocks the current accumulator has taken
-        auto landed = [&](uint32_t i) {
-          return mbar_wait(&full[i % kStages], (i / kStages) & 1, lim) &&
-                 (!PAIR || wait<PAIR>(&pfull[i % kStages], (i / kStages) & 1, lim));
-        };
-        StageWalk walk{q.nk, extra};
-        for (; walk.next(it, landed); walk.pass(it)) {
-          const int s = it % kStages, kb = walk.at;
+        for (int kb = 0; ok && kb < q.nk; ++kb, ++it) {
+          const int s = it % kStages;
+          if (!mbar_wait(&full[s], (it / kStages) & 1, lim) ||
+              (PAIR && !wait<PAIR>(&pfull[s], (it / kStages) & 1, lim))) {
+            report_error(err, YL_DEVERR_TIMEOUT);
+            ok = false;
+            break;
+          }
           const int kt = (q.kb0 + kb) / F::kSide;
           const int lmn = L.mn_major | (L.sym & (q.i < kt)), rmn = R.mn_major | (R.sym & (jt < kt));
           const int cols = narrow ? 64 : F::kTile;
@@ -797,7 +800,8 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           const bool fine = on_diagonal<PAIR, NARROW>(im, q, kb);
           const int buf = ci % kAccs;
           if (filled == 0 && ci >= kAccs && !wait<PAIR>(&acc_empty[buf], (ci / kAccs - 1) & 1, lim)) {
-            walk.lost = true;
+            report_error(err, YL_DEVERR_TIMEOUT);
+            ok = false;
             break;
           }
           tc_fence_after();
@@ -826,17 +830,25 @@ __global__ void __launch_bounds__(kProductThreads, 1)
               umma_f16(dacc + cols, sw128_desc(l + kOpBytes + kk * lstep, llbo, 1024),
                        sw128_desc(r + kk * rstep, rlbo, 1024), idesc, 1);
           }
-          if (kb + 1 < q.nk && (++filled == 2 || fine || on_diagonal<PAIR, NARROW>(im, q, kb + 1))) {
+          if (++filled == 2 || fine || kb + 1 == q.nk || on_diagonal<PAIR, NARROW>(im, q, kb + 1)) {
             commit(&acc_full[buf]);
             filled = 0;
             ++ci;
           }
           commit(&empty[s]);
         }
-        // the last one behind the walk, which has then seen the epilogue's own stages
-        ok = !walk.lost;
-        if (ok) commit(&acc_full[ci++ % kAccs]);
-        else report_error(err, YL_DEVERR_TIMEOUT);
+        if (!ok || extra == 0) continue;
+        ok = pass_stages(it, extra, [&](uint32_t i) {
+          return mbar_wait(&full[i % kStages], (i / kStages) & 1, lim) &&
+                 (!PAIR || wait<PAIR>(&pfull[i % kStages], (i / kStages) & 1, lim));
+        });
+        if (!ok) {
+          report_error(err, YL_DEVERR_TIMEOUT);
+        } else {  // the epilogue may free what this thread has seen
+          uint64_t* bar = &seen[squares++ & 1];
+          mbar_arrive(bar);
+          if (PAIR) mbar_arrive_cluster(map_to_rank(smem_u32(bar), 1));
+        }
       }
       // every MMA this thread issued has completed before TMEM and the other
       // block's shared memory are released
@@ -848,7 +860,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
     reg_inc<kRegsEpilogue>();
     // epilogue: warp w owns rows 32 (w % 4) .. + 31 of the block's 128 (its TMEM
     // lanes) and columns kCols (w / 4) .. of the tile
-    uint32_t it = 0, ci = 0;
+    uint32_t it = 0, ci = 0, squares = 0;
     uint8_t* stage = smem + kOutOff + warp * kOutWarp;
     const int wr = warp & 3, wc = warp >> 2;
     // barrier of the epilogue warps; bounded like every wait, so that no warp is
@@ -1070,7 +1082,14 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       // everything this block wrote of the tile is in memory before the count says so
       if (!together()) break;
       if (q.mode == SQUARE) {
-        if (threadIdx.x < F::kCtas) mbar_arrive(&empty[(it + threadIdx.x) % kStages]);
+        // freed once the tensor-core thread has passed them, long ago by now
+        if (threadIdx.x < F::kCtas) {
+          if (wait<PAIR>(&seen[squares & 1], (squares >> 1) & 1, lim))
+            mbar_arrive(&empty[(it + threadIdx.x) % kStages]);
+          else
+            report_error(err, YL_DEVERR_TIMEOUT);
+        }
+        ++squares;
         it += F::kCtas;
       }
       if (threadIdx.x == 0) add_release(t->ctrl + kCtrlDone + 3 * q.item + q.mode, 1);

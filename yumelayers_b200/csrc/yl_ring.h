@@ -11,38 +11,22 @@
 
 namespace yl {
 
-// A role's way through the stages of a tile, from ring number `it` on: `products`
-// that it works on, then `others` that another role reads and frees.  next() waits
-// with `landed(it)` for a stage's copies and says whether there is a product to do;
-// the loop's increment passes on to the next.
+// Passes `others` stages of a tile, from ring number `it` on, that another role
+// reads and frees; `landed(it)` waits for a stage's copies.
 //
-//   for (StageWalk w{products, others}; w.next(it, landed); w.pass(it)) ...
-//
-// The stages of the others are waited for as well.  A barrier's parity tells a
-// stage's present fill from the one before only to a role that has seen every
-// fill: past one that was skipped, the wait for the next lets this role into a
-// stage that still holds, or still receives, the skipped one.  For the same reason
-// the other role must not free its stages, and so have them filled again, before
-// this walk has seen them: what lets it begin (the last accumulator of a tile) is
-// handed over behind the walk.
-struct StageWalk {
-  int products, others;
-  int at = 0;
-  bool lost = false;  // a wait ran out
-
-  template <class Landed>
-  YL_HOST_DEVICE bool next(uint32_t& it, Landed landed) {
-    for (; at < products + others; pass(it)) {
-      lost = !landed(it);
-      if (lost) return false;
-      if (at < products) return true;
-    }
-    return false;
-  }
-  YL_HOST_DEVICE void pass(uint32_t& it) {
-    ++at;
-    ++it;
-  }
-};
+// A role has to wait for those as for its own.  A barrier's parity tells a stage's
+// present fill from the one before only to a role that has seen every fill: past one
+// that was skipped, the wait for the next lets the role into a stage that still
+// holds, or still receives, the skipped one.  For the same reason the other role must
+// not free its stages, and so have them filled again, before this one has seen them:
+// it is told so on a barrier.  (One of two barriers in turn is enough for that with a
+// ring of three: the tile after the next cannot be seen before the stages of this
+// one are free.)
+template <class Landed>
+YL_HOST_DEVICE bool pass_stages(uint32_t& it, int others, Landed landed) {
+  for (int e = 0; e < others; ++e, ++it)
+    if (!landed(it)) return false;
+  return true;
+}
 
 }  // namespace yl
