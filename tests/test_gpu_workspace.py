@@ -1,8 +1,6 @@
-"""One context's workspace under stream handles that change their stream: a call on
-the per-thread default stream (one handle, a stream per host thread) after another
-thread's, and one on a new stream after a destroyed one with work left."""
+"""One context's workspace under a stream handle that is given out again: calls on
+new streams behind destroyed ones with work left."""
 import ctypes as C
-import threading
 
 import numpy as np
 import pytest
@@ -12,7 +10,6 @@ from yumelayers_b200._lib import NsMatrix, call
 from yumelayers_b200.session import Context
 
 pytestmark = pytest.mark.gpu
-PER_THREAD = 2  # the handle of the per-thread default stream
 
 
 @pytest.fixture
@@ -33,25 +30,6 @@ def orthogonalise(ctx, x, y):
     r, c = x.shape
     table = (NsMatrix * 1)(NsMatrix(x.data_ptr(), y.data_ptr(), r, c, c, c))
     call("yl_newton_schulz", ctx.handle, table, 1, 5, None, 1e-7)
-
-
-def test_host_threads_in_turn_on_their_default_streams(own):
-    xs, ys = matrices(range(6), 600, 900)
-    want = []
-    for x, y in zip(xs, ys):
-        orthogonalise(own, x, y)
-        torch.cuda.synchronize()
-        want.append(y.clone())
-        y.zero_()
-    torch.cuda.synchronize()
-    own.set_stream(PER_THREAD)
-    for x, y in zip(xs, ys):  # one thread after the other, none waiting for the GPU
-        t = threading.Thread(target=orthogonalise, args=(own, x, y))
-        t.start()
-        t.join()
-    torch.cuda.synchronize()
-    own.set_stream(None)
-    assert all(torch.equal(a, b) for a, b in zip(want, ys))
 
 
 def test_streams_destroyed_with_work_left(own):
