@@ -1,6 +1,6 @@
 """Which coefficients the Newton-Schulz entry points take: the checks come before
-the first device call, so they run without a GPU.  A call that passes them goes on
-to the stand-in for the context and is refused by the CUDA runtime."""
+the first device call, so they run without a GPU.  A negative eps, which is looked
+at behind them, ends every call there."""
 import ctypes as C
 
 import numpy as np
@@ -8,7 +8,7 @@ import pytest
 
 from yumelayers_b200._lib import NsMatrix, YumeError, call
 
-UNSUPPORTED = 8
+INVALID, UNSUPPORTED = 7, 8
 BASE = 0x7F0000000000  # stands for device memory; never dereferenced
 
 
@@ -18,7 +18,8 @@ def refused(*coeffs):
     table = (NsMatrix * 1)(NsMatrix(BASE, BASE + 4096, 4, 4, 4, 4))
     with pytest.raises(YumeError) as e:
         call("yl_newton_schulz", C.create_string_buffer(8192), table, 1, len(coeffs),
-             (C.c_float * len(flat))(*flat), 1e-7)
+             (C.c_float * len(flat))(*flat), -1.0)
+    assert e.value.status in (INVALID, UNSUPPORTED), e.value
     return e.value.status == UNSUPPORTED
 
 

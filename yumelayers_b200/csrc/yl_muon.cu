@@ -1969,21 +1969,19 @@ yl_status plan_steps(const char* who, int steps, const float* given, Schedule* s
                who, i, s);
       out[3 * s + i] = q[i];
     }
-    // |p| on [0, top] is largest at its end or where p' = a + 3 b s^2 + 5 c s^4 = 0
+    // |p| on [0, top] is largest at its end or where p' = 5 c t^2 + 3 b t + a = 0 with
+    // t = s^2; the roots without a difference of nearly equal numbers
     const double a = q[0], b = q[1], c = q[2];
     auto p = [&](double v) { return std::fabs(v * (a + v * v * (b + v * v * c))); };
     double next = p(top);
     auto at = [&](double sq) {
       if (sq > 0 && sq < top * top) next = std::max(next, p(std::sqrt(sq)));
     };
-    if (c == 0.0) {
-      if (b != 0.0) at(-a / (3 * b));
-    } else {
-      const double d = 9 * b * b - 20 * a * c;
-      if (d >= 0) {
-        at((-3 * b + std::sqrt(d)) / (10 * c));
-        at((-3 * b - std::sqrt(d)) / (10 * c));
-      }
+    const double d = 9 * b * b - 20 * a * c;
+    if (d >= 0) {
+      const double r = -0.5 * (3 * b + std::copysign(std::sqrt(d), b));
+      if (c != 0.0) at(r / (5 * c));
+      if (r != 0.0) at(a / r);
     }
     const double inner = std::fabs(a) + std::fabs(b) * top * top + std::fabs(c) * top * top * top * top;
     YL_CHECK(next <= kMaxSigma && inner <= 1024.0, YL_ERR_UNSUPPORTED,
