@@ -328,9 +328,15 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
  * host table; row strides in floats): X0 = x / (|x|_F + eps), then `steps`
  * times X <- (a I + b A + c A^2) X with A = X X^T (X^T X A-products on the right
  * for matrices with more rows than columns), y = X.  coeffs is a host array of
- * (a, b, c) per step, or NULL for (3.4445, -4.7750, 2.0315) in every step.  All
- * products carry fp32 accuracy.  Coefficients that let a singular value grow
- * past 4 are YL_ERR_UNSUPPORTED; sides go to 65536.  y may be x itself (same
+ * (a, b, c) per step, or NULL for (3.4445, -4.7750, 2.0315) in every step.
+ * Against its norm a result is as accurate as with fp32 products: X and the m x m
+ * matrices are held to 22 bits, sums are fp32.  Unlike fp32 numbers those 22 bits
+ * end at 2^-17 of the largest value X can have, and what is under 2^-40 of it is
+ * lost: rows 1e-10 of the others come out as noise or zero.  So that nothing lost
+ * grows into the result, coefficients that let small singular values grow by more
+ * than 2^17 against the largest are YL_ERR_UNSUPPORTED, as are those that let one
+ * grow past 4: the default takes 9 steps, (1.5, -0.5, 0) 29, and any 7 steps within
+ * the limit of 4 pass.  Norms far below eps keep their bits.  Sides go to 65536.  y may be x itself (same
  * stride); any other overlap between a result and another matrix of the table
  * is YL_ERR_INVALID.  An empty matrix is skipped, a zero matrix gives zeros, and
  * one with a NaN or an infinity gives NaN and leaves the others alone.  Equal
@@ -482,7 +488,7 @@ typedef struct yl_muon_config {
   float momentum;          /* 0 to below 1, e.g. 0.95 */
   int nesterov;
   float weight_decay;
-  int steps;               /* Newton-Schulz steps, e.g. 5 */
+  int steps;               /* Newton-Schulz steps, e.g. 5; at most 9 */
 } yl_muon_config;
 yl_status yl_trainer_set_muon(yl_trainer* tr, const yl_muon_config* cfg_or_null);
 /* The inference path of Interpolation.swift:263-373 without the file and

@@ -60,3 +60,40 @@ def test_random_coefficients_against_a_grid():
         seen[top > 4.0] += 1
         assert refused(*q) == (top > 4.0), (q, top)
     assert min(seen.values()) > 50, seen
+
+
+def test_growth_of_small_values():
+    """Small singular values may grow by 2^17 against the largest: |p(s)| <= g s with g the
+    largest |a + b s^2 + c s^4|, so by the product of the g over the largest value at the
+    end.  The default's g is 3.4445 and its values stay under 1.21: 9 steps 5.7e4, 10
+    steps 1.9e5."""
+    quintic = (3.4445, -4.7750, 2.0315)
+    for steps in range(1, 33):
+        assert refused(*[quintic] * steps) == (steps > 9), steps
+    for steps in (1, 12, 29):  # 1.5^29 = 1.28e5, the largest value is 1
+        assert not refused(*[(1.5, -0.5, 0.0)] * steps)
+    assert refused(*[(1.5, -0.5, 0.0)] * 30)
+    # growth that the next step takes back lets nothing grow against the largest value
+    assert not refused(*[(3.9, 0.0, 0.0), (0.25, 0.0, 0.0)] * 16)
+    assert not refused(*[(1.0, 0.0, 0.0)] * 32)
+    # five is the most a step can do to an odd polynomial of degree five
+    assert not any(refused(*[(5.0, -20.0, 16.0)] * n) for n in range(1, 8))
+
+
+def test_no_growth_limit_below_seven_steps():
+    rng = np.random.default_rng(1)
+    for _ in range(100):
+        q = []
+        while len(q) < 7:
+            step = rng.uniform(-5, 5, 3)
+            step *= rng.uniform(0.3, 3.9) / largest(q + [tuple(step)], 2001)[-1]
+            q.append(tuple(float(np.float32(v)) for v in step))
+        assert not refused(*q), q
+
+
+def test_the_default_coefficients_are_checked_too():
+    table = (NsMatrix * 1)(NsMatrix(BASE, BASE + 4096, 4, 4, 4, 4))
+    for steps, status in ((9, INVALID), (10, UNSUPPORTED), (32, UNSUPPORTED)):
+        with pytest.raises(YumeError) as e:
+            call("yl_newton_schulz", C.create_string_buffer(8192), table, 1, steps, None, -1.0)
+        assert e.value.status == status

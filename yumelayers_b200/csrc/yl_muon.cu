@@ -39,7 +39,11 @@ constexpr int kNormParts = 1024;   // most partials of one matrix: larger ones t
 // tensor cores: as exact as an fp32 product (the dropped lo lo term is 2^-22 of
 // a product), at a third of the fp16 rate, where the tf32 rate is half of it
 // with 11 bits.  The scales are powers of two, per step, that keep the largest
-// value the iteration can reach under fp16's range.
+// value the iteration can reach under fp16's range.  A pair has 22 bits down to
+// 2^-17 of that value and none below 2^-40 of it, where an fp32 number goes on: so
+// the scales of a matrix whose norm is far below eps start higher (below_one), and
+// steps that would let what lies under that floor grow into the result are refused
+// (plan_steps).
 //
 // Each plane (hi, lo) is a grid of 64 x 64 blocks of 8 KB whose bytes are
 // already in the 128-byte-swizzled order the tensor core reads: 64 rows of 128
@@ -80,6 +84,7 @@ struct Table {
   int count;
   int pair;                     // worked on by pairs of blocks, 256 x 256 tiles
   int chip;                     // stays in shared memory
+  int below[kMaxItems];         // below_one of each item, from the split pass
   int* ctrl;                    // ticket counter, done[item][3], arrivals of split GRAM tiles
   int ctrl_ints;
 };
@@ -257,10 +262,19 @@ __device__ __forceinline__ double inverse_norm(double squares, float eps) {
   const double norm = sqrt(squares);
   return isinf(norm) ? __longlong_as_double(0x7ff8000000000000LL) : 1.0 / (norm + (double)eps);
 }
-__device__ __forceinline__ double inverse_norm(const Item& it, float eps) {
+__device__ __forceinline__ double item_squares(const Item& it) {
   double s = 0.0;
   for (int c = threadIdx.x; c < it.chunks; c += 256) s += it.part[c];
-  return inverse_norm(block_sum256(s), eps);
+  return block_sum256(s);
+}
+// X0's norm |u| / (|u| + eps) is at most 2^-(what this returns): 0 unless eps is the
+// larger of the two.
+constexpr int kMaxBelow = 120;  // X0's values are then at the end of fp32's range
+__device__ __forceinline__ int below_one(double squares, float eps) {
+  const double norm = sqrt(squares), e = (double)eps;
+  if (!(norm > 0.0 && norm < e)) return 0;
+  const double ratio = norm / (norm + e);
+  return ratio > 0.0 ? max(0, min(kMaxBelow, -1 - ilogb(ratio))) : 0;
 }
 
 __device__ __forceinline__ void split_pair(float v, __half* hi, __half* lo) {
@@ -271,13 +285,18 @@ __device__ __forceinline__ void split_pair(float v, __half* hi, __half* lo) {
 // X0 = u / (|u| + eps) as fp16 pairs, one 64 x 64 block per thread block; each
 // thread fills two 16-byte chunks of either plane.
 __global__ void __launch_bounds__(256)
-    ns_split_kernel(const Table* __restrict__ t, const __grid_constant__ Update u, float sx) {
+    ns_split_kernel(const Table* __restrict__ t, const __grid_constant__ Update u, float sx,
+                    int* __restrict__ below_out) {
   // from the end, which the pass before has left in L2 (U-Net 439 -> 436 us)
   const int at0 = gridDim.x - 1 - blockIdx.x, k = find_item(t->blocks, t->count, at0);
   const Item& it = t->it[k];
   const int b = at0 - t->blocks[k];
   const int rb = b / it.cb, cb = b - rb * it.cb;
-  const double inv = inverse_norm(it, u.eps);
+  const double squares = item_squares(it);
+  const int below = below_one(squares, u.eps);
+  double inv = inverse_norm(squares, u.eps);
+  if (below) inv = ldexp(inv, below);
+  if (b == 0 && threadIdx.x == 0) below_out[k] = below;
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   uint8_t* hi = it.x[0] + (size_t)b * kBlkBytes;
   uint8_t* lo = hi + (size_t)it.rb * it.cb * kBlkBytes;
@@ -320,7 +339,7 @@ __global__ void __launch_bounds__(256)
   const int k = find_item(t->chunks, t->count, blockIdx.x);
   const Item& it = t->it[k];
   const int chunk = blockIdx.x - t->chunks[k];
-  const double inv = inverse_norm(it, u.eps);
+  const double inv = inverse_norm(item_squares(it), u.eps);
   const float clipf = u.muon ? clip_factor(u) : 1.f;
   const long long total = (long long)it.rows * it.cols;
   const long long lo = (long long)chunk * it.chunk;
@@ -416,10 +435,30 @@ struct Steps {
   // with the shorter side up to one block and longer:
   float s0[kMaxSteps], s1[kMaxSteps], s2[2][kMaxSteps];  // SQUARE: P' = s0 I + s1 A' + s2 acc
   float u2[2][kMaxSteps];                                // UPDATE: X' = u2 acc
+  // X grows by at most 2^rise[k] before step k, against the bounds of the scales
+  int rise[kMaxSteps + 1];
+};
+
+// The factors of a matrix that starts `below` powers of two under the scales' bound:
+// X is kept by 2^s larger and A by 2^(2 s), as long as that still counts in P (A less
+// than 2^-60 of the identity's part does not), until the growth of the steps has
+// used it up.
+struct Lift {
+  int s, a;
+  __device__ Lift(const Steps& st, int below, int step)
+      : s(max(0, below - st.rise[step])), a(min(2 * s, 60)) {}
+  __device__ float gram(float g2) const { return ldexpf(g2, a - 2 * s); }
+  __device__ float linear(float s1) const { return ldexpf(s1, -a); }
+  __device__ float square(float s2) const { return ldexpf(s2, -2 * a); }
+  // (the last step's result is not kept at a scale)
+  __device__ float update(const Steps& st, int below, int step, float u2) const {
+    return ldexpf(u2, (step + 1 == st.n ? 0 : max(0, below - st.rise[step + 1])) - s);
+  }
 };
 
 struct Ticket {
   int step, mode, item, i, j, kb0, nk, share, tile;
+  float c2, s1;  // the tile is c2 times its sums (+ s1 A + s0 I)
 };
 constexpr int kTicketInts = sizeof(Ticket) / 4, kNoTicket = -1;  // mode behind the last one
 
@@ -574,11 +613,13 @@ __global__ void __launch_bounds__(kProductThreads, 1)
   int* last_share = reinterpret_cast<int*>(ring + kRing);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last_share + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 1);  // [3][kMaxItems + 1]
+  int* below = start + 3 * (kMaxItems + 1);            // [kMaxItems]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0;
   const int count = t->count;
   for (int i = threadIdx.x; i < 3 * (kMaxItems + 1); i += kProductThreads)
     start[i] = (&t->tiles[0][0])[i];
+  for (int i = threadIdx.x; i < count; i += kProductThreads) below[i] = t->below[i];
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], 1);
@@ -644,7 +685,23 @@ __global__ void __launch_bounds__(kProductThreads, 1)
           }
           const int n = atomicAdd(t->ctrl, 1);
           q.mode = kNoTicket;
-          if (n < total) q = ticket_of<PAIR, NARROW>(t, start, count, n);
+          if (n < total) {
+            q = ticket_of<PAIR, NARROW>(t, start, count, n);
+            // (looked up here and not in the epilogue, which every tile waits for: 512 x 512
+            // and 512 x 128 148.4 us, there 150.8)
+            const bool deep = t->it[q.item].mb > 1;
+            q.c2 = q.mode == GRAM     ? steps.g2[q.step]
+                   : q.mode == SQUARE ? steps.s2[deep][q.step]
+                                      : steps.u2[deep][q.step];
+            q.s1 = steps.s1[q.step];
+            if (const int e = below[q.item]) {
+              const Lift lift(steps, e, q.step);
+              q.c2 = q.mode == GRAM     ? lift.gram(q.c2)
+                     : q.mode == SQUARE ? lift.square(q.c2)
+                                        : lift.update(steps, e, q.step, q.c2);
+              q.s1 = lift.linear(q.s1);
+            }
+          }
           ring[slot] = q;
           mbar_arrive(&tfull[slot]);
           if (PAIR) {
@@ -970,9 +1027,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
       const int rbt = sq ? im.mb : im.rb, cbt = sq ? im.mb : im.cb;
       // row block and row inside it
       const int rblk = F::kSide * q.i + 2 * rank + (wr >> 1), r64 = (wr & 1) * 32 + lane;
-      const float c2 = q.mode == GRAM     ? steps.g2[q.step]
-                       : q.mode == SQUARE ? steps.s2[im.mb > 1][q.step]
-                                          : steps.u2[im.mb > 1][q.step];
+      const float c2 = q.c2;
       uint8_t* out = sq ? (q.mode == GRAM ? im.a : im.p) : im.x[(q.step & 1) ^ 1];
       const size_t plane = (size_t)rbt * cbt * kBlkBytes;
       const uint8_t* own = nullptr;  // this warp's 128 columns of the tile's own A
@@ -1027,7 +1082,7 @@ __global__ void __launch_bounds__(kProductThreads, 1)
         }
         const size_t blk = ((size_t)rblk * cbt + cblk) * kBlkBytes;
         if (q.mode == SQUARE) {
-          const float s1 = steps.s1[q.step], s0 = steps.s0[q.step];
+          const float s1 = q.s1, s0 = steps.s0[q.step];
           const uint8_t* ah = own + (2 * (wr >> 1) + (PAIR ? slab : wc)) * kBlkBytes + r64 * 128;
 #pragma unroll
           for (int ch = 0; ch < 8; ++ch) {
@@ -1121,7 +1176,10 @@ constexpr int kChipAOff = 2 * kChipXPlane;           // A, then P; before that t
 constexpr int kChipAPlane = 4 * kBlkBytes;
 constexpr int kChipOutOff = kChipAOff + 2 * kChipAPlane;  // what the block sends
 constexpr int kChipBarOff = kChipOutOff + 2 * kChipAPlane;
-constexpr int kChipSmem = kChipBarOff + 512 + 1024;  // barrier and norms, alignment
+// barriers and norms, the factors of every step, alignment
+constexpr int kChipFactors = 4;
+constexpr int kChipSmem = kChipBarOff + 512 + kMaxSteps * kChipFactors * 4 + 1024;
+static_assert(kChipSmem <= 227 * 1024, "a block's shared memory");
 constexpr int kChipThreads = 256;
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -1175,6 +1233,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   uint64_t* rows_in = done + 2;   // finished rows of A
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 3);
   double* norms = reinterpret_cast<double*>(smem + kChipBarOff + 64);  // [kChipShare]
+  float* factors = reinterpret_cast<float*>(smem + kChipBarOff + 512);  // g2, s1, s2, u2 per step
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp & 3, wc = warp >> 2;
   const int rank = (int)cluster_rank();
@@ -1274,7 +1333,17 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   cluster_wait();
   double total = 0.0;
   for (int r = 0; r < share; ++r) total += norms[r];
-  const double inv = inverse_norm(total, u.eps);
+  const int below = below_one(total, u.eps);
+  double inv = inverse_norm(total, u.eps);
+  if (below) inv = ldexp(inv, below);
+  if (tid < steps.n) {
+    const Lift lift(steps, below, tid);
+    float* f = factors + kChipFactors * tid;
+    f[0] = lift.gram(steps.g2[tid]);
+    f[1] = lift.linear(steps.s1[tid]);
+    f[2] = lift.square(steps.s2[mb > 1][tid]);
+    f[3] = lift.update(steps, below, tid, steps.u2[mb > 1][tid]);
+  }
 
   // Block (long, short) of the share: a wide X keeps its row blocks together (the
   // 128 rows of a K-major operand), a tall one its row blocks along the long side.
@@ -1351,6 +1420,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
   const int rows = mb * kBlk / share;  // rows of A that a block adds up
   uint8_t* outbox = smem + kChipOutOff;
   for (int s = 0; s < steps.n; ++s) {
+    const float* factor = factors + kChipFactors * s;
     // ---- this share of A = X X^T (X^T X)
     const int kks = 4 * mw, gchain = max(1, (kks + 3) / 4);
     if (kks > 0)
@@ -1368,7 +1438,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
     if (share == 1) {
       if (in_a) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c) p[c] *= steps.g2[s];
+        for (int c = 0; c < 64; ++c) p[c] *= factor[0];
 #pragma unroll
         for (int ch = 0; ch < 8; ++ch) {
           uint4 hi, lo;
@@ -1422,7 +1492,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
           a[4] += y.x, a[5] += y.y, a[6] += y.z, a[7] += y.w;
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] *= steps.g2[s];
+        for (int j = 0; j < 8; ++j) a[j] *= factor[0];
         split8(a, &hi[i], &lo[i]);
       }
       // ---- finished rows to every block: in both planes and each column block the
@@ -1461,7 +1531,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
     sum_accumulators(lanes, 4, p);
     drained();
     if (in_a) {
-      const float s0 = steps.s0[s], s1 = steps.s1[s], s2 = steps.s2[mb > 1][s];
+      const float s0 = steps.s0[s], s1 = factor[1], s2 = factor[2];
 #pragma unroll
       for (int ch = 0; ch < 8; ++ch) {
         uint8_t* at = a_row + ((ch ^ (r64 & 7)) << 4);
@@ -1508,7 +1578,7 @@ __global__ void __launch_bounds__(kChipThreads, 1)
       const int lrow = tall ? 2 * hf + (wr >> 1) : (wr >> 1);  // row and column block of the share
       const int lcol = tall ? wc : 2 * hf + wc;
       const bool inside = lrow < brows && lcol < bcols;
-      const float c2 = steps.u2[mb > 1][s];
+      const float c2 = factor[3];
       if (inside) {
 #pragma unroll
         for (int c = 0; c < 64; ++c) p[c] *= c2;
@@ -1715,6 +1785,7 @@ struct Schedule {
   float q[3 * kMaxSteps];    // coefficients
   float sx[kMaxSteps + 1];   // scales of X before each step and at the end
   float sa[kMaxSteps], sp[kMaxSteps];
+  int rise[kMaxSteps + 1];   // see Steps
 };
 
 // Coefficients with the scales of the pairs folded in, and the share of its sums
@@ -1722,6 +1793,7 @@ struct Schedule {
 Steps scaled_steps(const Schedule& s) {
   Steps st;
   st.n = s.steps;
+  std::copy(s.rise, s.rise + s.steps + 1, st.rise);
   for (int k = 0; k < s.steps; ++k) {
     const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
     st.g2[k] = sa / (sx * sx) * (1.f + 0x1p-22f);
@@ -1805,7 +1877,7 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
     ns_direct_kernel<<<t.chunks[t.count], 256, 0, ctx->stream>>>(dt, u);
     return check_launch("ns_direct_kernel");
   }
-  ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0]);
+  ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0], dt->below);
   YL_TRY(check_launch("ns_split_kernel"));
   const Steps st = scaled_steps(s);
   // More blocks than a phase has tickets: they hold tickets of the phases to come,
@@ -1954,14 +2026,24 @@ float scale_for(double top) {
   return (float)std::ldexp(1.0, std::min(e - 1, 20));
 }
 
+// How far the steps may let a small singular value grow against the largest one.
+// What lies under the pairs' floor is lost at the start of a step and grows from
+// there on; where the small values are those of small rows, fp32 products would have
+// kept it.  By a CPU model of the formats, rows of 1 and 1e-6 to 1e-10 by turns, 512 x
+// 1024: 9 quintic steps (2^16.1) end 1.5e-6 off where fp32 products end 3.0e-6 off, 10
+// (2^17.8) 4.7e-6 [3.5e-6], 12 (2^21.4) 5.4e-5, 20 (2^35.7) 2.8e-2.
+constexpr double kMaxGrowth = 131072.0;
+
 // The coefficients and scales of every step, if the coefficients keep the
-// singular values (at most 1 at the start) below kMaxSigma.
+// singular values (at most 1 at the start) below kMaxSigma and the growth of small
+// ones below kMaxGrowth.
 yl_status plan_steps(const char* who, int steps, const float* given, Schedule* s_out) {
   float* out = s_out->q;
   s_out->steps = steps;
   YL_CHECK(steps >= 0 && steps <= kMaxSteps, YL_ERR_INVALID, "%s: %d steps (0 to %d)", who, steps,
            kMaxSteps);
-  double top = 1.0;
+  double top = 1.0, growth = 1.0;
+  s_out->rise[0] = 0;
   for (int s = 0; s < steps; ++s) {
     const float* q = given ? given + 3 * s : kQuintic;
     for (int i = 0; i < 3; ++i) {
@@ -1992,6 +2074,18 @@ yl_status plan_steps(const char* who, int steps, const float* given, Schedule* s
     s_out->sx[s] = scale_for(top);
     s_out->sa[s] = scale_for(top * top);
     s_out->sp[s] = scale_for(inner);
+    // |p(s)| / s is largest at an end of [0, top] or where its derivative is 0
+    auto gain = [&](double sq) { return std::fabs(a + sq * (b + sq * c)); };
+    double most = std::max(gain(0.0), gain(top * top));
+    if (c != 0.0) most = std::max(most, gain(std::min(top * top, std::max(0.0, -b / (2 * c)))));
+    const double bound = std::max(next, 1e-3);  // what the next scale allows for
+    const double up = most * top / bound;
+    s_out->rise[s + 1] = s_out->rise[s] + (up > 1.0 ? (int)std::ceil(std::log2(up)) : 0);
+    growth = std::max(growth, 1.0) * up;
+    YL_CHECK(growth <= kMaxGrowth, YL_ERR_UNSUPPORTED,
+             "%s: by step %d the coefficients let small singular values grow by %.3g against the "
+             "largest (at most %.3g)",
+             who, s, growth, kMaxGrowth);
     top = next;
   }
   s_out->sx[std::max(steps, 0)] = scale_for(top);
@@ -2020,6 +2114,11 @@ bool rows_overlap(const float* a, long long lda, long long rows_a, long long col
   long long d = ((long long)(b0 - a0) / 4) % lda;
   if (d < 0) d += lda;
   return !(d >= cols_a && d + cols_b <= lda);
+}
+
+yl_status check_steps(const char* who, int steps, const float* coeffs) {
+  Schedule q;
+  return plan_steps(who, steps, coeffs, &q);
 }
 
 yl_status newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int steps,

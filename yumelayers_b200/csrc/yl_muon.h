@@ -17,6 +17,8 @@ struct MuonStep {
 };
 
 // coeffs: three per step, or null for the quintic (3.4445, -4.7750, 2.0315).
+// Whether the operators take these steps.
+yl_status check_steps(const char* who, int steps, const float* coeffs);
 yl_status newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int steps,
                         const float* coeffs, float eps);
 // norm: device scalar with the gradients' global norm for the clip, or null to

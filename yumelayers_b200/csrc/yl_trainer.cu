@@ -743,6 +743,7 @@ yl_status yl_trainer_set_muon(yl_trainer* tr, const yl_muon_config* cfg) {
            "yl_trainer_set_muon: momentum %g (0 to below 1)", (double)cfg->momentum);
   YL_CHECK(cfg->steps >= 1 && cfg->steps <= 32, YL_ERR_INVALID,
            "yl_trainer_set_muon: %d steps (1 to 32)", cfg->steps);
+  YL_TRY(check_steps("yl_trainer_set_muon", cfg->steps, nullptr));
   try {
     if (tr->muon_tables[0].matrices.empty()) {
       tr->muon_tables[0] = muon_tables_of(*tr->vae, "enc.conv_in", "dec.conv_out");

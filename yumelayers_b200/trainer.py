@@ -139,7 +139,7 @@ class Trainer:
     def set_muon(self, lr_vae=0.02, lr_motion=0.02, momentum=0.95, nesterov=True,
                  weight_decay=0.0, steps=5) -> None:
         """Muon for the hidden weight matrices from the next step on, Adam for the
-        rest (yl_trainer_set_muon)."""
+        rest (yl_trainer_set_muon); 1 to 9 steps."""
         kw = dict(lr_vae=float(lr_vae), lr_motion=float(lr_motion), momentum=float(momentum),
                   nesterov=bool(nesterov), weight_decay=float(weight_decay), steps=int(steps))
         cfg = MuonConfig(**{k: int(v) if k == "nesterov" else v for k, v in kw.items()})
