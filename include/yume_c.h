@@ -305,7 +305,10 @@ yl_status yl_adam_multi(yl_ctx* ctx, const yl_adam_tensor* table, int count, flo
  * mean_out / rstd_out (rows, optional) receive the statistics for the backward
  * call.  y may be x itself (same stride); any other overlap of a result is
  * YL_ERR_INVALID.
- * A row with a NaN or an infinity becomes NaN; other rows do not see it.
+ * A row with a NaN or an infinity becomes NaN; other rows do not see it.  So does a
+ * finite row whose differences from the mean have squares that sum past 3.4e38 (in
+ * rows of more than 16384 columns, whose sums are in double, only where a difference
+ * itself does).  With eps under 1e-30 and differences under 1e-18 squares lose bits.
  * Columns past cols in a padded row are neither read nor written.  cols goes to
  * 2^29. */
 yl_status yl_layernorm_fwd(yl_ctx* ctx, const float* x, long long ldx, long long rows, int cols,
@@ -316,7 +319,7 @@ yl_status yl_layernorm_fwd(yl_ctx* ctx, const float* x, long long ldx, long long
  *   dgamma = sum over rows of dy h, dbeta = sum over rows of dy (overwritten;
  *   zero for rows = 0; fixed summation order).
  * mean and rstd come from the forward call or are both NULL (recomputed with
- * eps).  dx, dgamma, dbeta may be NULL.  dx may be addend (same stride); any
+ * eps); a row that the forward call makes NaN has a NaN dx, and makes dgamma NaN.  dx, dgamma, dbeta may be NULL.  dx may be addend (same stride); any
  * other overlap of a result is YL_ERR_INVALID. */
 yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const float* dy,
                            long long lddy, long long rows, int cols, float eps, const float* gamma,

@@ -133,7 +133,10 @@ struct Block {
   }
 };
 
-// mean (rounded), what it is short of, and 1 / sqrt(var + eps)
+// mean (rounded), what it is short of, and 1 / sqrt(var + eps).  A row whose sums pass
+// fp32's range becomes NaN, as one with a NaN or an infinity does.  (A second look at
+// such rows with the differences scaled down, in registers or from memory, cost all
+// others: 25000 x 2047 forward 90 to 103 us, 6000 x 8192 backward 135 to 148.)
 template <class Own, class R, int PER>
 __device__ __forceinline__ void row_stats(const float (&x)[PER], int cols, int lane, float eps,
                                           float* red, float& m, float& e, float& rs) {
@@ -154,7 +157,7 @@ __device__ __forceinline__ void row_stats(const float (&x)[PER], int cols, int l
   Own::sum2(d1, d2, red);
   e = d1 * inv;
   rs = 1.f / sqrtf(fmaxf(fmaf(-e, e, d2 * inv), 0.f) + eps);
-  if (isnan(d2)) rs = d2;  // fmaxf would drop a NaN
+  if (!(d2 < INFINITY)) rs = NAN;
 }
 
 struct Fwd {
@@ -675,7 +678,8 @@ __device__ __forceinline__ void long_stats(const float* x, int cols, float eps, 
   s /= cols;
   s2 = s2 / cols - s * s;
   e = (float)s;
-  rs = (float)(1.0 / sqrt((s2 < 0.0 ? 0.0 : s2) + (double)eps));  // a NaN stays one
+  rs = (float)(1.0 / sqrt((s2 < 0.0 ? 0.0 : s2) + (double)eps));
+  if (!(s2 < INFINITY)) rs = NAN;  // a NaN, an infinity or a difference past fp32's range
 }
 
 __global__ void __launch_bounds__(kLong) ln_fwd_long_kernel(const __grid_constant__ Fwd p) {
