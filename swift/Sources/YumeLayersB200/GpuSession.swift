@@ -320,13 +320,15 @@ public final class GpuSession {
         return c
     }
 
-    /// One Muon step of one weight matrix, in place.
+    /// One Muon step of one weight matrix, in place.  `scale`: the matrix's factor on lr
+    /// (nil: sqrt(max(1, rows / cols))).
     public func muonUpdate(param: GPUTensor, grad: GPUTensor, momentum: GPUTensor, lr: Float,
                            mu: Float = 0.95, nesterov: Bool = true, weightDecay: Float = 0,
-                           scale: Float = 1) throws {
+                           scale: Float? = nil) throws {
         precondition(param.n == grad.n && param.n == momentum.n)
+        let factor = scale ?? max(1, Float(param.rows) / Float(max(param.cols, 1))).squareRoot()
         var t = yl_muon_tensor(param: param.ptr, grad: grad.ptr, momentum: momentum.ptr,
-                               rows: Int32(param.rows), cols: Int32(param.cols), scale: scale)
+                               rows: Int32(param.rows), cols: Int32(param.cols), scale: factor)
         try check(yl_muon_multi(ctx, &t, 1, lr, mu, nesterov ? 1 : 0, weightDecay, 5, nil, 1e-7, 1, 0,
                                 0, nil))
     }

@@ -12,7 +12,7 @@ import ctypes as C
 import numpy as np
 
 from ._lib import LAYOUT_NCHW, AdamTensor, ConvDesc, MuonTensor, NsMatrix, call
-from .session import Context, GPUTensor
+from .session import Context, GPUTensor, muon_scale
 
 
 def _dev(ctx: Context, a) -> GPUTensor:
@@ -230,12 +230,6 @@ def newton_schulz(matrices, steps=5, coeffs=None, eps=1e-7, ctx: Context | None 
     call("yl_newton_schulz", ctx.handle, table, len(shapes), int(steps), _coeffs(coeffs, steps),
          float(eps))
     return [y.toArray()[: r * c].reshape(r, c) for y, (r, c) in zip(yd, shapes)]
-
-
-def muon_scale(rows: int, cols: int) -> float:
-    """sqrt(max(1, rows / cols)): a factor on lr that gives the update of a tall
-    matrix the root-mean-square gain of a square one's."""
-    return float(max(1.0, rows / max(cols, 1)) ** 0.5)
 
 
 def muon_multi(params, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0,

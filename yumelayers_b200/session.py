@@ -19,6 +19,12 @@ from ._lib import BINARY, UNARY, MuonTensor, NsMatrix, YumeError, call, lib
 _CTX: dict[int, "Context"] = {}
 
 
+def muon_scale(rows: int, cols: int) -> float:
+    """sqrt(max(1, rows / cols)): a factor on lr that gives the update of a tall
+    matrix the root-mean-square gain of a square one's."""
+    return float(max(1.0, rows / max(cols, 1)) ** 0.5)
+
+
 class Context:
     """A ``yl_ctx``: one device, one stream (MetalEngine.swift:6-60)."""
 
@@ -360,12 +366,14 @@ class GpuSession:
         return out
 
     def muonUpdate(self, param, grad, momentum, lr, mu=0.95, nesterov=True,  # noqa: N802
-                   weight_decay=0.0, scale=1.0) -> None:
-        """One Muon step of one weight matrix, in place (yl_muon_multi)."""
+                   weight_decay=0.0, scale=None) -> None:
+        """One Muon step of one weight matrix, in place (yl_muon_multi).
+        scale: the matrix's factor on lr (None: muon_scale of its shape)."""
         self._same(param, grad, "muonUpdate")
         self._same(param, momentum, "muonUpdate")
+        scale = muon_scale(param.rows, param.cols) if scale is None else float(scale)
         table = (MuonTensor * 1)(MuonTensor(param.ptr, grad.ptr, momentum.ptr, param.rows,
-                                            param.cols, float(scale)))
+                                            param.cols, scale))
         call("yl_muon_multi", self.ctx.handle, table, 1, float(lr), float(mu), int(bool(nesterov)),
              float(weight_decay), 5, None, 1e-7, 1.0, 0.0, 0, None)
 
