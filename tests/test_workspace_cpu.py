@@ -1,5 +1,5 @@
-"""The workspace of operator calls (csrc/yl_runtime.cu) against a stand-in for the
-CUDA runtime that writes down what is asked of it.
+"""The workspace and the error messages of operator calls (csrc/yl_runtime.cu) against
+a stand-in for the CUDA runtime that writes down what is asked of it.
 
 A stream handle does not name a stream for good: a destroyed stream's handle is
 given out again while its work still runs, and the per-thread default stream's
@@ -16,6 +16,8 @@ CSRC = ROOT / "yumelayers_b200" / "csrc"
 PROGRAM = r"""
 #include <cstdio>
 #include <cstdlib>
+#include <cstring>
+#include <new>
 #include <string>
 #include <vector>
 #include "yl_internal.h"
@@ -49,6 +51,15 @@ cudaError_t cudaGetLastError() { return cudaSuccess; }
 const char* cudaGetErrorString(cudaError_t) { return "stand-in"; }
 }
 
+static bool no_new = false;  // operator new fails
+void* operator new(size_t n) {
+  void* p = no_new ? nullptr : malloc(n);
+  if (!p) throw std::bad_alloc();
+  return p;
+}
+void operator delete(void* p) noexcept { free(p); }
+void operator delete(void* p, size_t) noexcept { free(p); }
+
 static void use(yl_ctx* ctx, size_t bytes) {
   yl::Workspace w;
   char* p = nullptr;
@@ -67,6 +78,13 @@ int main(int, char** argv) {
     case 'l': use(&ctx, 100000); break;
     case 'c': capturing = !capturing; break;
     case 'm': no_memory = !no_memory; break;
+    case 'e': {  // an error is reported where there is no host memory left
+      no_new = true;
+      const yl_status st = yl::set_error(YL_ERR_OOM, "no host memory for %d matrices, %2000d", 7, 8);
+      const char* text = yl_last_error_message();
+      no_new = false;
+      printf("error %d %zu %.*s\n", (int)st, strlen(text), 24, text);
+    }
   }
   for (const std::string& s : log_) puts(s.c_str());
 }
@@ -122,3 +140,10 @@ def test_after_an_allocation_that_failed_the_next_call_takes_a_new_buffer(calls)
     log = [w for w, *_ in calls("asmlms")]
     assert log == ["malloc", "use", "record", "wait", "free", "status", "wait", "malloc", "use",
                    "record"]
+
+
+def test_errors_are_reported_without_host_memory(calls):
+    """A status that says there is no memory left takes none for its message."""
+    (what, status, length, *text), = calls("e")
+    assert what == "error" and int(length) == 1023
+    assert " ".join(text) == "no host memory for 7 mat"

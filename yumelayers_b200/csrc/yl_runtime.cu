@@ -7,22 +7,22 @@
 #include <atomic>
 #include <cstdio>
 #include <cstring>
-#include <string>
 #include <thread>
 
 #include "yl_internal.h"
 
 namespace yl {
 
-static thread_local std::string t_last_error;
+// (not a string: an error that says there is no host memory must not ask for some)
+static thread_local char t_last_error[1024];
 
 yl_status set_error(yl_status st, const char* fmt, ...) {
-  char buf[1024];
+  char buf[sizeof(t_last_error)];  // the last message may be among the arguments
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
-  t_last_error = buf;
+  strcpy(t_last_error, buf);
   return st;
 }
 
@@ -110,7 +110,7 @@ using namespace yl;
 
 extern "C" {
 
-const char* yl_last_error_message(void) { return t_last_error.c_str(); }
+const char* yl_last_error_message(void) { return t_last_error; }
 
 const char* yl_version(void) { return "yumelayers_b200 0.1 (sm_100a, tcgen05/TMA)"; }
 
