@@ -200,6 +200,7 @@ struct yl_trainer {
   bool muon_on = false;  // hidden weight matrices are updated by Muon
   yl_muon_config muon{};
   MuonTables muon_tables[2];  // VAE, U-Net
+  bool muon_tables_made = false;
   double prof_ms[kProfClasses] = {}, prof_flops[kProfClasses] = {}, prof_bytes[kProfClasses] = {};
   int prof_launches[kProfClasses] = {};
   double prof_exec[kProfClasses] = {};
@@ -745,9 +746,12 @@ yl_status yl_trainer_set_muon(yl_trainer* tr, const yl_muon_config* cfg) {
            "yl_trainer_set_muon: %d steps (1 to 32)", cfg->steps);
   YL_TRY(check_steps("yl_trainer_set_muon", cfg->steps, nullptr));
   try {
-    if (tr->muon_tables[0].matrices.empty()) {
-      tr->muon_tables[0] = muon_tables_of(*tr->vae, "enc.conv_in", "dec.conv_out");
-      tr->muon_tables[1] = muon_tables_of(*tr->unet, "conv_in", "conv_out");
+    if (!tr->muon_tables_made) {  // both or neither: memory may run out between them
+      MuonTables vae = muon_tables_of(*tr->vae, "enc.conv_in", "dec.conv_out");
+      MuonTables unet = muon_tables_of(*tr->unet, "conv_in", "conv_out");
+      tr->muon_tables[0] = std::move(vae);
+      tr->muon_tables[1] = std::move(unet);
+      tr->muon_tables_made = true;
     }
   } catch (const std::bad_alloc&) {
     return set_error(YL_ERR_OOM, "yl_trainer_set_muon: no host memory");
