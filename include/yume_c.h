@@ -593,6 +593,11 @@ yl_status yl_profile_layered(yl_ctx* ctx, int n, long long plane, int reps, doub
  * normally, so a shorter yl_session_end deadline can run out on the host. */
 yl_status yl_debug_wait_probe(yl_ctx* ctx);
 yl_status yl_debug_spin(yl_ctx* ctx, double seconds);
+/* As if the device had room for clusters of at most this many blocks of the
+ * kernel that keeps short matrices of yl_newton_schulz / yl_muon_multi on the
+ * chip (a power of two up to 16, 0: for none; -1: ask the device again).  Longer
+ * matrices then take smaller clusters or the kernel in memory. */
+yl_status yl_debug_cluster_limit(yl_ctx* ctx, int blocks);
 
 #ifdef __cplusplus
 }

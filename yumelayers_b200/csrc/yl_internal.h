@@ -83,6 +83,8 @@ struct yl_ctx {
   size_t work_bytes = 0;
   cudaEvent_t work_ev = nullptr;
   bool work_used = false;
+  // largest cluster of the on-chip Newton-Schulz kernel; -1: not asked yet
+  int chip_cluster = -1;
 };
 
 namespace yl {

@@ -1808,11 +1808,45 @@ Steps scaled_steps(const Schedule& s) {
   return st;
 }
 
-// Whether a matrix can stay on the chip.
-bool on_chip(const Item& it) {
+// Whether a matrix can stay on the chip, in a cluster of at most `largest` blocks.
+bool on_chip(const Item& it, int largest) {
   const int m = std::min(it.rows, it.cols), n = std::max(it.rows, it.cols);
   const int mb = (m + kBlk - 1) / kBlk, nb = (n + kBlk - 1) / kBlk;
-  return mb <= 2 && nb <= kChipShare * (kChipBlocks / mb);
+  return mb <= 2 && nb <= largest * (kChipBlocks / mb);
+}
+
+cudaLaunchConfig_t chip_config(int matrices, int share, cudaLaunchAttribute* cluster) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(matrices * share);
+  cfg.blockDim = dim3(kChipThreads);
+  cfg.dynamicSmemBytes = kChipSmem;
+  cluster->id = cudaLaunchAttributeClusterDimension;
+  cluster->val.clusterDim.x = share;
+  cluster->val.clusterDim.y = cluster->val.clusterDim.z = 1;
+  cfg.attrs = cluster;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// The largest cluster of the on-chip kernel that this device, or the part of it that
+// the process has, finds room for (0: none); asked once per context.
+int largest_cluster(yl_ctx* ctx) {
+  if (ctx->chip_cluster >= 0) return ctx->chip_cluster;
+  int largest = 0;
+  if (cudaFuncSetAttribute(ns_chip_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChipSmem) ==
+          cudaSuccess &&
+      cudaFuncSetAttribute(ns_chip_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) ==
+          cudaSuccess) {
+    for (int share = kChipShare; share > 0 && largest == 0; share /= 2) {
+      cudaLaunchAttribute cluster;
+      const cudaLaunchConfig_t cfg = chip_config(1, share, &cluster);
+      int room = 0;
+      if (cudaOccupancyMaxActiveClusters(&room, ns_chip_kernel, &cfg) == cudaSuccess && room > 0)
+        largest = share;
+    }
+  }
+  cudaGetLastError();  // sizes that do not fit are no error of this call
+  return ctx->chip_cluster = largest;
 }
 
 // Blocks that the longest of these matrices needs for its share to fit.
@@ -1832,23 +1866,15 @@ yl_status run_chip(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s) {
   for (int k = 0; k < t.count; ++k) longest = std::max({longest, t.it[k].rb, t.it[k].cb});
   // (clusters of 16 find room for only a few of themselves)
   while (share < longest && 2 * share * t.count <= (share < 8 ? 1.0 : 0.5) * ctx->num_sms &&
-         share < kChipShare)
+         2 * share <= largest_cluster(ctx))
     share *= 2;
   YL_CUDA(cudaFuncSetAttribute(ns_chip_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kChipSmem));
   if (share > 8)
     YL_CUDA(cudaFuncSetAttribute(ns_chip_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(t.count * share);
-  cfg.blockDim = dim3(kChipThreads);
-  cfg.dynamicSmemBytes = kChipSmem;
-  cfg.stream = ctx->stream;
   cudaLaunchAttribute cluster;
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = share;
-  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  cfg.attrs = &cluster;
-  cfg.numAttrs = 1;
+  cudaLaunchConfig_t cfg = chip_config(t.count, share, &cluster);
+  cfg.stream = ctx->stream;
   YL_CUDA(cudaLaunchKernelEx(&cfg, ns_chip_kernel, t, scaled_steps(s), u, s.sx[0], share,
                              ctx->dev_err));
   return check_launch("ns_chip_kernel");
@@ -1961,7 +1987,10 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn 
   // than a launch of their own, and so do more clusters than the SMs hold at once
   // (24 of 128 x 1152: 267 us in clusters of 8, 168 us in the steps kernel; 14 of
   // them 138 and 158 us).
-  const bool chip = steps > 0 && std::all_of(items.begin(), items.end(), on_chip) &&
+  const int largest = largest_cluster(ctx);
+  const bool chip = steps > 0 &&
+                    std::all_of(items.begin(), items.end(),
+                                [&](const Item& it) { return on_chip(it, largest); }) &&
                     (long long)items.size() * least_share(items.data(), (int)items.size()) <=
                         ctx->num_sms;
   // Where the tiles of a phase nearly all find an SM at once, the longest chains of
@@ -2279,6 +2308,15 @@ yl_status muon_multi(yl_ctx* ctx, const yl_muon_tensor* table, int count, const 
 using namespace yl;
 
 extern "C" {
+
+yl_status yl_debug_cluster_limit(yl_ctx* ctx, int blocks) {
+  YL_CHECK(ctx, YL_ERR_INVALID, "yl_debug_cluster_limit: ctx is NULL");
+  YL_CHECK(blocks >= -1 && blocks <= kChipShare && (blocks < 1 || (blocks & (blocks - 1)) == 0),
+           YL_ERR_INVALID, "yl_debug_cluster_limit: %d blocks (-1, 0 or a power of two up to %d)",
+           blocks, kChipShare);
+  ctx->chip_cluster = blocks;
+  return YL_OK;
+}
 
 yl_status yl_newton_schulz(yl_ctx* ctx, const yl_ns_matrix* table, int count, int steps,
                            const float* coeffs, float eps) {
