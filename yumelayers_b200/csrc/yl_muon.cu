@@ -382,14 +382,15 @@ __global__ void __launch_bounds__(256)
 // 256 x 2304 ended 7.3e-6 off, with two in GRAM and half a k-block elsewhere 2.1e-6
 // (fp32: 2.0e-6).  So it is one k-block where the tile meets the diagonal, two
 // elsewhere, whose handover then hides behind the tensor core's work.
-// Truncation takes off the same share on average, and scaled_steps puts it back:
-// 2^-22 in GRAM, whose diagonal adds up squares (10 x 4722 6.4e-7 to 5.6e-7, 100 x
-// 6000 1.17e-6 to 1.05e-6), and in SQUARE and UPDATE, by measurement (means over
-// six seeds, in 1e-6; fp32 products in brackets): with more than 64 rows 2^-22 and
-// 2^-23 (100 x 1000 0.77, with 2^-23 twice 0.97, without 1.44 [1.24]; 200 x 3000
-// 1.85, 2.40, 3.74 [2.10]; 512 x 4608 1.49, 1.75 [2.77]); up to 64 rows, where the
-// later products of a k-block add zeros, 2^-23 and nothing (7 x 1131 0.70, with both
-// 0.99 [0.78]; 12 x 1131 0.62, 0.80 [0.88]; 64 x 100 0.53, 0.79 [1.14]).
+// What truncation takes off depends on the data: about 2^-22 of a product of dense
+// operands (eight additions to an accumulator, half a last place of half the sum each),
+// nothing where a sum has one term.  scaled_steps puts half of the former back in GRAM
+// and SQUARE, so that neither kind of matrix has the whole of it left.  Mean errors
+// over eight seeds against those of fp32 products, normal and diagonal matrices, the
+// worst of seven shapes each: on the chip 1.4 and 1.4 (nothing put back 2.0 and 1.9,
+// all of it, 2^-22 in both and 2^-23 in UPDATE, 1.4 and 3.0), in tiles with a shorter
+// side past 128 1.1 and 1.5 (1.3 and 1.5; 0.8 and 3.9), with a shorter one 2.7, at 64 x
+// 1000, and 1.6 (3.3 and 1.5; 1.6 and 3.7).
 //
 // Two forms.  A single block works on 128 x 128 tiles; its MMAs are bound by their
 // reads of shared memory (12 of 128 x 128 a k-block, 8 KB each, take 117 cycles
@@ -432,9 +433,8 @@ struct Form {
 struct Steps {
   int n;
   float g2[kMaxSteps];                                // GRAM: A' = g2 acc
-  // with the shorter side up to one block and longer:
-  float s0[kMaxSteps], s1[kMaxSteps], s2[2][kMaxSteps];  // SQUARE: P' = s0 I + s1 A' + s2 acc
-  float u2[2][kMaxSteps];                                // UPDATE: X' = u2 acc
+  float s0[kMaxSteps], s1[kMaxSteps], s2[kMaxSteps];  // SQUARE: P' = s0 I + s1 A' + s2 acc
+  float u2[kMaxSteps];                                // UPDATE: X' = u2 acc
   // X grows by at most 2^rise[k] before step k, against the bounds of the scales
   int rise[kMaxSteps + 1];
 };
@@ -689,10 +689,9 @@ __global__ void __launch_bounds__(kProductThreads, 1)
             q = ticket_of<PAIR, NARROW>(t, start, count, n);
             // (looked up here and not in the epilogue, which every tile waits for: 512 x 512
             // and 512 x 128 148.4 us, there 150.8)
-            const bool deep = t->it[q.item].mb > 1;
             q.c2 = q.mode == GRAM     ? steps.g2[q.step]
-                   : q.mode == SQUARE ? steps.s2[deep][q.step]
-                                      : steps.u2[deep][q.step];
+                   : q.mode == SQUARE ? steps.s2[q.step]
+                                      : steps.u2[q.step];
             q.s1 = steps.s1[q.step];
             if (const int e = below[q.item]) {
               const Lift lift(steps, e, q.step);
@@ -1341,8 +1340,8 @@ __global__ void __launch_bounds__(kChipThreads, 1)
     float* f = factors + kChipFactors * tid;
     f[0] = lift.gram(steps.g2[tid]);
     f[1] = lift.linear(steps.s1[tid]);
-    f[2] = lift.square(steps.s2[mb > 1][tid]);
-    f[3] = lift.update(steps, below, tid, steps.u2[mb > 1][tid]);
+    f[2] = lift.square(steps.s2[tid]);
+    f[3] = lift.update(steps, below, tid, steps.u2[tid]);
   }
 
   // Block (long, short) of the share: a wide X keeps its row blocks together (the
@@ -1788,22 +1787,20 @@ struct Schedule {
   int rise[kMaxSteps + 1];   // see Steps
 };
 
-// Coefficients with the scales of the pairs folded in, and the share of its sums
-// that the tensor core's truncation takes off each product.
+// Coefficients with the scales of the pairs folded in, and half of what the tensor
+// core's truncation takes off the products of dense matrices.
 Steps scaled_steps(const Schedule& s) {
   Steps st;
   st.n = s.steps;
   std::copy(s.rise, s.rise + s.steps + 1, st.rise);
   for (int k = 0; k < s.steps; ++k) {
     const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
-    st.g2[k] = sa / (sx * sx) * (1.f + 0x1p-22f);
+    const float back = 1.f + 0x1p-23f;
+    st.g2[k] = sa / (sx * sx) * back;
     st.s0[k] = s.q[3 * k] * sp;
     st.s1[k] = s.q[3 * k + 1] * sp / sa;
-    for (int deep = 0; deep < 2; ++deep) {
-      const float s_back = 1.f + (deep ? 0x1p-22f : 0x1p-23f), u_back = deep ? 1.f + 0x1p-23f : 1.f;
-      st.s2[deep][k] = s.q[3 * k + 2] * sp / (sa * sa) * s_back;
-      st.u2[deep][k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx) * u_back;
-    }
+    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa) * back;
+    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx);
   }
   return st;
 }
