@@ -15,7 +15,7 @@ import numpy as np
 import pytest
 import torch
 
-from yumelayers_b200._lib import NsMatrix, call
+from yumelayers_b200._lib import MuonTensor, NsMatrix, call
 
 pytestmark = pytest.mark.gpu
 QUINTIC = (3.4445, -4.7750, 2.0315)
@@ -62,15 +62,25 @@ def plain(x, dtype):
     return z.T if x.shape[0] > x.shape[1] else z
 
 
+def off(a, b):
+    return float((a.double() - b).norm() / b.norm())
+
+
+def orthogonalise(h, xs):
+    ys = [torch.empty_like(x) for x in xs]
+    table = (NsMatrix * len(xs))(*[
+        NsMatrix(x.data_ptr(), y.data_ptr(), *x.shape, x.shape[1], x.shape[1])
+        for x, y in zip(xs, ys)])
+    call("yl_newton_schulz", h, table, len(xs), 5, None, C.c_float(1e-7))
+    return ys
+
+
 def ratio(h, kind, shape):
-    off = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
     ours, fp32 = [], []
     for seed in range(SEEDS):
         x = matrix(kind, *shape, seed)
-        y, want = torch.empty_like(x), plain(x, torch.float64)
-        table = (NsMatrix * 1)(NsMatrix(x.data_ptr(), y.data_ptr(), *shape, shape[1], shape[1]))
-        call("yl_newton_schulz", h, table, 1, 5, None, C.c_float(1e-7))
-        ours.append(off(y, want))
+        want = plain(x, torch.float64)
+        ours.append(off(orthogonalise(h, [x])[0], want))
         fp32.append(off(plain(x, torch.float32), want))
     return float(np.mean(ours) / np.mean(fp32))
 
@@ -87,3 +97,41 @@ def test_short_sides_in_tiles(h, kind, shape):
     """As beside longer matrices: the form that keeps X on the chip is put aside."""
     call("yl_debug_cluster_limit", h, 0)
     assert ratio(h, kind, shape) < 3.0
+
+
+# square and mixed tables; the forms they run in: on the chip, tiles of 64 and 128
+# columns, pairs of blocks
+TABLES = [[(64, 64), (100, 100), (128, 128), (17, 17)], [(300, 300)], [(700, 700), (129, 129)],
+          [(1500, 1500)] * 2, [(1030, 1000)] * 14 + [(64, 700)], [(2560, 2500)] * 2, SHORT + LONG]
+
+
+@pytest.mark.parametrize("shapes", TABLES, ids=lambda t: "%dx%d of %d" % (*t[0], len(t)))
+def test_every_matrix_of_a_table(h, shapes):
+    """Square matrices have small singular values, which magnify what a first step loses in
+    every arithmetic: so against fp32 products of the same matrix, one by one.  Single
+    errors scatter about their mean: twice the bound of the means."""
+    xs = [matrix("normal", *s, k) for k, s in enumerate(shapes)]
+    for x, y in zip(xs, orthogonalise(h, xs)):
+        want = plain(x, torch.float64)
+        bound = 1.6 if min(x.shape) > 128 or max(map(min, shapes)) <= 128 else 3.0
+        assert off(y, want) < 2 * bound * off(plain(x, torch.float32), want)
+
+
+@pytest.mark.parametrize("nesterov", [1, 0])
+def test_muon_step_of_a_table(h, nesterov):
+    """The parameters' own roundings are 1.5 of 2^-24 against their values; weights of zero
+    leave the update alone to be seen."""
+    shapes = SHORT + LONG
+    zero = [torch.zeros(s, device="cuda") for s in shapes]
+    g, m = ([matrix("normal", *s, k + o) for k, s in enumerate(shapes)] for o in (0, 50))
+    m0 = [t.clone() for t in m]
+    table = (MuonTensor * len(shapes))(*[
+        MuonTensor(p.data_ptr(), a.data_ptr(), b.data_ptr(), *s, 1.0)
+        for p, a, b, s in zip(zero, g, m, shapes)])
+    call("yl_muon_multi", h, table, len(shapes), 1.0, 0.5, nesterov, 0.0, 5, None, 1e-7, 1.0, 0.0, 0, None)
+    for p, a, b in zip(zero, g, m0):
+        b = 0.5 * b + a  # exact products; one rounding of the sum, as in the kernel
+        u = a + 0.5 * b if nesterov else b
+        want = -plain(u, torch.float64)
+        bound = 1.6 if min(p.shape) > 128 else 3.0
+        assert off(p, want) < 2 * bound * off(-plain(u, torch.float32), want) + 2.0 ** -23

@@ -287,7 +287,8 @@ __device__ __forceinline__ void split_pair(float v, __half* hi, __half* lo) {
 __global__ void __launch_bounds__(256)
     ns_split_kernel(const Table* __restrict__ t, const __grid_constant__ Update u, float sx,
                     int* __restrict__ below_out) {
-  // from the end, which the pass before has left in L2 (U-Net 439 -> 436 us)
+  // from the end, which the pass before has left in L2 (39 of the U-Net's weights 442 us,
+  // from the start 445)
   const int at0 = gridDim.x - 1 - blockIdx.x, k = find_item(t->blocks, t->count, at0);
   const Item& it = t->it[k];
   const int b = at0 - t->blocks[k];
@@ -1964,9 +1965,9 @@ double step_time(const std::vector<const Item*>& items, int num_sms, bool pair) 
 // The tables of a call: matrices for pairs of blocks first, then the others.
 // A pair does twice the products per shared-memory read, but has half as many and
 // larger tiles to share among the SMs, so it pays where those stay full: 4096 x 4096
-// 3.4 ms in pairs and 3.9 alone, 2560 x 2560 0.97 and 1.03, 8 of 1024 x 1024 0.53
-// and 0.56, but 4 of them 0.53 and 0.38, 2048 x 2048 0.59 and 0.52, 1024 x 8192
-// 0.68 and 0.61, 16 of 600 x 2400, which 256 x 256 tiles pad, 1.04 and 0.88.  (The estimates are within some
+// 3.76 ms in pairs and 4.30 alone, 2560 x 2560 1.07 and 1.17, 8 of 1024 x 1024 0.59
+// and 0.63, but 4 of them 0.41 and 0.34, 2048 x 2048 0.63 and 0.60, 1024 x 8192
+// 0.61 and 0.57, 16 of 600 x 2400, which 256 x 256 tiles pad, 1.22 and 1.05.  (The estimates are within some
 // 6% of that: pairs have to promise as much.)  Sides under kPairSide are mostly
 // padding.  Where other matrices remain, they take a launch of their own.
 template <class Fn>
@@ -1992,7 +1993,7 @@ yl_status for_tables(yl_ctx* ctx, const std::vector<Item>& items, int steps, Fn 
                         ctx->num_sms;
   // Where the tiles of a phase nearly all find an SM at once, the longest chains of
   // products come first: what has to wait is then short (five odd shapes 245 -> 233
-  // us).  Longer tables keep the caller's order (the U-Net's 39 matrices 436 us,
+  // us).  Longer tables keep the caller's order (39 of the U-Net's 436 us,
   // sorted 446).
   std::vector<const Item*> order;
   double all = 0, longest = 0;
