@@ -340,7 +340,8 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
  * grows into the result, coefficients that let small singular values grow by more
  * than 2^17 against the largest are YL_ERR_UNSUPPORTED, as are those that let one
  * grow past 4: the default takes 9 steps, (1.5, -0.5, 0) 29, and any 7 steps within
- * the limit of 4 pass.  Norms far below eps keep their bits.  Sides go to 65536.  y may be x itself (same
+ * the limit of 4 pass.  Norms far below eps keep their bits, and so does
+ * what steps with small coefficients shrink.  Sides go to 65536.  y may be x itself (same
  * stride); any other overlap between a result and another matrix of the table
  * is YL_ERR_INVALID.  An empty matrix is skipped, a zero matrix gives zeros, and
  * one with a NaN or an infinity gives NaN and leaves the others alone.  Equal

@@ -109,6 +109,22 @@ def test_small_norms_under_steps_that_shrink_and_grow(h):
             assert rel(y, ns64(x, 5, coeffs=q)) < TOL
 
 
+@pytest.mark.parametrize("shape", [(96, 160), (160, 96), (257, 400)])
+@pytest.mark.parametrize("coeffs", [
+    [(1e-9, 0.0, 0.0)], [(1e-9, 0.0, 0.0), (1.0, 0.0, 0.0)], [(1e-4, 0.0, 0.0)] * 4 + [(2.0, -1.0, 0.5)],
+    [(0.0, 1e-6, 0.0), (3.0, 0.0, 0.0)], [(0.0, 0.0, 1e-3), (0.5, 0.0, 1.0), (2.0, 0.0, 0.0)],
+    [(1e-12, 1e-12, -1e-12), (1e-12, 0.0, 0.0)], [(0.0, 0.0, 0.0), (1.0, 0.0, 0.0)]])
+def test_steps_that_shrink(h, shape, coeffs):
+    """Whatever the steps take off, the scales follow."""
+    x = normal(13, *shape)
+    y, = run(h, [x], steps=len(coeffs), coeffs=coeffs)
+    z = ns64(x, len(coeffs), coeffs=[[float(np.float32(v)) for v in q] for q in coeffs])
+    if not any(coeffs[0]):
+        assert not y.any()
+    else:
+        assert rel(y, z) < TOL
+
+
 @pytest.mark.parametrize("shape", [(96, 160), (160, 96), (300, 280), (512, 1024)])
 @pytest.mark.parametrize("small", [1e-3, 1e-6, 1e-8, 1e-10])
 @pytest.mark.parametrize("steps", [5, 9])

@@ -1783,8 +1783,8 @@ size_t place(Table* t, int num_sms, char* ws) {
 struct Schedule {
   int steps;
   float q[3 * kMaxSteps];    // coefficients
-  float sx[kMaxSteps + 1];   // scales of X before each step and at the end
-  float sa[kMaxSteps], sp[kMaxSteps];
+  double sx[kMaxSteps + 1];  // scales of X before each step and at the end, powers of two
+  double sa[kMaxSteps], sp[kMaxSteps];
   int rise[kMaxSteps + 1];   // see Steps
 };
 
@@ -1795,13 +1795,12 @@ Steps scaled_steps(const Schedule& s) {
   st.n = s.steps;
   std::copy(s.rise, s.rise + s.steps + 1, st.rise);
   for (int k = 0; k < s.steps; ++k) {
-    const float sx = s.sx[k], sa = s.sa[k], sp = s.sp[k];
-    const float back = 1.f + 0x1p-23f;
-    st.g2[k] = sa / (sx * sx) * back;
-    st.s0[k] = s.q[3 * k] * sp;
-    st.s1[k] = s.q[3 * k + 1] * sp / sa;
-    st.s2[k] = s.q[3 * k + 2] * sp / (sa * sa) * back;
-    st.u2[k] = (k + 1 == s.steps ? 1.f : s.sx[k + 1]) / (sp * sx);
+    const double sx = s.sx[k], sa = s.sa[k], sp = s.sp[k], back = 1.0 + 0x1p-23;
+    st.g2[k] = (float)(sa / (sx * sx) * back);
+    st.s0[k] = (float)(s.q[3 * k] * sp);
+    st.s1[k] = (float)(s.q[3 * k + 1] * sp / sa);
+    st.s2[k] = (float)(s.q[3 * k + 2] * sp / (sa * sa) * back);
+    st.u2[k] = (float)((k + 1 == s.steps ? 1.0 : s.sx[k + 1]) / (sp * sx));
   }
   return st;
 }
@@ -1873,7 +1872,7 @@ yl_status run_chip(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s) {
   cudaLaunchAttribute cluster;
   cudaLaunchConfig_t cfg = chip_config(t.count, share, &cluster);
   cfg.stream = ctx->stream;
-  YL_CUDA(cudaLaunchKernelEx(&cfg, ns_chip_kernel, t, scaled_steps(s), u, s.sx[0], share,
+  YL_CUDA(cudaLaunchKernelEx(&cfg, ns_chip_kernel, t, scaled_steps(s), u, (float)s.sx[0], share,
                              ctx->dev_err));
   return check_launch("ns_chip_kernel");
 }
@@ -1901,7 +1900,7 @@ yl_status run_table(yl_ctx* ctx, Table& t, const Update& u, const Schedule& s, c
     ns_direct_kernel<<<t.chunks[t.count], 256, 0, ctx->stream>>>(dt, u);
     return check_launch("ns_direct_kernel");
   }
-  ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, s.sx[0], dt->below);
+  ns_split_kernel<<<t.blocks[t.count], 256, 0, ctx->stream>>>(dt, u, (float)s.sx[0], dt->below);
   YL_TRY(check_launch("ns_split_kernel"));
   const Steps st = scaled_steps(s);
   // More blocks than a phase has tickets: they hold tickets of the phases to come,
@@ -2046,11 +2045,13 @@ size_t norm_parts(long long n) { return (size_t)((n + kNormChunk - 1) / kNormChu
 constexpr float kQuintic[3] = {3.4445f, -4.7750f, 2.0315f};
 
 // Largest power of two that keeps values up to `top` under fp16's 65504 with
-// room for rounding.
-float scale_for(double top) {
+// room for rounding.  (What steps have shrunk below kMinTop is at the end of fp32's
+// range.)
+constexpr double kMinTop = 0x1p-100;
+double scale_for(double top) {
   int e;
-  std::frexp(32768.0 / std::max(top, 1e-3), &e);
-  return (float)std::ldexp(1.0, std::min(e - 1, 20));
+  std::frexp(32768.0 / std::max(top, kMinTop), &e);
+  return std::ldexp(1.0, e - 1);
 }
 
 // How far the steps may let a small singular value grow against the largest one.
@@ -2105,7 +2106,7 @@ yl_status plan_steps(const char* who, int steps, const float* given, Schedule* s
     auto gain = [&](double sq) { return std::fabs(a + sq * (b + sq * c)); };
     double most = std::max(gain(0.0), gain(top * top));
     if (c != 0.0) most = std::max(most, gain(std::min(top * top, std::max(0.0, -b / (2 * c)))));
-    const double bound = std::max(next, 1e-3);  // what the next scale allows for
+    const double bound = std::max(next, kMinTop);  // what the next scale allows for
     const double up = most * top / bound;
     s_out->rise[s + 1] = s_out->rise[s] + (up > 1.0 ? (int)std::ceil(std::log2(up)) : 0);
     growth = std::max(growth, 1.0) * up;
