@@ -334,16 +334,16 @@ yl_status yl_layernorm_bwd(yl_ctx* ctx, const float* x, long long ldx, const flo
  * (a, b, c) per step, or NULL for (3.4445, -4.7750, 2.0315) in every step.
  * Against its norm a result is about as accurate as with fp32 products (mean errors
  * 0.25 to 1.5 times theirs, up to 2.7 times for sides of up to 128 beside longer
- * matrices): X and the m x m matrices are held to 22 bits, sums are fp32.  Unlike fp32 numbers those 22 bits
- * end at 2^-17 of the largest value X can have, and what is under 2^-40 of it is
- * lost: rows 1e-10 of the others come out as noise or zero.  So that nothing lost
- * grows into the result, coefficients that let small singular values grow by more
- * than 2^17 against the largest are YL_ERR_UNSUPPORTED, as are those that let one
- * grow past 4: the default takes 9 steps, (1.5, -0.5, 0) 29, and any 7 steps within
- * the limit of 4 pass.  Norms far below eps keep their bits, and so does
- * what steps with small coefficients shrink.  Sides go to 65536.  y may be x itself (same
- * stride); any other overlap between a result and another matrix of the table
- * is YL_ERR_INVALID.  An empty matrix is skipped, a zero matrix gives zeros, and
+ * matrices): X and the m x m matrices are held to 22 bits, sums are fp32.  Unlike
+ * fp32 numbers those 22 bits end at 2^-17 of the largest value X can have, and what
+ * is under 2^-40 of it is lost: rows 1e-10 of the others come out as noise or zero.
+ * So that nothing lost grows into the result, coefficients that let small singular
+ * values grow by more than 2^17 against the largest are YL_ERR_UNSUPPORTED, as are
+ * those that let one grow past 4: the default takes 9 steps, (1.5, -0.5, 0) 29, and
+ * any 7 steps within the limit of 4 pass.  Norms far below eps keep their bits, and
+ * so does what steps with small coefficients shrink.  Sides go to 65536.  y may be x
+ * itself (same stride); any other overlap between a result and another matrix of the
+ * table is YL_ERR_INVALID.  An empty matrix is skipped, a zero matrix gives zeros, and
  * one with a NaN or an infinity gives NaN and leaves the others alone.  Equal
  * calls give equal bits; a matrix in another table may come out with other
  * roundings.  No counterpart in the reference. */
